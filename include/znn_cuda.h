@@ -256,6 +256,54 @@ int znn_softmax_xent_bwd_u8(const float* probs, const uint8_t* targets, float* d
  *     overlap on the GPU (different streams, no dependency) race on it; serialise them. */
 int znn_softmax_xent_fwd_static(const float* logits, const int32_t* targets, float* probs, float* loss,
                                 int M, int N, void* cuda_stream);
+/* ---- fine-tuning losses on a language model's logits (no counterpart in the reference, whose only loss is
+ *      SoftmaxCrossEntropy).  Conventions of the four calls:
+ *   - row i of the logits starts at logits + i * ld (ld >= N floats; any alignment).  inv_temp > 0 is 1 / temperature;
+ *     with x = row i, xm = max_j x_j and d_j = inv_temp * (x_j - xm):  s = sum_j exp(d_j), p_j = exp(d_j) / s,
+ *     logp = d_t - log s for the target t, entropy = -sum_j p_j log p_j (a term with p_j = 0 counts as 0);
+ *   - targets[i] < 0 leaves the row out (prompt, padding): its logits and its entries of the other inputs are not used
+ *     (they may hold NaN), its outputs are 0 and it gets no gradient.  targets[i] >= N is never used as an index: the
+ *     row's logp (and a loss it is part of) becomes NaN, it gets no gradient and ZNN_DEV_BAD_INDEX is set;
+ *   - a logit of -inf switches its column off (p_j = 0, gradient 0).  A row of -inf alone has logp = -inf, entropy 0 and
+ *     gradient 0; a row that holds NaN or +inf gives NaN;
+ *   - sums of a row are kept in fp32 per thread and joined in a fixed order, per-row scalars and sums over rows in fp64:
+ *     results do not depend on timing.  Nothing is kept in the library between calls.
+ *
+ * znn_token_logprob_fwd: logp[M], entropy[M] (may be NULL) and stats[M][2] = (xm, s) (may be NULL), which the backward
+ * needs; log sum exp = inv_temp * xm + log s.  Rows left out: stats = (0, 0).
+ * znn_token_logprob_bwd, from dlogp and dentropy (NULL = no such gradient; then entropy may be NULL too):
+ *   dlogits_j (+)= inv_temp * (dlogp * ([j = t] - p_j) - dentropy * p_j * (log p_j + entropy)).
+ * accumulate = 1 adds (rows left out stay as they are), 0 stores (rows left out become 0).  With accumulate = 0 dlogits
+ * may be the logits' own buffer (ld_d == ld). */
+int znn_token_logprob_fwd(const float* logits, long long ld, const int32_t* targets, float inv_temp, float* logp, float* entropy,
+                          float* stats, int M, int N);
+int znn_token_logprob_bwd(const float* logits, long long ld, const int32_t* targets, float inv_temp, const float* stats,
+                          const float* entropy, const float* dlogp, const float* dentropy, float* dlogits, long long ld_d,
+                          int accumulate, int M, int N);
+/* Clipped policy loss with a KL term and an entropy bonus, and its gradient, in one pass over the logits.  Per row
+ *   r = exp(logp - old_logp),  q = ref_logp - logp,
+ *   l = -min(r * A, clip(r, 1 - clip_low, 1 + clip_high) * A) + kl_coef * (exp(q) - q - 1) - entropy_coef * entropy
+ * with A = advantages[i] (A = 0: the first term and its gradient are 0 whatever r is).  On a border r counts as inside.
+ *   loss[0] = sum_i w_i l_i,  w_i = weights[i], or 1 / (number of rows not left out) where weights is NULL (0 when there is
+ *   none); a row of weight 0 is left out.  loss[1] = the number of rows not left out.
+ * token_loss[M] = l; logp[M] and entropy[M] (either may be NULL) as above; dlogits = d loss[0] / d logits, stored, NULL = the
+ * loss alone; it may be the logits' own buffer (ld_d == ld).  ref_logp may be NULL where kl_coef is 0. */
+int znn_policy_loss(const float* logits, long long ld, const int32_t* targets, float inv_temp, const float* old_logp,
+                    const float* ref_logp, const float* advantages, const float* weights, float clip_low, float clip_high,
+                    float kl_coef, float entropy_coef, float* loss, float* token_loss, float* logp, float* entropy,
+                    float* dlogits, long long ld_d, int M, int N);
+/* Preference loss on P pairs of sequences, from the log-probabilities of their tokens.  Sequence s holds the rows
+ * seq_offsets[s] <= i < seq_offsets[s + 1] (2P + 1 device int32, ascending, within 0 .. M); sequence 2p is the preferred one
+ * of pair p, 2p + 1 the other; a sequence may be empty.  targets (may be NULL) leaves rows out as above.
+ *   rewards[s] = beta * sum_i (logp_i - ref_logp_i) (ref_logp may be NULL = 0), divided by the number of its rows not left
+ *   out where length_normalize = 1 (0 for none);  m = rewards[2p] - rewards[2p + 1] - margin;
+ *   pair_loss[p] = -(1 - label_smoothing) * log sigmoid(m) - label_smoothing * log sigmoid(-m);  loss[0] = mean of pair_loss.
+ * dlogp (may be NULL) = d loss[0] / d logp for the rows of the sequences, 0 for those left out, which
+ * znn_token_logprob_bwd takes; rows behind the last sequence stay as they were.  A pair whose offsets are not ascending within
+ * 0 .. M has rewards and loss NaN, its rows are neither read nor written, and ZNN_DEV_BAD_INDEX is set. */
+int znn_preference_loss(const float* logp, const float* ref_logp, const int32_t* targets, const int32_t* seq_offsets, float beta,
+                        float label_smoothing, float margin, int length_normalize, float* loss, float* pair_loss, float* rewards,
+                        float* dlogp, int P, int M);
 /* Softmax over the last dimension: :435-461 / :1054-1076 */
 int znn_softmax_fwd(const float* A, float* C, size_t rows, int D);
 int znn_softmax_bwd(const float* Y, const float* dY, float* dA, size_t rows, int D);
@@ -319,6 +367,26 @@ int znn_sgd_step(float* w, const float* g, float* v, float lr, float momentum, f
  * lr*sqrt(1-beta2^t)/(1-beta1^t) is computed on the host in fp32 as the reference does; m, v are the moment buffers. */
 int znn_adam_step(float* w, const float* g, float* m, float* v, float lr, float beta1, float beta2, float eps, float t,
                   float grad_scale, size_t n);
+/* Clipping by the global norm of a set of gradient tensors (an addition).  grads (HOST array of n device pointers, which may
+ * be unaligned to 16 bytes) and counts (host array, floats per tensor; 0 is allowed) describe the set; both are read during
+ * the call.
+ * znn_grad_norm: result[0] = |grad_scale| * sqrt(sum of all squares), result[1] = the factor that brings it to max_norm:
+ *   max_norm / norm where norm > max_norm, 1 otherwise, 0 where the norm is not finite.  Squares are summed in fp64 in a fixed
+ *   order: no overflow or underflow for any finite fp32 gradients, and the same bits every time.  max_norm = INFINITY: the
+ *   norm alone.  `result` is ZNN_GRAD_NORM_FLOATS floats of device memory, 16-byte aligned; what follows the two values is the
+ *   call's workspace.  Give calls that may run at the same time (two streams, two captured graphs) a result each.
+ * znn_clip_grads: grads *= result[1], in place; a factor of 1 or 0 leaves them untouched.
+ * znn_sgd_step_clipped, znn_adam_step_clipped: znn_sgd_step / znn_adam_step with the gradient multiplied by
+ *   grad_scale * result[1], read on the device: no pass over the gradients for the clipping and nothing for the host to wait
+ *   for.  A factor of 0 (the norm was not finite) skips the step: w, v and m stay as they are.  With a factor of 1 the result is
+ *   that of the unclipped step, bit for bit. */
+#define ZNN_GRAD_NORM_FLOATS 4096
+int znn_grad_norm(const float** grads, const size_t* counts, int n, float grad_scale, float max_norm, float* result);
+int znn_clip_grads(float** grads, const size_t* counts, int n, const float* result);
+int znn_sgd_step_clipped(float* w, const float* g, float* v, float lr, float momentum, float grad_scale, const float* result,
+                         size_t n);
+int znn_adam_step_clipped(float* w, const float* g, float* m, float* v, float lr, float beta1, float beta2, float eps, float t,
+                          float grad_scale, const float* result, size_t n);
 /* Input pipeline on the device.
  * znn_pixels_to_unit: IDX pixel bytes -> fp32 pixel / 255.0, the conversion of loadImages (src/dataset.zig:53-63).
  * znn_batch_gather: the copy loop of DataLoader.nextInto (src/dataset.zig:211-220): for j < batch,

@@ -120,6 +120,10 @@ pub extern fn znn_softmax_xent_fwd_u8(logits: ?[*]const f32, targets: ?[*]const 
 pub extern fn znn_softmax_xent_bwd(probs: ?[*]const f32, targets: ?[*]const i32, dlogits: ?[*]f32, M: c_int, N: c_int) c_int;
 pub extern fn znn_softmax_xent_bwd_u8(probs: ?[*]const f32, targets: ?[*]const u8, dlogits: ?[*]f32, M: c_int, N: c_int) c_int;
 pub extern fn znn_softmax_xent_fwd_static(logits: ?[*]const f32, targets: ?[*]const i32, probs: ?[*]f32, loss: ?[*]f32, M: c_int, N: c_int, cuda_stream: ?*anyopaque) c_int;
+pub extern fn znn_token_logprob_fwd(logits: ?[*]const f32, ld: c_longlong, targets: ?[*]const i32, inv_temp: f32, logp: ?[*]f32, entropy: ?[*]f32, stats: ?[*]f32, M: c_int, N: c_int) c_int;
+pub extern fn znn_token_logprob_bwd(logits: ?[*]const f32, ld: c_longlong, targets: ?[*]const i32, inv_temp: f32, stats: ?[*]const f32, entropy: ?[*]const f32, dlogp: ?[*]const f32, dentropy: ?[*]const f32, dlogits: ?[*]f32, ld_d: c_longlong, accumulate: c_int, M: c_int, N: c_int) c_int;
+pub extern fn znn_policy_loss(logits: ?[*]const f32, ld: c_longlong, targets: ?[*]const i32, inv_temp: f32, old_logp: ?[*]const f32, ref_logp: ?[*]const f32, advantages: ?[*]const f32, weights: ?[*]const f32, clip_low: f32, clip_high: f32, kl_coef: f32, entropy_coef: f32, loss: ?[*]f32, token_loss: ?[*]f32, logp: ?[*]f32, entropy: ?[*]f32, dlogits: ?[*]f32, ld_d: c_longlong, M: c_int, N: c_int) c_int;
+pub extern fn znn_preference_loss(logp: ?[*]const f32, ref_logp: ?[*]const f32, targets: ?[*]const i32, seq_offsets: ?[*]const i32, beta: f32, label_smoothing: f32, margin: f32, length_normalize: c_int, loss: ?[*]f32, pair_loss: ?[*]f32, rewards: ?[*]f32, dlogp: ?[*]f32, P: c_int, M: c_int) c_int;
 pub extern fn znn_softmax_fwd(A: ?[*]const f32, C: ?[*]f32, rows: usize, D: c_int) c_int;
 pub extern fn znn_softmax_bwd(Y: ?[*]const f32, dY: ?[*]const f32, dA: ?[*]f32, rows: usize, D: c_int) c_int;
 pub extern fn znn_causal_softmax_fwd(S: ?[*]const f32, scale: f32, P: ?[*]f32, nslices: c_int, T: c_int) c_int;
@@ -147,6 +151,10 @@ pub extern fn znn_argmax(A: ?[*]const f32, out: ?[*]f32, M: c_int, N: c_int, dim
 pub extern fn znn_accuracy_u8(logits: ?[*]const f32, labels: ?[*]const u8, M: c_int, N: c_int, acc: ?[*]f32) c_int;
 pub extern fn znn_sgd_step(w: ?[*]f32, g: ?[*]const f32, v: ?[*]f32, lr: f32, momentum: f32, grad_scale: f32, n: usize) c_int;
 pub extern fn znn_adam_step(w: ?[*]f32, g: ?[*]const f32, m: ?[*]f32, v: ?[*]f32, lr: f32, beta1: f32, beta2: f32, eps: f32, t: f32, grad_scale: f32, n: usize) c_int;
+pub extern fn znn_grad_norm(grads: *?[*]f32, counts: ?[*]const usize, n: c_int, grad_scale: f32, max_norm: f32, result: ?[*]f32) c_int;
+pub extern fn znn_clip_grads(grads: *?[*]f32, counts: ?[*]const usize, n: c_int, result: ?[*]const f32) c_int;
+pub extern fn znn_sgd_step_clipped(w: ?[*]f32, g: ?[*]const f32, v: ?[*]f32, lr: f32, momentum: f32, grad_scale: f32, result: ?[*]const f32, n: usize) c_int;
+pub extern fn znn_adam_step_clipped(w: ?[*]f32, g: ?[*]const f32, m: ?[*]f32, v: ?[*]f32, lr: f32, beta1: f32, beta2: f32, eps: f32, t: f32, grad_scale: f32, result: ?[*]const f32, n: usize) c_int;
 pub extern fn znn_pixels_to_unit(pixels: ?[*]const u8, out: ?[*]f32, n: usize) c_int;
 pub extern fn znn_batch_gather(images: ?[*]const f32, labels: ?[*]const u8, indices: ?[*]const i32, x_dest: ?[*]f32, y_dest: ?[*]u8, batch: c_int, input_dim: c_int, num_samples: usize) c_int;
 pub extern fn znn_fill(dst: ?[*]f32, value: f32, n: usize) c_int;

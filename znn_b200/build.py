@@ -28,6 +28,8 @@ SOURCES = [
     ("rowops.cu", ["-fmad=false"]),
     ("conv.cu", ["-fmad=false"]),
     ("conv_tc.cu", []),
+    ("policy.cu", []),
+    ("gradclip.cu", ["-fmad=false"]),
     ("dp.cu", []),
     ("host/graph.cpp", []),
     ("host/nn.cpp", []),

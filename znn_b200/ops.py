@@ -618,3 +618,127 @@ def sgd_step(w, g, v, lr, momentum, grad_scale=1.0):
     dw.into(w)
     if v is not None:
         dv.into(v)
+
+
+# ---- fine-tuning losses and clipping by the global gradient norm (include/znn_cuda.h) ----
+def token_logprob_fwd(logits, targets, inv_temp=1.0, want_entropy=True):
+    """(logp[M], entropy[M] or None, stats[M, 2]) of the target tokens; a negative target leaves its row out."""
+    _ensure()
+    logits = _f(logits)
+    M, N = logits.shape
+    x, t = _up(logits), _up(targets, np.int32)
+    lp, st = DevBuf(M * 4), DevBuf(M * 8)
+    en = DevBuf(M * 4) if want_entropy else None
+    lib().call("znn_token_logprob_fwd", x.ptr, N, t.ptr, inv_temp, lp.ptr, _ptr(en), st.ptr, M, N)
+    return lp.to_host((M,)), en.to_host((M,)) if want_entropy else None, st.to_host((M, 2))
+
+
+def token_logprob_bwd(logits, targets, stats, dlogp, dlogits=None, entropy=None, dentropy=None, inv_temp=1.0):
+    """Gradient of the logits; added to dlogits in place where that is given, returned as a fresh array otherwise."""
+    _ensure()
+    logits = _f(logits)
+    M, N = logits.shape
+    x, t, st, g = _up(logits), _up(targets, np.int32), _up(stats), _up(dlogp)
+    en, h = _up(entropy), _up(dentropy)
+    out = _up(dlogits) if dlogits is not None else DevBuf(logits.nbytes)
+    lib().call("znn_token_logprob_bwd", x.ptr, N, t.ptr, inv_temp, st.ptr, _ptr(en), _ptr(g), _ptr(h), out.ptr, N,
+               int(dlogits is not None), M, N)
+    if dlogits is None:
+        return out.to_host((M, N))
+    out.into(dlogits)
+    return dlogits
+
+
+def policy_loss(logits, targets, old_logp, advantages, ref_logp=None, weights=None, clip=(0.2, 0.2), kl_coef=0.0,
+                entropy_coef=0.0, inv_temp=1.0, want_grad=True):
+    """Clipped policy loss: dict with loss, rows, token_loss[M], logp[M], entropy[M] and dlogits[M, N] (None without want_grad)."""
+    _ensure()
+    logits = _f(logits)
+    M, N = logits.shape
+    x, t, old, adv = _up(logits), _up(targets, np.int32), _up(old_logp), _up(advantages)
+    ref, w = _up(ref_logp), _up(weights)
+    loss, tl, lp, en = DevBuf(8), DevBuf(M * 4), DevBuf(M * 4), DevBuf(M * 4)
+    dx = DevBuf(logits.nbytes) if want_grad else None
+    lib().call("znn_policy_loss", x.ptr, N, t.ptr, inv_temp, old.ptr, _ptr(ref), adv.ptr, _ptr(w), clip[0], clip[1], kl_coef,
+               entropy_coef, loss.ptr, tl.ptr, lp.ptr, en.ptr, _ptr(dx), N, M, N)
+    both = loss.to_host((2,))
+    return {"loss": both[0], "rows": int(both[1]), "token_loss": tl.to_host((M,)), "logp": lp.to_host((M,)),
+            "entropy": en.to_host((M,)), "dlogits": dx.to_host((M, N)) if want_grad else None}
+
+
+def preference_loss(logp, seq_offsets, ref_logp=None, targets=None, beta=0.1, label_smoothing=0.0, margin=0.0,
+                    length_normalize=False, dlogp=None):
+    """Preference loss on the pairs of sequences that seq_offsets (2P + 1 row numbers) cut out of logp: dict with loss,
+    pair_loss[P], rewards[2P] and dlogp[M] (rows of no sequence keep what `dlogp` gives them, 0 by default)."""
+    _ensure()
+    logp = _f(logp)
+    M, P = logp.size, (len(seq_offsets) - 1) // 2
+    lp, ref, t, off = _up(logp), _up(ref_logp), _up(targets, np.int32), _up(seq_offsets, np.int32)
+    loss, pl, rw = DevBuf(4), DevBuf(P * 4), DevBuf(2 * P * 4)
+    g = _up(np.zeros(M, np.float32) if dlogp is None else dlogp)
+    lib().call("znn_preference_loss", lp.ptr, _ptr(ref), _ptr(t), off.ptr, beta, label_smoothing, margin, int(length_normalize),
+               loss.ptr, pl.ptr, rw.ptr, g.ptr, P, M)
+    return {"loss": loss.to_host((1,))[0], "pair_loss": pl.to_host((P,)), "rewards": rw.to_host((2 * P,)), "dlogp": g.to_host((M,))}
+
+
+GRAD_NORM_FLOATS = 4096
+
+
+def _grad_set(arrays):
+    bufs = [_up(a) for a in arrays]
+    ptrs = (C.c_void_p * max(1, len(bufs)))(*[b.ptr for b in bufs])
+    counts = (C.c_size_t * max(1, len(bufs)))(*[a.size for a in arrays])
+    return bufs, ptrs, counts
+
+
+def grad_norm(grads, max_norm=float("inf"), grad_scale=1.0):
+    """(global norm, clip factor) of a list of gradient arrays."""
+    _ensure()
+    bufs, ptrs, counts = _grad_set(grads)
+    res = DevBuf(GRAD_NORM_FLOATS * 4)
+    lib().call("znn_grad_norm", ptrs, counts, len(bufs), grad_scale, max_norm, res.ptr)
+    both = res.to_host((2,))
+    return both[0], both[1]
+
+
+def clip_grads(grads, max_norm, grad_scale=1.0):
+    """Clips the gradient arrays in place by their global norm; returns (norm before, factor)."""
+    _ensure()
+    bufs, ptrs, counts = _grad_set(grads)
+    res = DevBuf(GRAD_NORM_FLOATS * 4)
+    lib().call("znn_grad_norm", ptrs, counts, len(bufs), grad_scale, max_norm, res.ptr)
+    lib().call("znn_clip_grads", ptrs, counts, len(bufs), res.ptr)
+    for a, b in zip(grads, bufs):
+        b.into(a)
+    both = res.to_host((2,))
+    return both[0], both[1]
+
+
+def sgd_step_clipped(w, g, v, lr, momentum, max_norm, grad_scale=1.0):
+    """One SGD step on w (and v), in place, with the gradient clipped to max_norm; returns (norm, factor)."""
+    _ensure()
+    dw, dv = _up(w), _up(v)
+    bufs, ptrs, counts = _grad_set([g])
+    res = DevBuf(GRAD_NORM_FLOATS * 4)
+    lib().call("znn_grad_norm", ptrs, counts, 1, grad_scale, max_norm, res.ptr)
+    lib().call("znn_sgd_step_clipped", dw.ptr, bufs[0].ptr, _ptr(dv), lr, momentum, grad_scale, res.ptr, w.size)
+    dw.into(w)
+    if v is not None:
+        dv.into(v)
+    both = res.to_host((2,))
+    return both[0], both[1]
+
+
+def adam_step_clipped(w, g, m, v, lr, beta1, beta2, eps, t, max_norm, grad_scale=1.0):
+    """One Adam step on w, m, v, in place, with the gradient clipped to max_norm; returns (norm, factor)."""
+    _ensure()
+    dw, dm, dv = _up(w), _up(m), _up(v)
+    bufs, ptrs, counts = _grad_set([g])
+    res = DevBuf(GRAD_NORM_FLOATS * 4)
+    lib().call("znn_grad_norm", ptrs, counts, 1, grad_scale, max_norm, res.ptr)
+    lib().call("znn_adam_step_clipped", dw.ptr, bufs[0].ptr, dm.ptr, dv.ptr, lr, beta1, beta2, eps, t, grad_scale, res.ptr, w.size)
+    dw.into(w)
+    dm.into(m)
+    dv.into(v)
+    both = res.to_host((2,))
+    return both[0], both[1]
