@@ -2,49 +2,78 @@
 // with its gradient, the preference loss on pairs of sequences.  Formulas: include/znn_cuda.h.
 //
 // Every operator is bound by HBM: 10 to 20 operations per logit against 4 to 12 bytes.
+#include <cooperative_groups.h>
 #include <math.h>
 #include <math_constants.h>
 
+#include <algorithm>
+
 #include "common.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace znn {
 
-// What a row of logits sums to, relative to the largest logit mx seen: s = sum exp(d), u = sum d exp(d) with
-// d = it * (x - mx).  The entropy is log s - u / s.
-struct RowSums {
-    float mx, s, u;
-};
+constexpr unsigned kAllLanes = 0xffffffffu;
 
-// d for one logit: -inf stays -inf, and a row of -inf alone (mx = -inf) is measured from 0 so that no inf - inf arises
-__device__ __forceinline__ float base_of(float mx) { return mx == -CUDART_INF_F ? 0.0f : mx; }
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+// Where exp2() is 0 in fp32 whatever comes after the point.  Exponents are clamped to it, so that no 0 * inf arises.
+constexpr float kNothing = -150.0f;
 
-// sums of two disjoint parts of a row; an empty part (s = 0) changes nothing, a NaN stays
-__device__ __forceinline__ RowSums join(const RowSums& a, const RowSums& b, float it)
+// 2^x as the special-function unit gives it (2 units in the last place, subnormal results 0).  The exponentials of this file
+// are 2^t with t = (x - xm) * inv_temp * log2(e): a subtraction, a product and this, where expf() would take twice as many
+// operations after the same two roundings, and the kernels here are as near to the issue rate as to the memory's.
+__device__ __forceinline__ float exp2_fast(float x)
 {
-    if (b.s == 0.0f) return a;
-    if (a.s == 0.0f) return b;
-    RowSums r;
-    r.mx = fmaxf(a.mx, b.mx);
-    const float da = (base_of(a.mx) - base_of(r.mx)) * it, db = (base_of(b.mx) - base_of(r.mx)) * it;
-    const float fa = expf(da), fb = expf(db);
-    r.s = a.s * fa + b.s * fb;
-    // a part that is too far below to count adds nothing here, even where da * a.s overflows (logits of the type's lowest value)
-    r.u = (fa > 0.0f ? fa * (a.u + da * a.s) : 0.0f) + (fb > 0.0f ? fb * (b.u + db * b.s) : 0.0f);
-    return r;
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 
-__device__ __forceinline__ RowSums warp_join(RowSums v, float it)
+// the larger of the two, and NaN where there is one (fmaxf() would drop it)
+__device__ __forceinline__ float max_nan(float a, float b)
+{
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
+
+// What a row of logits (or a part of one) sums to, relative to the largest logit mx seen, with t = (x - mx) * inv_temp * log2(e):
+// `ties` logits equal mx, s = sum of 2^t over the others, u = sum of t 2^t.  The row's sum is ties + s.  The ones are kept apart
+// because a row that is nearly certain has s << 1, and its log-probability -log(1 + s) is only as exact as s is: 1 + s in fp32
+// would leave an error of 6e-8 / s.
+struct __align__(16) RowSums {
+    float mx, ties, s, u;
+};
+
+// A row of -inf alone (mx = -inf) is measured from 0, so that no inf - inf arises: all its terms are 0.
+__device__ __forceinline__ float base_of(float mx) { return mx == -CUDART_INF_F ? 0.0f : mx; }
+
+__device__ __forceinline__ float warp_max(float v)
 {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        RowSums w;
-        w.mx = __shfl_xor_sync(0xffffffffu, v.mx, o);
-        w.s = __shfl_xor_sync(0xffffffffu, v.s, o);
-        w.u = __shfl_xor_sync(0xffffffffu, v.u, o);
-        // the lower lane's part comes first on both sides, so that both compute the same bits
-        v = (threadIdx.x & o) ? join(w, v, it) : join(v, w, it);
-    }
+    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(kAllLanes, v, o));
     return v;
+}
+
+__device__ __forceinline__ float warp_sum(float v)
+{
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kAllLanes, v, o);
+    return v;
+}
+
+// the sums of a warp's 32 disjoint parts, in every lane; an empty part (nothing but -inf) changes nothing, a NaN stays
+__device__ __forceinline__ RowSums join_lanes(const RowSums& v, float c)
+{
+    RowSums r;
+    r.mx = warp_max(v.mx);
+    const bool top = v.mx == r.mx;
+    const float delta = top ? 0.0f : fmaxf((v.mx - r.mx) * c, kNothing), f = exp2_fast(delta);
+    r.ties = warp_sum(top ? v.ties : 0.0f);
+    r.s = warp_sum(top ? v.s : (v.s + v.ties) * f);
+    r.u = warp_sum(f * (v.u + delta * (v.s + v.ties)));
+    return r;
 }
 
 // sum over a block of up to 1024 threads in a fixed order, valid in every thread
@@ -52,7 +81,7 @@ __device__ __forceinline__ double block_sum(double v, double* sh)
 {
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, nw = blockDim.x >> 5;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kAllLanes, v, o);
     __syncthreads();
     if (lane == 0) sh[w] = v;
     __syncthreads();
@@ -61,11 +90,25 @@ __device__ __forceinline__ double block_sum(double v, double* sh)
     return t;
 }
 
+// log(ties + s) to about 4e-8, absolutely and (for sums near 1) relatively, with fp32's own logarithms: log1p() of s beside a
+// single one, and elsewhere the logarithm of the mantissa beside an exact power of two.
+__device__ __forceinline__ double log_of_sum(float ties, float s)
+{
+    if (ties == 1.0f && s < 1.0f) return (double)log1pf(s);
+    const float total = ties + s;
+    const int e = ilogbf(total);
+    return total == 0.0f ? -CUDART_INF : (double)e * 0.693147180559945309417 + (double)logf(scalbnf(total, -e));
+}
+
+// exp(x) of a difference of log-probabilities: fp32 has the accuracy that the difference leaves, fp64 the range
+__device__ __forceinline__ double exp_of(double x) { return x > 80.0 ? exp(x) : (double)expf((float)x); }
+__device__ __forceinline__ double expm1_of(double x) { return x > 80.0 ? exp(x) : (double)expm1f((float)x); }
+
 struct RowParams {
     const float* logits;
     long long ld;
     const int32_t* targets;
-    float it;
+    float it, c;   // inv_temp, inv_temp * log2(e)
     int M, N;
     float *logp, *entropy, *stats;
     // policy loss only
@@ -78,32 +121,53 @@ struct RowParams {
     int* status;
 };
 
-// What a row's gradient is made of: dx_j = p_j * (a + b * (log p_j)) for j != t, and dx_t as it is.
-struct RowGrad {
-    float a, b, at_target;
+// What a row's gradient is made of: dx_j = 2^t * (a + b * t) for j != target, and dx at the target as it is.  t is measured
+// from `mx`.
+struct __align__(16) RowGrad {
+    float a, b, at_target, mx;
 };
 
-// The scalars of one row from its sums (one thread): writes logp, entropy, stats, token_loss, returns the gradient's
-// coefficients.  Log-probability, ratio and loss are computed in fp64 from the fp32 sums: a ratio is exp() of a difference of
-// numbers around 10, which fp32 would leave with an error of 1e-6.
+// One row's entries of the other inputs, fetched by the thread that makes the row's scalars.  It does so before the walk over
+// the row, and before any gradient is written: dlogits may be the logits' own buffer.
+struct RowInputs {
+    float x_t, old_logp, ref_logp, advantage;
+};
+
 template <bool Policy>
-__device__ __forceinline__ RowGrad row_scalars(const RowParams& p, int row, const RowSums& r, float x_t, float w)
+__device__ __forceinline__ RowInputs row_inputs(const RowParams& p, int row, int t)
 {
-    const bool empty = (r.s == 0.0f);
-    const double log_s = log((double)r.s);
-    const double logp = empty ? -CUDART_INF : (double)p.it * ((double)x_t - (double)base_of(r.mx)) - log_s;
-    const double H = empty ? 0.0 : log_s - (double)r.u / (double)r.s;
-    if (p.logp) p.logp[row] = (float)logp;
-    if (p.entropy) p.entropy[row] = (float)H;
-    if (p.stats) {
-        p.stats[2 * (size_t)row] = r.mx;
-        p.stats[2 * (size_t)row + 1] = r.s;
-    }
-    RowGrad g{0.0f, 0.0f, 0.0f};
+    RowInputs in{p.logits[(size_t)row * p.ld + t], 0.0f, 0.0f, 0.0f};
     if (Policy) {
-        const double A = p.advantages[row], ratio = exp(logp - (double)p.old_logp[row]);
+        in.old_logp = p.old_logp[row];
+        in.advantage = p.advantages[row];
+        if (p.kl_coef != 0.0f) in.ref_logp = p.ref_logp[row];
+    }
+    return in;
+}
+
+// The scalars of one row from its sums (one thread): writes logp, entropy, stats, token_loss (where `write`), returns the
+// gradient's coefficients for a walk over logits measured from `from`.  The log-probability, and the differences that ratio and
+// KL term are made of, are fp64: fp32 would leave a ratio of two probabilities of e^-10 an error of 1e-6.
+template <bool Policy>
+__device__ __forceinline__ RowGrad row_scalars(const RowParams& p, int row, const RowSums& r, const RowInputs& in, float w, bool write,
+                                               float from)
+{
+    const float total = r.ties + r.s;
+    const bool empty = total == 0.0f;
+    const double log_s = log_of_sum(r.ties, r.s);
+    const double logp = empty ? -CUDART_INF : (double)p.it * ((double)in.x_t - (double)base_of(r.mx)) - log_s;
+    const double H = empty ? 0.0 : log_s - (double)(kLn2 * r.u / total);
+    if (write) {
+        if (p.logp) p.logp[row] = (float)logp;
+        if (p.entropy) p.entropy[row] = (float)H;
+        if (p.stats) *reinterpret_cast<float2*>(p.stats + 2 * (size_t)row) = make_float2(r.mx, total);
+    }
+    RowGrad g{0.0f, 0.0f, 0.0f, from};
+    if (Policy) {
+        const double A = in.advantage;
         double loss = 0.0, slope = 0.0;
         if (A != 0.0) {
+            const double ratio = exp_of(logp - (double)in.old_logp);
             const double lo = 1.0 - (double)p.clip_low, hi = 1.0 + (double)p.clip_high;
             // a gain counts up to the upper border, a loss down to the lower one
             const bool outside = A > 0.0 ? ratio > hi : ratio < lo;
@@ -111,8 +175,11 @@ __device__ __forceinline__ RowGrad row_scalars(const RowParams& p, int row, cons
             slope = outside ? 0.0 : loss;
         }
         if (p.kl_coef != 0.0f) {
-            const double q = (double)p.ref_logp[row] - logp, e = expm1(q);
-            loss += (double)p.kl_coef * (e - q);
+            const double q = (double)in.ref_logp - logp, e = expm1_of(q);
+            // e - q loses what e and q share: for a small q the first terms of its series, q^2/2 + q^3/6 + q^4/24 + q^5/120 (the next
+            // is below 1e-8 of the first for |q| < 1/32)
+            const double rest = fabs(q) < 0.03125 ? q * q * (0.5 + q * (1.0 / 6.0 + q * (1.0 / 24.0 + q * (1.0 / 120.0)))) : e - q;
+            loss += (double)p.kl_coef * rest;
             slope -= (double)p.kl_coef * e;
         }
         double h = 0.0;
@@ -120,13 +187,15 @@ __device__ __forceinline__ RowGrad row_scalars(const RowParams& p, int row, cons
             loss -= (double)p.entropy_coef * H;
             h = -(double)p.entropy_coef;
         }
-        p.token_loss[row] = (float)loss;
+        if (write) p.token_loss[row] = (float)loss;
         if (!empty) {
             const double G = (double)p.it * w * slope, E = (double)p.it * w * h;
-            g.a = (float)(-G - E * H);
-            g.b = (float)(-E);
-            const double pt = exp(logp);
-            g.at_target = (float)(-G * expm1(logp) - (pt > 0.0 ? E * pt * (logp + H) : 0.0));
+            const float rest = expm1f((float)logp);   // p_t - 1
+            g.at_target = (float)(-G * rest - (rest > -1.0f && E != 0.0 ? E * (1.0 + rest) * (logp + H) : 0.0));
+            // p_j (-G - E (log p_j + H)),  p_j = 2^(t + delta) / s,  log p_j = log(2) (t + delta) - log s
+            const float delta = from == r.mx ? 0.0f : fmaxf((from - r.mx) * p.c, kNothing), inv = exp2_fast(delta) / total;
+            g.a = inv * (float)(-G - E * (H + (double)(kLn2 * delta) - log_s));
+            g.b = inv * (float)(-E) * kLn2;
         }
     }
     return g;
@@ -147,93 +216,326 @@ __device__ __forceinline__ void row_unused(const RowParams& p, int row, bool bad
     if (bad && p.status) atomicOr(p.status, ZNN_DEV_BAD_INDEX);
 }
 
-// One block per row, any length: the first walk over the row makes the sums, the second (policy loss with gradient) reads
-// the logits again and writes the gradient.
-template <bool Policy>
-__global__ void __launch_bounds__(256) rows_walk_kernel(const RowParams p)
+// ---- a row held in registers ----------------------------------------------------------------------------------------
+// Group threads hold V quads of four columns each of a row's part: thread k has the 16-byte quads k, k + Group, ... of memory
+// from the one that the part starts in, so rows may start at any float.
+template <int Group, int V>
+struct RowPart {
+    float v[V][4];
+    int begin;   // column that the first thread's first quad begins at: a multiple of 4 floats of memory, so it may be negative
+    int n;       // columns of the part
+
+    __device__ __forceinline__ int column(int tid, int k) const { return begin + 4 * (tid + k * Group); }
+
+    __device__ __forceinline__ void load_from(const float* x, int columns, int from, int tid)
+    {
+        n = columns;
+        begin = from;
+#pragma unroll
+        for (int k = 0; k < V; k++) {
+            const int j = column(tid, k);
+            if (j >= 0 && j + 4 <= n) {
+                const float4 q = __ldcs(reinterpret_cast<const float4*>(x + j));
+                v[k][0] = q.x; v[k][1] = q.y; v[k][2] = q.z; v[k][3] = q.w;
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; i++) v[k][i] = (j + i >= 0 && j + i < n) ? __ldcs(x + j + i) : -CUDART_INF_F;
+            }
+        }
+    }
+
+    __device__ __forceinline__ void load(const float* x, int columns, int tid) { load_from(x, columns, -((int)((uintptr_t)x >> 2) & 3), tid); }
+
+    // whether the columns of a quad lie in one 16-byte quad of the row y as well
+    __device__ __forceinline__ bool same_quads(const float* y) const { return (((uintptr_t)(y + begin) >> 2) & 3) == 0; }
+
+    // the same columns of another row, whatever its alignment, to hold beside this part's
+    __device__ __forceinline__ void load_beside(const float* y, int tid, float (&o)[V][4]) const
+    {
+        const bool quads = same_quads(y);
+#pragma unroll
+        for (int k = 0; k < V; k++) {
+            const int j = column(tid, k);
+            if (quads && j >= 0 && j + 4 <= n) {
+                const float4 q = __ldcs(reinterpret_cast<const float4*>(y + j));
+                o[k][0] = q.x; o[k][1] = q.y; o[k][2] = q.z; o[k][3] = q.w;
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; i++) o[k][i] = (j + i >= 0 && j + i < n) ? __ldcs(y + j + i) : 0.0f;
+            }
+        }
+    }
+
+    // whether this thread is the one that holds (and stores) column c
+    __device__ __forceinline__ bool owns(int c, int tid) const
+    {
+        const int quad = (c - begin) >> 2;
+        return c >= 0 && c < n && quad >= 0 && quad < Group * V && quad % Group == tid;
+    }
+
+    // writes what the caller has put into v to a row of any alignment
+    __device__ __forceinline__ void store(float* y, int tid) const
+    {
+        const bool quads = same_quads(y);
+#pragma unroll
+        for (int k = 0; k < V; k++) {
+            const int j = column(tid, k);
+            if (quads && j >= 0 && j + 4 <= n) {
+                __stcs(reinterpret_cast<float4*>(y + j), make_float4(v[k][0], v[k][1], v[k][2], v[k][3]));
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (j + i >= 0 && j + i < n) __stcs(y + j + i, v[k][i]);
+            }
+        }
+    }
+};
+
+__device__ __forceinline__ int cluster_size()
 {
-    __shared__ RowSums sh[8];
+    unsigned r;
+    asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(r));
+    return (int)r;
+}
+__device__ __forceinline__ int cluster_rank()
+{
+    unsigned r;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return (int)r;
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
+// The sums that each thread of a row's block (or of the cluster that shares the row) brings, joined: every warp joins its lanes,
+// the first warp of every block joins the warps and writes the result to its place in every block of the cluster, and joins
+// those.  Returns what thread 0 needs (the first warp has it).  A block's memory may be written to once it runs: the cluster
+// has arrived at its barrier when the kernel began, and is waited for here.
+template <int Group>
+__device__ __forceinline__ RowSums join_row(const RowSums& mine, float c, int tid, int ranks, int rank, RowSums* sh_warps, RowSums* sh_ranks)
+{
+    RowSums r = join_lanes(mine, c);
+    if (Group == 32) return r;
+    if ((tid & 31) == 0) sh_warps[tid >> 5] = r;
+    __syncthreads();
+    const RowSums none{-CUDART_INF_F, 0.0f, 0.0f, 0.0f};
+    if (tid < 32) r = join_lanes(tid < Group / 32 ? sh_warps[tid] : none, c);
+    if (ranks > 1) {
+        cluster_wait();
+        if (tid < ranks) *cg::this_cluster().map_shared_rank(sh_ranks + rank, tid) = r;
+        __syncwarp();   // the barrier's instructions want whole warps
+        cluster_arrive();
+        cluster_wait();
+        if (tid < 32) r = join_lanes(tid < ranks ? sh_ranks[tid] : none, c);
+    }
+    return r;
+}
+
+// One pass over the logits: a group of threads (a warp, or a block, or the blocks of a cluster, which take `part` columns
+// each) holds a whole row in registers from the load to the gradient's store.  The maximum (of a block's part) comes first, so
+// that every exponential is taken once, relative to it.
+template <bool Policy, bool Entropy, int Group, int V>
+__global__ void __launch_bounds__(Group == 32 ? 128 : Group, Group == 32 ? 8 : 1024 / Group) rows_held_kernel(const RowParams p, int part)
+{
+    constexpr int kWarps = Group / 32;
+    __shared__ float sh_max[kWarps];
+    __shared__ RowSums sh_warps[kWarps], sh_ranks[8];
     __shared__ RowGrad sh_grad;
-    const int row = blockIdx.x, tid = threadIdx.x;
+    const int ranks = Group == 32 ? 1 : cluster_size(), rank = Group == 32 ? 0 : cluster_rank();
+    if (ranks > 1) cluster_arrive();
+    const int tid = Group == 32 ? threadIdx.x & 31 : threadIdx.x;
+    const int row = Group == 32 ? blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x / ranks;
+    if (Group == 32 && row >= p.M) return;
+    const int first = rank * part, n = max(0, min(part, p.N - first));
+    const float* x = p.logits + (size_t)row * p.ld + first;
+    float* dx = Policy && p.dlogits ? p.dlogits + (size_t)row * p.ld_d + first : nullptr;
+
+    const int t = p.targets[row];
+    float w = 1.0f;
+    if (Policy && p.weights) w = p.weights[row];
+    if (t < 0 || t >= p.N || w == 0.0f) {   // the same in every block of a cluster
+        if (tid == 0 && rank == 0) row_unused<Policy>(p, row, t >= p.N && w != 0.0f);
+        if (dx)
+            for (int j = tid; j < n; j += Group) __stcs(dx + j, 0.0f);
+        return;
+    }
+    RowPart<Group, V> r;
+    r.load(x, n, tid);
+    RowInputs in{};
+    if (tid == 0) in = row_inputs<Policy>(p, row, t);
+    if (Policy && !p.weights) w = 1.0f / *p.count;
+
+    RowSums sums{-CUDART_INF_F, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int k = 0; k < V; k++)
+        sums.mx = fmaxf(fmaxf(sums.mx, fmaxf(r.v[k][0], r.v[k][1])), fmaxf(r.v[k][2], r.v[k][3]));
+    const float own = sums.mx;
+    sums.mx = warp_max(sums.mx);
+    if (Group > 32) {
+        if ((tid & 31) == 0) sh_max[tid >> 5] = sums.mx;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kWarps; i++) sums.mx = fmaxf(sums.mx, sh_max[i]);
+    }
+    const float base = base_of(sums.mx);
+#pragma unroll
+    for (int k = 0; k < V; k++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            // with an entropy term t is clamped (0 * -inf is to be 0), and kept for the gradient, which takes 2^t again
+            const float t2 = (r.v[k][i] - base) * p.c, te = Entropy ? max_nan(t2, kNothing) : t2, e = exp2_fast(te);
+            sums.s += e;
+            if (Entropy) sums.u += te * e;
+            if (Policy) r.v[k][i] = Entropy ? te : e;
+            else if (Entropy) r.v[k][i] = te;
+            else r.v[k][i] = e;
+        }
+    if (own == base && sums.mx == base) {   // the few threads that hold the largest logit tell its ones from the rest
+        sums.s = 0.0f;
+#pragma unroll
+        for (int k = 0; k < V; k++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float e = Entropy ? exp2_fast(r.v[k][i]) : r.v[k][i];
+                if (e == 1.0f) sums.ties += 1.0f;
+                else sums.s += e;
+            }
+    }
+    const RowSums all = join_row<Group>(sums, p.c, tid, ranks, rank, sh_warps, sh_ranks);
+    RowGrad g{};
+    if (tid == 0) g = row_scalars<Policy>(p, row, all, in, w, rank == 0, sums.mx);
+    if (!dx) return;
+    if (Group > 32) {
+        if (tid == 0) sh_grad = g;
+        __syncthreads();
+        g = sh_grad;
+    } else {
+        g.a = __shfl_sync(kAllLanes, g.a, 0);
+        g.b = __shfl_sync(kAllLanes, g.b, 0);
+        g.at_target = __shfl_sync(kAllLanes, g.at_target, 0);
+    }
+#pragma unroll
+    for (int k = 0; k < V; k++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if (Entropy) r.v[k][i] = exp2_fast(r.v[k][i]) * (g.a + g.b * r.v[k][i]);
+            else r.v[k][i] *= g.a;
+        }
+    r.store(dx, tid);
+    if (r.owns(t - first, tid)) dx[t - first] = g.at_target;
+}
+
+// Rows that need not be held (no gradient is asked for) or cannot be (longer than a cluster's registers): a block, or a cluster
+// of blocks, walks over the row with running sums per thread, and a second time for the gradient.
+template <bool Policy, bool Entropy>
+__global__ void __launch_bounds__(256) rows_walk_kernel(const RowParams p, int part)
+{
+    constexpr int kQuads = 4;
+    __shared__ RowSums sh_warps[8], sh_ranks[8];
+    __shared__ RowGrad sh_grad;
+    const int ranks = cluster_size(), rank = cluster_rank(), tid = threadIdx.x;
+    if (ranks > 1) cluster_arrive();
+    const int row = blockIdx.x / ranks, first = rank * part, n = max(0, min(part, p.N - first));
+    const float* x = p.logits + (size_t)row * p.ld + first;
+    float* dx = Policy && p.dlogits ? p.dlogits + (size_t)row * p.ld_d + first : nullptr;
     const int t = p.targets[row];
     float w = 1.0f;
     if (Policy && p.weights) w = p.weights[row];
     if (t < 0 || t >= p.N || w == 0.0f) {
-        if (tid == 0) row_unused<Policy>(p, row, t >= p.N && w != 0.0f);
-        if (Policy && p.dlogits)
-            for (int j = tid; j < p.N; j += 256) p.dlogits[(size_t)row * p.ld_d + j] = 0.0f;
+        if (tid == 0 && rank == 0) row_unused<Policy>(p, row, t >= p.N && w != 0.0f);
+        if (dx)
+            for (int j = tid; j < n; j += 256) __stcs(dx + j, 0.0f);
         return;
     }
-    const float* x = p.logits + (size_t)row * p.ld;
-    RowSums r{-CUDART_INF_F, 0.0f, 0.0f};
-    for (int j0 = tid; j0 < p.N; j0 += 256 * 8) {
-        float v[8];
-        float mx = -CUDART_INF_F;
+    RowInputs in{};
+    if (tid == 0) in = row_inputs<Policy>(p, row, t);
+    if (Policy && !p.weights) w = 1.0f / *p.count;
+
+    RowSums sums{-CUDART_INF_F, 0.0f, 0.0f, 0.0f};
+    const int shift = (int)((uintptr_t)x >> 2) & 3, step = 4 * 256 * kQuads;
+    for (int j0 = -shift; j0 < n; j0 += step) {
+        RowPart<256, kQuads> r;
+        r.load_from(x, n, j0, tid);
+        float mx = sums.mx;
 #pragma unroll
-        for (int k = 0; k < 8; k++) {
-            const int j = j0 + 256 * k;
-            v[k] = j < p.N ? x[j] : -CUDART_INF_F;
-            mx = fmaxf(mx, v[k]);
+        for (int k = 0; k < kQuads; k++)
+            mx = fmaxf(fmaxf(mx, fmaxf(r.v[k][0], r.v[k][1])), fmaxf(r.v[k][2], r.v[k][3]));
+        if (mx != sums.mx) {
+            const float delta = fmaxf((sums.mx - mx) * p.c, kNothing), f = exp2_fast(delta);
+            sums.u = f * (sums.u + delta * (sums.s + sums.ties));
+            sums.s = f * (sums.s + sums.ties);
+            sums.ties = 0.0f;
+            sums.mx = mx;
         }
-        RowSums c{mx, 0.0f, 0.0f};
         const float base = base_of(mx);
 #pragma unroll
-        for (int k = 0; k < 8; k++) {
-            const float d = (v[k] - base) * p.it, e = expf(d);
-            c.s += e;
-            c.u += e > 0.0f ? d * e : 0.0f;
-        }
-        r = join(r, c, p.it);
+        for (int k = 0; k < kQuads; k++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float t2 = (r.v[k][i] - base) * p.c, te = Entropy ? max_nan(t2, kNothing) : t2, e = exp2_fast(te);
+                if (e == 1.0f) sums.ties += 1.0f;
+                else sums.s += e;
+                if (Entropy) sums.u += te * e;
+            }
     }
-    r = warp_join(r, p.it);
-    if ((tid & 31) == 0) sh[tid >> 5] = r;
-    float x_t = 0.0f;
-    if (tid == 0) x_t = x[t];   // before any gradient is written: dlogits may be the logits' own buffer
-    __syncthreads();
-    r = sh[0];
-    for (int i = 1; i < 8; i++) r = join(r, sh[i], p.it);
-    if (Policy && !p.weights) w = 1.0f / *p.count;
-    if (tid == 0) sh_grad = row_scalars<Policy>(p, row, r, x_t, w);
-    if (!Policy || !p.dlogits) return;
+    const RowSums all = join_row<256>(sums, p.c, tid, ranks, rank, sh_warps, sh_ranks);
+    if (tid == 0) sh_grad = row_scalars<Policy>(p, row, all, in, w, rank == 0, all.mx);
+    if (!dx) return;
     __syncthreads();
     const RowGrad g = sh_grad;
-    const float base = base_of(r.mx), inv_s = r.s == 0.0f ? 0.0f : 1.0f / r.s, log_s = logf(r.s);
-    float* dx = p.dlogits + (size_t)row * p.ld_d;
-    for (int j = tid; j < p.N; j += 256) {
-        const float d = (x[j] - base) * p.it, e = expf(d);
-        float o = e * inv_s * g.a;
-        if (g.b != 0.0f && e != 0.0f) o = e * inv_s * (g.a + g.b * (d - log_s));
-        dx[j] = j == t ? g.at_target : o;
+    const float base = base_of(g.mx);
+    for (int j0 = -shift; j0 < n; j0 += step) {
+        RowPart<256, kQuads> r;
+        r.load_from(x, n, j0, tid);
+#pragma unroll
+        for (int k = 0; k < kQuads; k++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float te = max_nan((r.v[k][i] - base) * p.c, kNothing);
+                r.v[k][i] = exp2_fast(te) * (g.a + g.b * te);
+            }
+        r.store(dx, tid);
+        if (r.owns(t - first, tid)) dx[t - first] = g.at_target;
     }
 }
 
-// dlogits of the log-probabilities from the forward's statistics: one block per row
-template <bool Accumulate>
-__global__ void __launch_bounds__(256)
+// dlogits of the log-probabilities from the forward's statistics.  A group of threads takes 4 * Group * V columns of a row;
+// every load of the logits, and of the gradient that is added to, is under way before the first result is made.
+template <bool Accumulate, int Group, int V>
+__global__ void __launch_bounds__(Group == 32 ? 128 : Group)
 logprob_bwd_kernel(const float* logits, long long ld, const int32_t* __restrict__ targets, float it,
                    const float* __restrict__ stats, const float* __restrict__ entropy, const float* __restrict__ dlogp,
-                   const float* __restrict__ dentropy, float* dlogits, long long ld_d, int N)
+                   const float* __restrict__ dentropy, float* dlogits, long long ld_d, int M, int N, int parts, int part)
 {
-    const int row = blockIdx.x, tid = threadIdx.x;
+    const int tid = Group == 32 ? threadIdx.x & 31 : threadIdx.x;
+    const unsigned unit = Group == 32 ? blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x;
+    const int row = (int)(unit / (unsigned)parts), first = (int)(unit % (unsigned)parts) * part, n = min(part, N - first);
+    if (row >= M) return;
+    const float* x = logits + (size_t)row * ld + first;
+    float* dx = dlogits + (size_t)row * ld_d + first;
     const int t = targets[row];
-    float* dx = dlogits + (size_t)row * ld_d;
     const float s = stats[2 * (size_t)row + 1];
     if (t < 0 || t >= N || s == 0.0f) {
         if (!Accumulate)
-            for (int j = tid; j < N; j += 256) dx[j] = 0.0f;
+            for (int j = tid; j < n; j += Group) __stcs(dx + j, 0.0f);
         return;
     }
-    const float* x = logits + (size_t)row * ld;
-    const float base = base_of(stats[2 * (size_t)row]), inv_s = 1.0f / s;
+    RowPart<Group, V> r;
+    float old[V][4];
+    r.load(x, n, tid);
+    if (Accumulate) r.load_beside(dx, tid, old);
+    // p_j (-G - E (log p_j + H)) with p_j = 2^t / s, log p_j = log(2) t - log s
     const float G = it * (dlogp ? dlogp[row] : 0.0f), E = it * (dentropy ? dentropy[row] : 0.0f);
-    const float a = -G - (E != 0.0f ? E * entropy[row] : 0.0f), b = -E, log_s = logf(s);
-    for (int j = tid; j < N; j += 256) {
-        const float d = (x[j] - base) * it, e = expf(d);
-        float o = e * inv_s * a;
-        if (b != 0.0f && e != 0.0f) o = e * inv_s * (a + b * (d - log_s));
-        if (j == t) o += G;
-        dx[j] = Accumulate ? dx[j] + o : o;
-    }
+    const float base = base_of(stats[2 * (size_t)row]), c = it * kLog2e, inv = 1.0f / s;
+    const float a = inv * (-G - (E != 0.0f ? E * (entropy[row] - logf(s)) : 0.0f)), b = -inv * E * kLn2;
+#pragma unroll
+    for (int k = 0; k < V; k++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float te = max_nan((r.v[k][i] - base) * c, kNothing), o = exp2_fast(te) * (a + b * te);
+            r.v[k][i] = Accumulate ? old[k][i] + o : o;
+        }
+    r.store(dx, tid);
+    if (r.owns(t - first, tid)) dx[t - first] += G;
 }
 
 // loss[1] = rows in use; with_sum: loss[0] = sum of w_i token_loss_i as well.  One block, fixed order.
@@ -325,6 +627,65 @@ using namespace znn;
         if (!stream()) return fail(ZNN_ERR_CUDA, "no CUDA device state; call znn_init (no CPU fallback)"); \
     } while (0)
 
+// ---- launches
+// Columns that a group can take whatever their alignment: up to three floats lie before the first column of a part.
+static constexpr int room(int group, int v, bool aligned) { return 4 * group * v - (aligned ? 0 : 3); }
+
+static int launch_rows_kernel(void (*kernel)(RowParams, int), const RowParams& p, long long blocks, int threads, int ranks, int part)
+{
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)blocks);
+    cfg.blockDim = dim3(threads);
+    cfg.stream = stream();
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim = {(unsigned)ranks, 1, 1};
+    cfg.attrs = &attr;
+    cfg.numAttrs = ranks > 1 ? 1 : 0;
+    ZNN_CUDA_OK(cudaLaunchKernelEx(&cfg, kernel, p, part));
+    ZNN_LAUNCH_OK("rows kernel");
+    return ZNN_OK;
+}
+
+template <bool Policy, bool Entropy, int Group, int V>
+static int launch_held(const RowParams& p, int ranks, int part)
+{
+    return launch_rows_kernel(rows_held_kernel<Policy, Entropy, Group, V>, p, Group == 32 ? (p.M + 3LL) / 4 : (long long)p.M * ranks,
+                              Group == 32 ? 128 : Group, ranks, part);
+}
+
+template <bool Policy, bool Entropy>
+static int launch_rows(const RowParams& p)
+{
+    const bool aligned = ((uintptr_t)p.logits & 15) == 0 && p.ld % 4 == 0;
+    // a warp per row while a row fits one; then a block; then a cluster of blocks; then two walks
+    if (p.N <= room(32, 2, aligned)) return launch_held<Policy, Entropy, 32, 2>(p, 1, p.N);
+    if (p.N <= room(32, 8, aligned)) return launch_held<Policy, Entropy, 32, 8>(p, 1, p.N);
+    if (p.N <= room(256, 4, aligned)) return launch_held<Policy, Entropy, 256, 4>(p, 1, p.N);
+    if (p.N <= room(256, 8, aligned)) return launch_held<Policy, Entropy, 256, 8>(p, 1, p.N);
+    // (the policy loss without a gradient takes the same way, so that it gives the same bits)
+    for (int ranks = 1; Policy && ranks <= 8; ranks *= 2) {
+        const int part = (ceil_div(p.N, ranks) + 3) & ~3;   // parts start where the row's quads do
+        if (part <= room(512, 8, aligned)) return launch_held<Policy, Entropy, 512, 8>(p, ranks, part);
+    }
+    int ranks = Policy ? 8 : 1;
+    while (ranks < 8 && (long long)p.M * ranks < 4 * sm_count()) ranks *= 2;
+    return launch_rows_kernel(rows_walk_kernel<Policy, Entropy>, p, (long long)p.M * ranks, 256, ranks, (ceil_div(p.N, ranks) + 3) & ~3);
+}
+
+template <bool Accumulate, int Group, int V>
+static int launch_bwd(const float* logits, long long ld, const int32_t* targets, float it, const float* stats, const float* entropy,
+                      const float* dlogp, const float* dentropy, float* dlogits, long long ld_d, int M, int N, bool aligned)
+{
+    const int fit = room(Group, V, aligned) & ~3, parts = ceil_div(N, fit), part = (ceil_div(N, parts) + 3) & ~3;
+    const long long units = (long long)M * ceil_div(N, part);
+    const unsigned grid = (unsigned)(Group == 32 ? (units + 3) / 4 : units);
+    logprob_bwd_kernel<Accumulate, Group, V><<<grid, Group == 32 ? 128 : Group, 0, stream()>>>(
+        logits, ld, targets, it, stats, entropy, dlogp, dentropy, dlogits, ld_d, M, N, ceil_div(N, part), part);
+    ZNN_LAUNCH_OK("logprob_bwd_kernel");
+    return ZNN_OK;
+}
+
 static int check_rows(const float* logits, long long ld, const int32_t* targets, float inv_temp, int M, int N)
 {
     ZNN_REQUIRE(M >= 0 && N > 0, "M must not be negative and N must be positive");
@@ -345,11 +706,9 @@ int znn_token_logprob_fwd(const float* logits, long long ld, const int32_t* targ
     ZNN_REQUIRE(logp, "logp is NULL");
     ZNN_NEED_DEVICE();
     RowParams p{};
-    p.logits = logits; p.ld = ld; p.targets = targets; p.it = inv_temp; p.M = M; p.N = N;
+    p.logits = logits; p.ld = ld; p.targets = targets; p.it = inv_temp; p.c = (float)(inv_temp * 1.4426950408889634); p.M = M; p.N = N;
     p.logp = logp; p.entropy = entropy; p.stats = stats; p.status = device_status_word();
-    rows_walk_kernel<false><<<M, 256, 0, stream()>>>(p);
-    ZNN_LAUNCH_OK("rows_walk_kernel");
-    return ZNN_OK;
+    return entropy ? launch_rows<false, true>(p) : launch_rows<false, false>(p);
 }
 
 int znn_token_logprob_bwd(const float* logits, long long ld, const int32_t* targets, float inv_temp, const float* stats,
@@ -364,12 +723,12 @@ int znn_token_logprob_bwd(const float* logits, long long ld, const int32_t* targ
     ZNN_REQUIRE(ld_d >= N, "ld_d = %lld is smaller than N = %d", ld_d, N);
     ZNN_REQUIRE(dlogits != logits || (ld_d == ld && !accumulate), "dlogits may be the logits' own buffer only with ld_d == ld and accumulate = 0");
     ZNN_NEED_DEVICE();
-    if (accumulate)
-        logprob_bwd_kernel<true><<<M, 256, 0, stream()>>>(logits, ld, targets, inv_temp, stats, entropy, dlogp, dentropy, dlogits, ld_d, N);
-    else
-        logprob_bwd_kernel<false><<<M, 256, 0, stream()>>>(logits, ld, targets, inv_temp, stats, entropy, dlogp, dentropy, dlogits, ld_d, N);
-    ZNN_LAUNCH_OK("logprob_bwd_kernel");
-    return ZNN_OK;
+    const bool aligned = ((uintptr_t)logits & 15) == 0 && ld % 4 == 0;
+#define ZNN_BWD(acc, group, v) \
+    launch_bwd<acc, group, v>(logits, ld, targets, inv_temp, stats, entropy, dlogp, dentropy, dlogits, ld_d, M, N, aligned)
+    if (N <= room(32, 4, aligned)) return accumulate ? ZNN_BWD(true, 32, 4) : ZNN_BWD(false, 32, 4);
+    return accumulate ? ZNN_BWD(true, 256, 4) : ZNN_BWD(false, 256, 4);
+#undef ZNN_BWD
 }
 
 int znn_policy_loss(const float* logits, long long ld, const int32_t* targets, float inv_temp, const float* old_logp,
@@ -389,7 +748,7 @@ int znn_policy_loss(const float* logits, long long ld, const int32_t* targets, f
     ZNN_REQUIRE(dlogits != logits || ld_d == ld, "dlogits may be the logits' own buffer only with ld_d == ld");
     ZNN_NEED_DEVICE();
     RowParams p{};
-    p.logits = logits; p.ld = ld; p.targets = targets; p.it = inv_temp; p.M = M; p.N = N;
+    p.logits = logits; p.ld = ld; p.targets = targets; p.it = inv_temp; p.c = (float)(inv_temp * 1.4426950408889634); p.M = M; p.N = N;
     p.logp = logp; p.entropy = entropy; p.status = device_status_word();
     p.old_logp = old_logp; p.ref_logp = ref_logp; p.advantages = advantages; p.weights = weights;
     p.clip_low = clip_low; p.clip_high = clip_high; p.kl_coef = kl_coef; p.entropy_coef = entropy_coef;
@@ -398,8 +757,8 @@ int znn_policy_loss(const float* logits, long long ld, const int32_t* targets, f
         policy_total_kernel<<<1, 1024, 0, stream()>>>(targets, weights, token_loss, loss, M, 0);
         ZNN_LAUNCH_OK("policy_total_kernel");
     }
-    rows_walk_kernel<true><<<M, 256, 0, stream()>>>(p);
-    ZNN_LAUNCH_OK("rows_walk_kernel");
+    const int done = entropy || entropy_coef != 0.0f ? launch_rows<true, true>(p) : launch_rows<true, false>(p);
+    if (done != ZNN_OK) return done;
     policy_total_kernel<<<1, 1024, 0, stream()>>>(targets, weights, token_loss, loss, M, 1);
     ZNN_LAUNCH_OK("policy_total_kernel");
     return ZNN_OK;

@@ -232,11 +232,13 @@ int znn_init(int device)
                     e != cudaSuccess ? cudaGetErrorString(e) : "device count is 0");
     ZNN_REQUIRE(device >= 0 && device < n && device < kMaxDev, "device %d out of range (have %d)", device, n);
     ZNN_CUDA_OK(cudaSetDevice(device));
-    cudaDeviceProp prop;
-    ZNN_CUDA_OK(cudaGetDeviceProperties(&prop, device));
-    if (prop.major != 10)
-        return fail(ZNN_ERR_UNSUPPORTED, "device %d is sm_%d%d; this library is built for sm_100a only", device,
-                    prop.major, prop.minor);
+    // two attributes, not cudaGetDeviceProperties, which takes milliseconds: a program that drives several devices comes
+    // here at every znn_set_device
+    int major = 0, minor = 0;
+    ZNN_CUDA_OK(cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, device));
+    ZNN_CUDA_OK(cudaDeviceGetAttribute(&minor, cudaDevAttrComputeCapabilityMinor, device));
+    if (major != 10)
+        return fail(ZNN_ERR_UNSUPPORTED, "device %d is sm_%d%d; this library is built for sm_100a only", device, major, minor);
     if (!cur(true)) return fail(ZNN_ERR_CUDA, "could not create per-device state");
     return ZNN_OK;
 }
