@@ -2,15 +2,14 @@
 // with its gradient, the preference loss on pairs of sequences.  Formulas: include/znn_cuda.h.
 //
 // Every operator is bound by HBM: 10 to 20 operations per logit against 4 to 12 bytes.
-#include <cooperative_groups.h>
 #include <math.h>
 #include <math_constants.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "common.cuh"
-
-namespace cg = cooperative_groups;
+#include "tc_ptx.cuh"
 
 namespace znn {
 
@@ -27,6 +26,14 @@ __device__ __forceinline__ float exp2_fast(float x)
 {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// The same, for an exponential that is taken again rather than kept: the compiler does not see that it has been made already.
+__device__ __forceinline__ float exp2_again(float x)
+{
+    float y;
+    asm volatile("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
 
@@ -49,30 +56,34 @@ struct __align__(16) RowSums {
 // A row of -inf alone (mx = -inf) is measured from 0, so that no inf - inf arises: all its terms are 0.
 __device__ __forceinline__ float base_of(float mx) { return mx == -CUDART_INF_F ? 0.0f : mx; }
 
-__device__ __forceinline__ float warp_max(float v)
+// over the W lanes of a warp that `mask` names (W neighbours), in a fixed order, the result in each of them
+template <int W = 32>
+__device__ __forceinline__ float warp_max(float v, unsigned mask = kAllLanes)
 {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(kAllLanes, v, o));
+    for (int o = W / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(mask, v, o));
     return v;
 }
 
-__device__ __forceinline__ float warp_sum(float v)
+template <int W = 32>
+__device__ __forceinline__ float warp_sum(float v, unsigned mask = kAllLanes)
 {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kAllLanes, v, o);
+    for (int o = W / 2; o > 0; o >>= 1) v += __shfl_xor_sync(mask, v, o);
     return v;
 }
 
-// the sums of a warp's 32 disjoint parts, in every lane; an empty part (nothing but -inf) changes nothing, a NaN stays
-__device__ __forceinline__ RowSums join_lanes(const RowSums& v, float c)
+// the sums of W lanes' disjoint parts, in each of them; an empty part (nothing but -inf) changes nothing, a NaN stays
+template <int W = 32>
+__device__ __forceinline__ RowSums join_lanes(const RowSums& v, float c, unsigned mask = kAllLanes)
 {
     RowSums r;
-    r.mx = warp_max(v.mx);
+    r.mx = warp_max<W>(v.mx, mask);
     const bool top = v.mx == r.mx;
     const float delta = top ? 0.0f : fmaxf((v.mx - r.mx) * c, kNothing), f = exp2_fast(delta);
-    r.ties = warp_sum(top ? v.ties : 0.0f);
-    r.s = warp_sum(top ? v.s : (v.s + v.ties) * f);
-    r.u = warp_sum(f * (v.u + delta * (v.s + v.ties)));
+    r.ties = warp_sum<W>(top ? v.ties : 0.0f, mask);
+    r.s = warp_sum<W>(top ? v.s : (v.s + v.ties) * f, mask);
+    r.u = warp_sum<W>(f * (v.u + delta * (v.s + v.ties)), mask);
     return r;
 }
 
@@ -95,14 +106,19 @@ __device__ __forceinline__ double block_sum(double v, double* sh)
 __device__ __forceinline__ double log_of_sum(float ties, float s)
 {
     if (ties == 1.0f && s < 1.0f) return (double)log1pf(s);
-    const float total = ties + s;
-    const int e = ilogbf(total);
-    return total == 0.0f ? -CUDART_INF : (double)e * 0.693147180559945309417 + (double)logf(scalbnf(total, -e));
+    const float total = ties + s;   // at least 1, or 0, or NaN
+    const int bits = __float_as_int(total);
+    if (total == 0.0f) return -CUDART_INF;
+    return (double)((bits >> 23) - 127) * 0.693147180559945309417 + (double)logf(__int_as_float((bits & 0x007fffff) | 0x3f800000)) + (total - total);
 }
 
-// exp(x) of a difference of log-probabilities: fp32 has the accuracy that the difference leaves, fp64 the range
-__device__ __forceinline__ double exp_of(double x) { return x > 80.0 ? exp(x) : (double)expf((float)x); }
-__device__ __forceinline__ double expm1_of(double x) { return x > 80.0 ? exp(x) : (double)expm1f((float)x); }
+// exp(x), exp(x) - 1 of a difference of log-probabilities: fp32 has the accuracy that the difference leaves, fp64 the range
+__device__ __forceinline__ double exp_of(double x)
+{
+    const float z = (float)x, e = expf(z > 80.0f ? 0.5f * z : z);
+    return z > 80.0f ? (double)e * (double)e : (double)e;
+}
+__device__ __forceinline__ double expm1_of(double x) { return x > 80.0 ? exp_of(x) : (double)expm1f((float)x); }
 
 struct RowParams {
     const float* logits;
@@ -127,35 +143,42 @@ struct __align__(16) RowGrad {
     float a, b, at_target, mx;
 };
 
-// One row's entries of the other inputs, fetched by the thread that makes the row's scalars.  It does so before the walk over
-// the row, and before any gradient is written: dlogits may be the logits' own buffer.
-struct RowInputs {
-    float x_t, old_logp, ref_logp, advantage;
+// What decides whether a row is used: its target and (policy loss) its weight.  With them, in the thread that makes the row's
+// scalars (`inputs`), the row's entries of the other inputs.  All of it is fetched well ahead: behind the rows that are on
+// their way, a single load takes microseconds.
+struct RowHead {
+    int t;
+    float w, old_logp, ref_logp, advantage;
+    __device__ __forceinline__ bool used(int N) const { return t >= 0 && t < N && w != 0.0f; }
 };
 
 template <bool Policy>
-__device__ __forceinline__ RowInputs row_inputs(const RowParams& p, int row, int t)
+__device__ __forceinline__ RowHead row_head(const RowParams& p, unsigned row, bool inputs)
 {
-    RowInputs in{p.logits[(size_t)row * p.ld + t], 0.0f, 0.0f, 0.0f};
-    if (Policy) {
-        in.old_logp = p.old_logp[row];
-        in.advantage = p.advantages[row];
-        if (p.kl_coef != 0.0f) in.ref_logp = p.ref_logp[row];
+    RowHead h{-1, 1.0f, 0.0f, 0.0f, 0.0f};
+    if (row < (unsigned)p.M) {
+        h.t = p.targets[row];
+        if (Policy && p.weights) h.w = p.weights[row];
+        if (Policy && inputs) {
+            h.old_logp = p.old_logp[row];
+            h.advantage = p.advantages[row];
+            if (p.kl_coef != 0.0f) h.ref_logp = p.ref_logp[row];
+        }
     }
-    return in;
+    return h;
 }
 
 // The scalars of one row from its sums (one thread): writes logp, entropy, stats, token_loss (where `write`), returns the
 // gradient's coefficients for a walk over logits measured from `from`.  The log-probability, and the differences that ratio and
 // KL term are made of, are fp64: fp32 would leave a ratio of two probabilities of e^-10 an error of 1e-6.
 template <bool Policy>
-__device__ __forceinline__ RowGrad row_scalars(const RowParams& p, int row, const RowSums& r, const RowInputs& in, float w, bool write,
-                                               float from)
+__device__ __forceinline__ RowGrad row_scalars(const RowParams& p, int row, const RowSums& r, const RowHead& in, float x_t, float w,
+                                               bool write, float from)
 {
     const float total = r.ties + r.s;
     const bool empty = total == 0.0f;
     const double log_s = log_of_sum(r.ties, r.s);
-    const double logp = empty ? -CUDART_INF : (double)p.it * ((double)in.x_t - (double)base_of(r.mx)) - log_s;
+    const double logp = empty ? -CUDART_INF : (double)p.it * ((double)x_t - (double)base_of(r.mx)) - log_s;
     const double H = empty ? 0.0 : log_s - (double)(kLn2 * r.u / total);
     if (write) {
         if (p.logp) p.logp[row] = (float)logp;
@@ -218,36 +241,72 @@ __device__ __forceinline__ void row_unused(const RowParams& p, int row, bool bad
 
 // ---- a row held in registers ----------------------------------------------------------------------------------------
 // Group threads hold V quads of four columns each of a row's part: thread k has the 16-byte quads k, k + Group, ... of memory
-// from the one that the part starts in, so rows may start at any float.
-template <int Group, int V>
+// from the one that the part starts in, so rows may start at any float.  Aligned: every row starts with a quad and has whole
+// quads only; no code for the others then stands between the memory instructions.
+template <int Group, int V, bool Aligned>
 struct RowPart {
     float v[V][4];
-    int begin;   // column that the first thread's first quad begins at: a multiple of 4 floats of memory, so it may be negative
+    int begin;   // column that the first thread's first quad begins at: that is on a multiple of 16 bytes, so it may be negative
     int n;       // columns of the part
 
     __device__ __forceinline__ int column(int tid, int k) const { return begin + 4 * (tid + k * Group); }
+    __device__ __forceinline__ bool whole(int j) const { return Aligned ? j < n : j >= 0 && j + 4 <= n; }
 
-    __device__ __forceinline__ void load_from(const float* x, int columns, int from, int tid)
+    __device__ __forceinline__ void place(const float* x, int columns)
     {
         n = columns;
-        begin = from;
+        begin = Aligned ? 0 : -((int)((uintptr_t)x >> 2) & 3);
+    }
+
+    __device__ __forceinline__ void load(const float* x, int tid)
+    {
 #pragma unroll
         for (int k = 0; k < V; k++) {
             const int j = column(tid, k);
-            if (j >= 0 && j + 4 <= n) {
+            if (whole(j)) {
                 const float4 q = __ldcs(reinterpret_cast<const float4*>(x + j));
                 v[k][0] = q.x; v[k][1] = q.y; v[k][2] = q.z; v[k][3] = q.w;
             } else {
 #pragma unroll
-                for (int i = 0; i < 4; i++) v[k][i] = (j + i >= 0 && j + i < n) ? __ldcs(x + j + i) : -CUDART_INF_F;
+                for (int i = 0; i < 4; i++) v[k][i] = (!Aligned && j + i >= 0 && j + i < n) ? __ldcs(x + j + i) : -CUDART_INF_F;
             }
         }
     }
 
-    __device__ __forceinline__ void load(const float* x, int columns, int tid) { load_from(x, columns, -((int)((uintptr_t)x >> 2) & 3), tid); }
+    // The part is copied to shared memory ahead of its use, every thread its own quads to places of its own (`mine`, `pitch`
+    // quads apart): only the thread itself waits for them, with no barrier.
+    __device__ __forceinline__ void fetch(const float* x, int tid, float4* mine, int pitch) const
+    {
+#pragma unroll
+        for (int k = 0; k < V; k++) {
+            const int j = column(tid, k);
+            const unsigned to = (unsigned)__cvta_generic_to_shared(mine + k * pitch);
+            if (whole(j)) {
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(x + j) : "memory");
+            } else if (Aligned) {
+                mine[k * pitch] = make_float4(-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F);
+            } else {
+#pragma unroll 1
+                for (int i = 0; i < 4; i++) {
+                    if (j + i >= 0 && j + i < n) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to + 4 * i), "l"(x + j + i) : "memory");
+                    else reinterpret_cast<float*>(mine + k * pitch)[i] = -CUDART_INF_F;
+                }
+            }
+        }
+    }
+
+    __device__ __forceinline__ void take(const float4* mine, int pitch)
+    {
+        asm volatile("cp.async.wait_all;" ::: "memory");
+#pragma unroll
+        for (int k = 0; k < V; k++) {
+            const float4 q = mine[k * pitch];
+            v[k][0] = q.x; v[k][1] = q.y; v[k][2] = q.z; v[k][3] = q.w;
+        }
+    }
 
     // whether the columns of a quad lie in one 16-byte quad of the row y as well
-    __device__ __forceinline__ bool same_quads(const float* y) const { return (((uintptr_t)(y + begin) >> 2) & 3) == 0; }
+    __device__ __forceinline__ bool same_quads(const float* y) const { return Aligned || (((uintptr_t)(y + begin) >> 2) & 3) == 0; }
 
     // the same columns of another row, whatever its alignment, to hold beside this part's
     __device__ __forceinline__ void load_beside(const float* y, int tid, float (&o)[V][4]) const
@@ -256,21 +315,22 @@ struct RowPart {
 #pragma unroll
         for (int k = 0; k < V; k++) {
             const int j = column(tid, k);
-            if (quads && j >= 0 && j + 4 <= n) {
+            if (quads && whole(j)) {
                 const float4 q = __ldcs(reinterpret_cast<const float4*>(y + j));
                 o[k][0] = q.x; o[k][1] = q.y; o[k][2] = q.z; o[k][3] = q.w;
             } else {
 #pragma unroll
-                for (int i = 0; i < 4; i++) o[k][i] = (j + i >= 0 && j + i < n) ? __ldcs(y + j + i) : 0.0f;
+                for (int i = 0; i < 4; i++) o[k][i] = (!Aligned && j + i >= 0 && j + i < n) ? __ldcs(y + j + i) : 0.0f;
             }
         }
     }
 
-    // whether this thread is the one that holds (and stores) column c
+    // the quad, in the order of the threads, that holds column c, and whether it is one of this thread's
+    __device__ __forceinline__ int quad_of(int c) const { return (c - begin) >> 2; }
     __device__ __forceinline__ bool owns(int c, int tid) const
     {
-        const int quad = (c - begin) >> 2;
-        return c >= 0 && c < n && quad >= 0 && quad < Group * V && quad % Group == tid;
+        const int q = quad_of(c);
+        return c >= 0 && c < n && q >= 0 && q < Group * V && q % Group == tid;
     }
 
     // writes what the caller has put into v to a row of any alignment
@@ -280,17 +340,34 @@ struct RowPart {
 #pragma unroll
         for (int k = 0; k < V; k++) {
             const int j = column(tid, k);
-            if (quads && j >= 0 && j + 4 <= n) {
+            if (quads && whole(j)) {
                 __stcs(reinterpret_cast<float4*>(y + j), make_float4(v[k][0], v[k][1], v[k][2], v[k][3]));
-            } else {
+            } else if (!Aligned) {
 #pragma unroll
                 for (int i = 0; i < 4; i++)
                     if (j + i >= 0 && j + i < n) __stcs(y + j + i, v[k][i]);
             }
         }
     }
+
+    __device__ __forceinline__ void clear(float* y, int tid) const
+    {
+        const bool quads = same_quads(y);
+#pragma unroll 1
+        for (int k = 0; k < V; k++) {
+            const int j = column(tid, k);
+            if (quads && whole(j)) {
+                __stcs(reinterpret_cast<float4*>(y + j), make_float4(0.0f, 0.0f, 0.0f, 0.0f));
+            } else if (!Aligned) {
+#pragma unroll 1
+                for (int i = 0; i < 4; i++)
+                    if (j + i >= 0 && j + i < n) __stcs(y + j + i, 0.0f);
+            }
+        }
+    }
 };
 
+// ---- what the blocks of a cluster tell one another -------------------------------------------------------------------
 __device__ __forceinline__ int cluster_size()
 {
     unsigned r;
@@ -303,158 +380,236 @@ __device__ __forceinline__ int cluster_rank()
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
     return (int)r;
 }
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
-// The sums that each thread of a row's block (or of the cluster that shares the row) brings, joined: every warp joins its lanes,
-// the first warp of every block joins the warps and writes the result to its place in every block of the cluster, and joins
-// those.  Returns what thread 0 needs (the first warp has it).  A block's memory may be written to once it runs: the cluster
-// has arrived at its barrier when the kernel began, and is waited for here.
-template <int Group>
-__device__ __forceinline__ RowSums join_row(const RowSums& mine, float c, int tid, int ranks, int rank, RowSums* sh_warps, RowSums* sh_ranks)
+// The sums of every block's part of a row, written by the blocks themselves, with the target's logit from the one that has it.
+// Two such places take turns, so that a block may be one row ahead of another: it cannot be two ahead, since the row between
+// needs the other's word.
+struct RowWord {
+    RowSums sums[8];
+    float x_t;
+    unsigned long long bar;
+};
+
+// Sends this block's sums (and x_t, where `has_target`) to every block of the cluster and waits for theirs; all lanes of one
+// warp call it.  The stores count on the receiver's barrier as they land: no fence waits for the gradients that are on their
+// way to memory.  parity: of the number of rows that have used this place.
+__device__ __forceinline__ void exchange(RowWord* word, const RowSums& mine, float x_t, bool has_target, int ranks, int rank, unsigned parity, int* status)
 {
-    RowSums r = join_lanes(mine, c);
-    if (Group == 32) return r;
-    if ((tid & 31) == 0) sh_warps[tid >> 5] = r;
-    __syncthreads();
-    const RowSums none{-CUDART_INF_F, 0.0f, 0.0f, 0.0f};
-    if (tid < 32) r = join_lanes(tid < Group / 32 ? sh_warps[tid] : none, c);
-    if (ranks > 1) {
-        cluster_wait();
-        if (tid < ranks) *cg::this_cluster().map_shared_rank(sh_ranks + rank, tid) = r;
-        __syncwarp();   // the barrier's instructions want whole warps
-        cluster_arrive();
-        cluster_wait();
-        if (tid < 32) r = join_lanes(tid < ranks ? sh_ranks[tid] : none, c);
+    const int lane = threadIdx.x & 31;
+    const uint32_t bar = smem_u32(&word->bar), sums = smem_u32(&word->sums[rank]), target = smem_u32(&word->x_t);
+    if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)(ranks * sizeof(RowSums) + sizeof(float)));
+    if (lane < ranks) {
+        const uint32_t there = mapa_shared(bar, lane);
+        asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(mapa_shared(sums, lane)),
+                     "f"(mine.mx), "f"(mine.ties), "f"(mine.s), "f"(mine.u), "r"(there)
+                     : "memory");
+        if (has_target)
+            asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.f32 [%0], %1, [%2];" ::"r"(mapa_shared(target, lane)), "f"(x_t), "r"(there)
+                         : "memory");
     }
-    return r;
+    // (every block of the cluster runs and takes the same rows: the wait ends.  Its limit is there for what nobody foresees; the
+    // row is then made of what has arrived, and the status word says so)
+    if (!mbar_wait_bounded_cluster(bar, parity, kWaitLimitCycles) && status) atomicOr(status, ZNN_DEV_TMA_WAIT_EXPIRED);
+    __syncwarp();
 }
 
-// One pass over the logits: a group of threads (a warp, or a block, or the blocks of a cluster, which take `part` columns
-// each) holds a whole row in registers from the load to the gradient's store.  The maximum (of a block's part) comes first, so
-// that every exponential is taken once, relative to it.
-template <bool Policy, bool Entropy, int Group, int V>
-__global__ void __launch_bounds__(Group == 32 ? 128 : Group, Group == 32 ? 8 : 1024 / Group) rows_held_kernel(const RowParams p, int part)
+// One pass over the logits: a group of threads (8 lanes, a warp, a block, or the blocks of a cluster, which take `part` columns
+// each) holds a whole row in registers from its arrival to the gradient's store.  The maximum (of a block's part) comes first,
+// so that every exponential is taken once, relative to it.  Groups stay and walk over the rows.  Ahead: the next row travels to
+// shared memory while this one is worked on, so that the memory does not wait for the reductions and the row's scalars.
+template <bool Policy, bool Entropy, bool Aligned, bool Ahead, int Group, int V>
+__global__ void __launch_bounds__(Group < 256 ? 128 : Group, Group < 256 ? 8 : 1024 / Group) rows_held_kernel(const RowParams p, int part)
 {
-    constexpr int kWarps = Group / 32;
-    __shared__ float sh_max[kWarps];
-    __shared__ RowSums sh_warps[kWarps], sh_ranks[8];
+    constexpr int kThreads = Group < 256 ? 128 : Group, kWarps = kThreads / 32, kLanes = Group < 32 ? Group : 32;
+    using Part = RowPart<Group, V, Aligned>;
+    extern __shared__ float4 sh_quads[];
+    __shared__ float sh_max[kWarps], sh_target;
+    __shared__ RowSums sh_warps[kWarps];
     __shared__ RowGrad sh_grad;
-    const int ranks = Group == 32 ? 1 : cluster_size(), rank = Group == 32 ? 0 : cluster_rank();
-    if (ranks > 1) cluster_arrive();
-    const int tid = Group == 32 ? threadIdx.x & 31 : threadIdx.x;
-    const int row = Group == 32 ? blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x / ranks;
-    if (Group == 32 && row >= p.M) return;
-    const int first = rank * part, n = max(0, min(part, p.N - first));
-    const float* x = p.logits + (size_t)row * p.ld + first;
-    float* dx = Policy && p.dlogits ? p.dlogits + (size_t)row * p.ld_d + first : nullptr;
-
-    const int t = p.targets[row];
-    float w = 1.0f;
-    if (Policy && p.weights) w = p.weights[row];
-    if (t < 0 || t >= p.N || w == 0.0f) {   // the same in every block of a cluster
-        if (tid == 0 && rank == 0) row_unused<Policy>(p, row, t >= p.N && w != 0.0f);
-        if (dx)
-            for (int j = tid; j < n; j += Group) __stcs(dx + j, 0.0f);
-        return;
-    }
-    RowPart<Group, V> r;
-    r.load(x, n, tid);
-    RowInputs in{};
-    if (tid == 0) in = row_inputs<Policy>(p, row, t);
-    if (Policy && !p.weights) w = 1.0f / *p.count;
-
-    RowSums sums{-CUDART_INF_F, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int k = 0; k < V; k++)
-        sums.mx = fmaxf(fmaxf(sums.mx, fmaxf(r.v[k][0], r.v[k][1])), fmaxf(r.v[k][2], r.v[k][3]));
-    const float own = sums.mx;
-    sums.mx = warp_max(sums.mx);
-    if (Group > 32) {
-        if ((tid & 31) == 0) sh_max[tid >> 5] = sums.mx;
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < kWarps; i++) sums.mx = fmaxf(sums.mx, sh_max[i]);
-    }
-    const float base = base_of(sums.mx);
-#pragma unroll
-    for (int k = 0; k < V; k++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            // with an entropy term t is clamped (0 * -inf is to be 0), and kept for the gradient, which takes 2^t again
-            const float t2 = (r.v[k][i] - base) * p.c, te = Entropy ? max_nan(t2, kNothing) : t2, e = exp2_fast(te);
-            sums.s += e;
-            if (Entropy) sums.u += te * e;
-            if (Policy) r.v[k][i] = Entropy ? te : e;
-            else if (Entropy) r.v[k][i] = te;
-            else r.v[k][i] = e;
+    __shared__ __align__(16) RowWord sh_word[2];
+    const int ranks = Group < 512 ? 1 : cluster_size(), rank = Group < 512 ? 0 : cluster_rank();
+    const int tid = Group < 256 ? threadIdx.x % Group : threadIdx.x;
+    const unsigned mask = Group < 32 ? ((1u << (Group & 31)) - 1) << (threadIdx.x & 31 & ~(Group - 1)) : kAllLanes;
+    const unsigned stride = Group < 256 ? gridDim.x * (kThreads / Group) : gridDim.x / ranks;
+    const int first = rank * part;
+    float4* mine = sh_quads + threadIdx.x;
+    if (Group >= 512 && ranks > 1) {   // the barriers must be there before a block writes to another
+        if (threadIdx.x == 0) {
+            mbar_init(smem_u32(&sh_word[0].bar), 1);
+            mbar_init(smem_u32(&sh_word[1].bar), 1);
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         }
-    if (own == base && sums.mx == base) {   // the few threads that hold the largest logit tell its ones from the rest
-        sums.s = 0.0f;
-#pragma unroll
-        for (int k = 0; k < V; k++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float e = Entropy ? exp2_fast(r.v[k][i]) : r.v[k][i];
-                if (e == 1.0f) sums.ties += 1.0f;
-                else sums.s += e;
+        cluster_sync_all();
+    }
+    unsigned row = Group < 256 ? blockIdx.x * (kThreads / Group) + threadIdx.x / Group : blockIdx.x / ranks;
+    unsigned uses = 0;   // rows of this group so far that are not left out
+    Part r;
+    RowHead cur = row_head<Policy>(p, row, tid == 0), nxt{-1, 0.0f, 0.0f, 0.0f, 0.0f};
+    if (Ahead) {
+        nxt = row_head<Policy>(p, row + stride, tid == 0);
+        const float* x = p.logits + (size_t)row * p.ld + first;
+        r.place(x, max(0, min(part, p.N - first)));
+        if (cur.used(p.N)) r.fetch(x, tid, mine, kThreads);
+    }
+    const float per_row = Policy && !p.weights ? 1.0f / *p.count : 0.0f;
+    for (; row < (unsigned)p.M; row += stride) {
+        const float* x = p.logits + (size_t)row * p.ld + first;
+        float* dx = Policy && p.dlogits ? p.dlogits + (size_t)row * p.ld_d + first : nullptr;
+        const int at = cur.t - first;      // the target's column in this block's part, if it is there
+        const bool used = cur.used(p.N);   // the same in every block of a cluster
+        r.place(x, max(0, min(part, p.N - first)));
+        float x_t = 0.0f, top = -CUDART_INF_F;
+        if (used) {
+            if (Ahead) {
+                r.take(mine, kThreads);
+                // the target's logit, from the thread that holds it
+                const int q = r.quad_of(at);
+                if (r.owns(at, tid)) x_t = reinterpret_cast<const float*>(mine + q / Group * kThreads)[(at - r.begin) & 3];
+                if (Group > 32) {
+                    if (r.owns(at, tid)) sh_target = x_t;
+                } else {
+                    x_t = __shfl_sync(mask, x_t, q % Group, kLanes);
+                }
+            } else {
+                r.load(x, tid);
+                if (tid == 0) x_t = p.logits[(size_t)row * p.ld + cur.t];   // before a gradient is written over it
             }
-    }
-    const RowSums all = join_row<Group>(sums, p.c, tid, ranks, rank, sh_warps, sh_ranks);
-    RowGrad g{};
-    if (tid == 0) g = row_scalars<Policy>(p, row, all, in, w, rank == 0, sums.mx);
-    if (!dx) return;
-    if (Group > 32) {
-        if (tid == 0) sh_grad = g;
-        __syncthreads();
-        g = sh_grad;
-    } else {
-        g.a = __shfl_sync(kAllLanes, g.a, 0);
-        g.b = __shfl_sync(kAllLanes, g.b, 0);
-        g.at_target = __shfl_sync(kAllLanes, g.at_target, 0);
-    }
 #pragma unroll
-    for (int k = 0; k < V; k++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            if (Entropy) r.v[k][i] = exp2_fast(r.v[k][i]) * (g.a + g.b * r.v[k][i]);
-            else r.v[k][i] *= g.a;
+            for (int k = 0; k < V; k++) top = fmaxf(fmaxf(top, fmaxf(r.v[k][0], r.v[k][1])), fmaxf(r.v[k][2], r.v[k][3]));
         }
-    r.store(dx, tid);
-    if (r.owns(t - first, tid)) dx[t - first] = g.at_target;
+        RowHead after{-1, 0.0f, 0.0f, 0.0f, 0.0f};
+        if (Ahead) {
+            if (nxt.used(p.N)) {
+                Part f;
+                f.place(x + (size_t)stride * p.ld, r.n);
+                f.fetch(x + (size_t)stride * p.ld, tid, mine, kThreads);
+            }
+            after = row_head<Policy>(p, row + 2 * stride, tid == 0);
+        }
+        if (used) {
+            RowSums sums{warp_max<kLanes>(top, mask), 0.0f, 0.0f, 0.0f};
+            if (Group > 32) {
+                if ((tid & 31) == 0) sh_max[tid >> 5] = sums.mx;
+                __syncthreads();
+                sums.mx = sh_max[0];
+#pragma unroll
+                for (int i = 1; i < kWarps; i++) sums.mx = fmaxf(sums.mx, sh_max[i]);
+            }
+            const float base = base_of(sums.mx);
+#pragma unroll
+            for (int k = 0; k < V; k++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    // with an entropy term t is clamped (0 * -inf is to be 0), and kept for the gradient, which takes 2^t again
+                    const float t2 = (r.v[k][i] - base) * p.c, te = Entropy ? max_nan(t2, kNothing) : t2, e = exp2_fast(te);
+                    sums.s += e;
+                    if (Entropy) sums.u += te * e;
+                    r.v[k][i] = Entropy ? te : e;
+                }
+            if (top == base) {   // the few threads that hold the largest logit tell its ones from the rest
+                const float with_ones = sums.s;
+                sums.s = 0.0f;
+#pragma unroll
+                for (int k = 0; k < V; k++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const float e = Entropy ? exp2_again(r.v[k][i]) : r.v[k][i];
+                        if (!(e == 1.0f)) sums.s += e;
+                    }
+                sums.ties = rintf(with_ones - sums.s);
+            }
+            sums = join_lanes<kLanes>(sums, p.c, mask);
+            const float from = sums.mx;
+            RowGrad g{};
+            if (Group > 32) {
+                if ((tid & 31) == 0) sh_warps[tid >> 5] = sums;
+                __syncthreads();
+                if (tid < 32) {
+                    const RowSums none{-CUDART_INF_F, 0.0f, 0.0f, 0.0f};
+                    sums = join_lanes(tid < kWarps ? sh_warps[tid] : none, p.c);
+                    x_t = Ahead ? sh_target : __shfl_sync(kAllLanes, x_t, 0);
+                    if (Group >= 512 && ranks > 1) {
+                        RowWord* word = sh_word + (uses & 1);
+                        exchange(word, sums, x_t, Ahead ? at >= 0 && at < r.n : rank == 0, ranks, rank, (uses >> 1) & 1, p.status);
+                        sums = join_lanes(tid < ranks ? word->sums[tid] : none, p.c);
+                        x_t = word->x_t;
+                    }
+                }
+            }
+            uses++;
+            if (tid == 0) g = row_scalars<Policy>(p, row, sums, cur, x_t, p.weights ? cur.w : per_row, rank == 0, from);
+            if (dx) {
+                if (Group > 32) {
+                    if (tid == 0) sh_grad = g;
+                    __syncthreads();
+                    g = sh_grad;
+                } else {
+                    g.a = __shfl_sync(mask, g.a, 0, kLanes);
+                    g.b = __shfl_sync(mask, g.b, 0, kLanes);
+                    g.at_target = __shfl_sync(mask, g.at_target, 0, kLanes);
+                }
+#pragma unroll
+                for (int k = 0; k < V; k++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        if (Entropy) r.v[k][i] = exp2_again(r.v[k][i]) * (g.a + g.b * r.v[k][i]);
+                        else r.v[k][i] *= g.a;
+                    }
+                r.store(dx, tid);
+                if (r.owns(at, tid)) dx[at] = g.at_target;
+            }
+        } else {
+            if (tid == 0 && rank == 0) row_unused<Policy>(p, row, cur.t >= p.N && cur.w != 0.0f);
+            if (dx) r.clear(dx, tid);
+        }
+        if (Ahead) {
+            cur = nxt;
+            nxt = after;
+        } else {
+            cur = row_head<Policy>(p, row + stride, tid == 0);
+        }
+    }
 }
 
-// Rows that need not be held (no gradient is asked for) or cannot be (longer than a cluster's registers): a block, or a cluster
-// of blocks, walks over the row with running sums per thread, and a second time for the gradient.
-template <bool Policy, bool Entropy>
-__global__ void __launch_bounds__(256) rows_walk_kernel(const RowParams p, int part)
+// Rows that need not be held (log-probabilities alone) or cannot be (longer than a cluster's registers): a block walks over the
+// row with running sums per thread, and a second time for the gradient; short calls give a row to a cluster of blocks.
+template <bool Policy, bool Entropy, bool Aligned, int Threads>
+__global__ void __launch_bounds__(Threads) rows_walk_kernel(const RowParams p, int part)
 {
-    constexpr int kQuads = 4;
-    __shared__ RowSums sh_warps[8], sh_ranks[8];
+    constexpr int kQuads = 4, kWarps = Threads / 32;
+    using Part = RowPart<Threads, kQuads, Aligned>;
+    __shared__ RowSums sh_warps[kWarps];
     __shared__ RowGrad sh_grad;
+    __shared__ __align__(16) RowWord sh_word;
     const int ranks = cluster_size(), rank = cluster_rank(), tid = threadIdx.x;
-    if (ranks > 1) cluster_arrive();
+    if (ranks > 1) {
+        if (tid == 0) {
+            mbar_init(smem_u32(&sh_word.bar), 1);
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        }
+        cluster_sync_all();
+    }
     const int row = blockIdx.x / ranks, first = rank * part, n = max(0, min(part, p.N - first));
     const float* x = p.logits + (size_t)row * p.ld + first;
     float* dx = Policy && p.dlogits ? p.dlogits + (size_t)row * p.ld_d + first : nullptr;
-    const int t = p.targets[row];
-    float w = 1.0f;
-    if (Policy && p.weights) w = p.weights[row];
-    if (t < 0 || t >= p.N || w == 0.0f) {
-        if (tid == 0 && rank == 0) row_unused<Policy>(p, row, t >= p.N && w != 0.0f);
+    const RowHead in = row_head<Policy>(p, row, tid == 0);
+    const int at = in.t - first;
+    if (!in.used(p.N)) {
+        if (tid == 0 && rank == 0) row_unused<Policy>(p, row, in.t >= p.N && in.w != 0.0f);
         if (dx)
-            for (int j = tid; j < n; j += 256) __stcs(dx + j, 0.0f);
+            for (int j = tid; j < n; j += Threads) __stcs(dx + j, 0.0f);
         return;
     }
-    RowInputs in{};
-    if (tid == 0) in = row_inputs<Policy>(p, row, t);
-    if (Policy && !p.weights) w = 1.0f / *p.count;
+    const float w = Policy && !p.weights ? 1.0f / *p.count : in.w;
+    // before any gradient is written: dlogits may be the logits' own buffer
+    float x_t = tid == 0 ? p.logits[(size_t)row * p.ld + in.t] : 0.0f;
 
     RowSums sums{-CUDART_INF_F, 0.0f, 0.0f, 0.0f};
-    const int shift = (int)((uintptr_t)x >> 2) & 3, step = 4 * 256 * kQuads;
-    for (int j0 = -shift; j0 < n; j0 += step) {
-        RowPart<256, kQuads> r;
-        r.load_from(x, n, j0, tid);
+    Part r;
+    constexpr int kStep = 4 * Threads * kQuads;
+#pragma unroll 1
+    for (r.place(x, n); r.begin < n; r.begin += kStep) {
+        r.load(x, tid);
         float mx = sums.mx;
 #pragma unroll
         for (int k = 0; k < kQuads; k++)
@@ -477,15 +632,25 @@ __global__ void __launch_bounds__(256) rows_walk_kernel(const RowParams p, int p
                 if (Entropy) sums.u += te * e;
             }
     }
-    const RowSums all = join_row<256>(sums, p.c, tid, ranks, rank, sh_warps, sh_ranks);
-    if (tid == 0) sh_grad = row_scalars<Policy>(p, row, all, in, w, rank == 0, all.mx);
+    sums = join_lanes(sums, p.c);
+    if ((tid & 31) == 0) sh_warps[tid >> 5] = sums;
+    __syncthreads();
+    if (tid < 32) {
+        const RowSums none{-CUDART_INF_F, 0.0f, 0.0f, 0.0f};
+        sums = join_lanes(tid < kWarps ? sh_warps[tid] : none, p.c);
+        if (ranks > 1) {
+            exchange(&sh_word, sums, __shfl_sync(kAllLanes, x_t, 0), rank == 0, ranks, rank, 0, p.status);
+            sums = join_lanes(tid < ranks ? sh_word.sums[tid] : none, p.c);
+        }
+        if (tid == 0) sh_grad = row_scalars<Policy>(p, row, sums, in, x_t, w, rank == 0, sums.mx);
+    }
     if (!dx) return;
     __syncthreads();
     const RowGrad g = sh_grad;
     const float base = base_of(g.mx);
-    for (int j0 = -shift; j0 < n; j0 += step) {
-        RowPart<256, kQuads> r;
-        r.load_from(x, n, j0, tid);
+#pragma unroll 1
+    for (r.place(x, n); r.begin < n; r.begin += kStep) {
+        r.load(x, tid);
 #pragma unroll
         for (int k = 0; k < kQuads; k++)
 #pragma unroll
@@ -494,20 +659,20 @@ __global__ void __launch_bounds__(256) rows_walk_kernel(const RowParams p, int p
                 r.v[k][i] = exp2_fast(te) * (g.a + g.b * te);
             }
         r.store(dx, tid);
-        if (r.owns(t - first, tid)) dx[t - first] = g.at_target;
+        if (r.owns(at, tid)) dx[at] = g.at_target;
     }
 }
 
 // dlogits of the log-probabilities from the forward's statistics.  A group of threads takes 4 * Group * V columns of a row;
 // every load of the logits, and of the gradient that is added to, is under way before the first result is made.
-template <bool Accumulate, int Group, int V>
-__global__ void __launch_bounds__(Group == 32 ? 128 : Group)
+template <bool Accumulate, bool Aligned, int Group, int V>
+__global__ void __launch_bounds__(Group < 256 ? 128 : Group)
 logprob_bwd_kernel(const float* logits, long long ld, const int32_t* __restrict__ targets, float it,
                    const float* __restrict__ stats, const float* __restrict__ entropy, const float* __restrict__ dlogp,
                    const float* __restrict__ dentropy, float* dlogits, long long ld_d, int M, int N, int parts, int part)
 {
-    const int tid = Group == 32 ? threadIdx.x & 31 : threadIdx.x;
-    const unsigned unit = Group == 32 ? blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x;
+    const int tid = Group < 256 ? threadIdx.x % Group : threadIdx.x;
+    const unsigned unit = Group < 256 ? blockIdx.x * (128 / Group) + threadIdx.x / Group : blockIdx.x;
     const int row = (int)(unit / (unsigned)parts), first = (int)(unit % (unsigned)parts) * part, n = min(part, N - first);
     if (row >= M) return;
     const float* x = logits + (size_t)row * ld + first;
@@ -519,9 +684,10 @@ logprob_bwd_kernel(const float* logits, long long ld, const int32_t* __restrict_
             for (int j = tid; j < n; j += Group) __stcs(dx + j, 0.0f);
         return;
     }
-    RowPart<Group, V> r;
+    RowPart<Group, V, Aligned> r;
     float old[V][4];
-    r.load(x, n, tid);
+    r.place(x, n);
+    r.load(x, tid);
     if (Accumulate) r.load_beside(dx, tid, old);
     // p_j (-G - E (log p_j + H)) with p_j = 2^t / s, log p_j = log(2) t - log s
     const float G = it * (dlogp ? dlogp[row] : 0.0f), E = it * (dentropy ? dentropy[row] : 0.0f);
@@ -631,11 +797,13 @@ using namespace znn;
 // Columns that a group can take whatever their alignment: up to three floats lie before the first column of a part.
 static constexpr int room(int group, int v, bool aligned) { return 4 * group * v - (aligned ? 0 : 3); }
 
-static int launch_rows_kernel(void (*kernel)(RowParams, int), const RowParams& p, long long blocks, int threads, int ranks, int part)
+static int launch_rows_kernel(void (*kernel)(RowParams, int), const RowParams& p, long long blocks, int threads, int ranks, int part,
+                              size_t shared)
 {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)blocks);
     cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = shared;
     cfg.stream = stream();
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeClusterDimension;
@@ -647,43 +815,130 @@ static int launch_rows_kernel(void (*kernel)(RowParams, int), const RowParams& p
     return ZNN_OK;
 }
 
-template <bool Policy, bool Entropy, int Group, int V>
-static int launch_held(const RowParams& p, int ranks, int part)
+// Blocks (or clusters of `ranks` blocks) of the kernel that run on the device at a time: asked of the driver once per device.
+template <class Kernel>
+static int resident(Kernel* kernel, int threads, size_t shared, int ranks, std::atomic<int> (&known)[16], int* out)
 {
-    return launch_rows_kernel(rows_held_kernel<Policy, Entropy, Group, V>, p, Group == 32 ? (p.M + 3LL) / 4 : (long long)p.M * ranks,
-                              Group == 32 ? 128 : Group, ranks, part);
+    int dev = 0;
+    ZNN_CUDA_OK(cudaGetDevice(&dev));
+    ZNN_REQUIRE(dev >= 0 && dev < 16, "device index %d out of range", dev);
+    int n = known[dev].load(std::memory_order_acquire);
+    if (n == 0) {
+        ZNN_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared));
+        if (ranks == 1) {
+            ZNN_CUDA_OK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, shared));
+            n *= sm_count();
+        } else {
+            cudaLaunchConfig_t cfg{};
+            cfg.gridDim = dim3((unsigned)(ranks * sm_count()));
+            cfg.blockDim = dim3(threads);
+            cfg.dynamicSmemBytes = shared;
+            cudaLaunchAttribute attr{};
+            attr.id = cudaLaunchAttributeClusterDimension;
+            attr.val.clusterDim = {(unsigned)ranks, 1, 1};
+            cfg.attrs = &attr;
+            cfg.numAttrs = 1;
+            ZNN_CUDA_OK(cudaOccupancyMaxActiveClusters(&n, kernel, &cfg));
+        }
+        if (n < 1) return fail(ZNN_ERR_CUDA, "the rows kernel does not fit the device");
+        known[dev].store(n, std::memory_order_release);
+    }
+    *out = n;
+    return ZNN_OK;
 }
 
-template <bool Policy, bool Entropy>
-static int launch_rows(const RowParams& p)
+#ifndef ZNN_AHEAD
+#define ZNN_AHEAD 1
+#endif
+template <bool Policy, bool Entropy, bool Aligned, int Group, int V, int Ranks>
+static int launch_held(const RowParams& p, int part)
 {
-    const bool aligned = ((uintptr_t)p.logits & 15) == 0 && p.ld % 4 == 0;
-    // a warp per row while a row fits one; then a block; then a cluster of blocks; then two walks
-    if (p.N <= room(32, 2, aligned)) return launch_held<Policy, Entropy, 32, 2>(p, 1, p.N);
-    if (p.N <= room(32, 8, aligned)) return launch_held<Policy, Entropy, 32, 8>(p, 1, p.N);
-    if (p.N <= room(256, 4, aligned)) return launch_held<Policy, Entropy, 256, 4>(p, 1, p.N);
-    if (p.N <= room(256, 8, aligned)) return launch_held<Policy, Entropy, 256, 8>(p, 1, p.N);
-    // (the policy loss without a gradient takes the same way, so that it gives the same bits)
-    for (int ranks = 1; Policy && ranks <= 8; ranks *= 2) {
-        const int part = (ceil_div(p.N, ranks) + 3) & ~3;   // parts start where the row's quads do
-        if (part <= room(512, 8, aligned)) return launch_held<Policy, Entropy, 512, 8>(p, ranks, part);
-    }
+    constexpr bool ahead = ZNN_AHEAD;
+    constexpr int threads = Group < 256 ? 128 : Group, rows = threads / Group;
+    constexpr size_t shared = ahead ? (size_t)threads * V * sizeof(float4) : 0;
+    static std::atomic<int> known[16];
+    auto kernel = rows_held_kernel<Policy, Entropy, Aligned, ahead, Group, V>;
+    const long long want = (p.M + (long long)rows - 1) / rows;
+    int most = 0;
+    const int rc = resident(kernel, threads, shared, Ranks, known, &most);
+    if (rc != ZNN_OK) return rc;
+    return launch_rows_kernel(kernel, p, (ahead ? std::min<long long>(want, most) : want) * Ranks, threads, Ranks, part, shared);
+}
+
+template <bool Policy, bool Entropy, bool Aligned, int Threads>
+static int launch_walk(const RowParams& p)
+{
+    // a block per row, unless that leaves most of the device idle
     int ranks = Policy ? 8 : 1;
     while (ranks < 8 && (long long)p.M * ranks < 4 * sm_count()) ranks *= 2;
-    return launch_rows_kernel(rows_walk_kernel<Policy, Entropy>, p, (long long)p.M * ranks, 256, ranks, (ceil_div(p.N, ranks) + 3) & ~3);
+    const int part = (ceil_div(p.N, ranks) + 3) & ~3;   // parts start where the row's quads do
+    return launch_rows_kernel(rows_walk_kernel<Policy, Entropy, Aligned, Threads>, p, (long long)p.M * ranks, Threads, ranks, part, 0);
 }
 
-template <bool Accumulate, int Group, int V>
-static int launch_bwd(const float* logits, long long ld, const int32_t* targets, float it, const float* stats, const float* entropy,
-                      const float* dlogp, const float* dentropy, float* dlogits, long long ld_d, int M, int N, bool aligned)
+template <bool Policy, bool Entropy, bool Aligned>
+static int launch_rows_as(const RowParams& p)
 {
-    const int fit = room(Group, V, aligned) & ~3, parts = ceil_div(N, fit), part = (ceil_div(N, parts) + 3) & ~3;
-    const long long units = (long long)M * ceil_div(N, part);
-    const unsigned grid = (unsigned)(Group == 32 ? (units + 3) / 4 : units);
-    logprob_bwd_kernel<Accumulate, Group, V><<<grid, Group == 32 ? 128 : Group, 0, stream()>>>(
-        logits, ld, targets, it, stats, entropy, dlogp, dentropy, dlogits, ld_d, M, N, ceil_div(N, part), part);
+    // 8 lanes per row while a row fits them; then a warp; then a block; then a cluster of blocks; then two walks
+    if (p.N <= room(8, 2, Aligned)) return launch_held<Policy, Entropy, Aligned, 8, 2, 1>(p, p.N);
+    if (p.N <= room(8, 8, Aligned)) return launch_held<Policy, Entropy, Aligned, 8, 8, 1>(p, p.N);
+    if (p.N <= room(32, 8, Aligned)) return launch_held<Policy, Entropy, Aligned, 32, 8, 1>(p, p.N);
+    if constexpr (Policy) {   // (without a gradient as with one, so that the loss has the same bits)
+        auto part = [&](int ranks) { return (ceil_div(p.N, ranks) + 3) & ~3; };   // parts start where the row's quads do
+        if (p.N <= room(256, 4, Aligned)) return launch_held<Policy, Entropy, Aligned, 256, 4, 1>(p, p.N);
+        if (p.N <= room(256, 8, Aligned)) return launch_held<Policy, Entropy, Aligned, 256, 8, 1>(p, p.N);
+        if (part(1) <= room(512, 8, Aligned)) return launch_held<Policy, Entropy, Aligned, 512, 8, 1>(p, part(1));
+        if (part(2) <= room(512, 8, Aligned)) return launch_held<Policy, Entropy, Aligned, 512, 8, 2>(p, part(2));
+        if (part(4) <= room(512, 8, Aligned)) return launch_held<Policy, Entropy, Aligned, 512, 8, 4>(p, part(4));
+        if (part(8) <= room(512, 8, Aligned)) return launch_held<Policy, Entropy, Aligned, 512, 8, 8>(p, part(8));
+    }
+    if (!Policy && p.N <= 2048) return launch_walk<Policy, Entropy, Aligned, 64>(p);
+    if (!Policy && p.N <= 4096) return launch_walk<Policy, Entropy, Aligned, 128>(p);
+    return launch_walk<Policy, Entropy, Aligned, 256>(p);
+}
+
+// every row of the matrix starts with a 16-byte quad and has whole quads only
+static bool rows_aligned(const float* m, long long ld, int N) { return ((uintptr_t)m & 15) == 0 && ld % 4 == 0 && N % 4 == 0; }
+
+template <bool Policy>
+static int launch_rows(const RowParams& p, bool entropy)
+{
+    if (rows_aligned(p.logits, p.ld, p.N) && (!p.dlogits || rows_aligned(p.dlogits, p.ld_d, p.N)))
+        return entropy ? launch_rows_as<Policy, true, true>(p) : launch_rows_as<Policy, false, true>(p);
+    return entropy ? launch_rows_as<Policy, true, false>(p) : launch_rows_as<Policy, false, false>(p);
+}
+
+struct BwdArgs {
+    const float* logits;
+    long long ld;
+    const int32_t* targets;
+    float it;
+    const float *stats, *entropy, *dlogp, *dentropy;
+    float* dlogits;
+    long long ld_d;
+    int M, N;
+};
+
+template <bool Accumulate, bool Aligned, int Group, int V>
+static int launch_bwd(const BwdArgs& b)
+{
+    constexpr int rows = Group < 256 ? 128 / Group : 1;
+    const int fit = room(Group, V, Aligned) & ~3, part = (ceil_div(b.N, ceil_div(b.N, fit)) + 3) & ~3, parts = ceil_div(b.N, part);
+    const long long units = (long long)b.M * parts;
+    logprob_bwd_kernel<Accumulate, Aligned, Group, V><<<(unsigned)((units + rows - 1) / rows), Group < 256 ? 128 : Group, 0, stream()>>>(
+        b.logits, b.ld, b.targets, b.it, b.stats, b.entropy, b.dlogp, b.dentropy, b.dlogits, b.ld_d, b.M, b.N, parts, part);
     ZNN_LAUNCH_OK("logprob_bwd_kernel");
     return ZNN_OK;
+}
+
+template <bool Accumulate, bool Aligned>
+static int launch_bwd_as(const BwdArgs& b)
+{
+    if (b.N <= (room(8, 2, Aligned) & ~3)) return launch_bwd<Accumulate, Aligned, 8, 2>(b);
+    if (b.N <= (room(8, 4, Aligned) & ~3)) return launch_bwd<Accumulate, Aligned, 8, 4>(b);
+    if (b.N <= (room(32, 4, Aligned) & ~3)) return launch_bwd<Accumulate, Aligned, 32, 4>(b);
+    if (b.N <= (room(32, 8, Aligned) & ~3)) return launch_bwd<Accumulate, Aligned, 32, 8>(b);
+    if (b.N <= (room(256, 2, Aligned) & ~3)) return launch_bwd<Accumulate, Aligned, 256, 2>(b);
+    return launch_bwd<Accumulate, Aligned, 256, 4>(b);
 }
 
 static int check_rows(const float* logits, long long ld, const int32_t* targets, float inv_temp, int M, int N)
@@ -708,7 +963,7 @@ int znn_token_logprob_fwd(const float* logits, long long ld, const int32_t* targ
     RowParams p{};
     p.logits = logits; p.ld = ld; p.targets = targets; p.it = inv_temp; p.c = (float)(inv_temp * 1.4426950408889634); p.M = M; p.N = N;
     p.logp = logp; p.entropy = entropy; p.stats = stats; p.status = device_status_word();
-    return entropy ? launch_rows<false, true>(p) : launch_rows<false, false>(p);
+    return launch_rows<false>(p, entropy != nullptr);
 }
 
 int znn_token_logprob_bwd(const float* logits, long long ld, const int32_t* targets, float inv_temp, const float* stats,
@@ -723,12 +978,9 @@ int znn_token_logprob_bwd(const float* logits, long long ld, const int32_t* targ
     ZNN_REQUIRE(ld_d >= N, "ld_d = %lld is smaller than N = %d", ld_d, N);
     ZNN_REQUIRE(dlogits != logits || (ld_d == ld && !accumulate), "dlogits may be the logits' own buffer only with ld_d == ld and accumulate = 0");
     ZNN_NEED_DEVICE();
-    const bool aligned = ((uintptr_t)logits & 15) == 0 && ld % 4 == 0;
-#define ZNN_BWD(acc, group, v) \
-    launch_bwd<acc, group, v>(logits, ld, targets, inv_temp, stats, entropy, dlogp, dentropy, dlogits, ld_d, M, N, aligned)
-    if (N <= room(32, 4, aligned)) return accumulate ? ZNN_BWD(true, 32, 4) : ZNN_BWD(false, 32, 4);
-    return accumulate ? ZNN_BWD(true, 256, 4) : ZNN_BWD(false, 256, 4);
-#undef ZNN_BWD
+    const BwdArgs b{logits, ld, targets, inv_temp, stats, entropy, dlogp, dentropy, dlogits, ld_d, M, N};
+    if (rows_aligned(logits, ld, N) && rows_aligned(dlogits, ld_d, N)) return accumulate ? launch_bwd_as<true, true>(b) : launch_bwd_as<false, true>(b);
+    return accumulate ? launch_bwd_as<true, false>(b) : launch_bwd_as<false, false>(b);
 }
 
 int znn_policy_loss(const float* logits, long long ld, const int32_t* targets, float inv_temp, const float* old_logp,
@@ -757,7 +1009,7 @@ int znn_policy_loss(const float* logits, long long ld, const int32_t* targets, f
         policy_total_kernel<<<1, 1024, 0, stream()>>>(targets, weights, token_loss, loss, M, 0);
         ZNN_LAUNCH_OK("policy_total_kernel");
     }
-    const int done = entropy || entropy_coef != 0.0f ? launch_rows<true, true>(p) : launch_rows<true, false>(p);
+    const int done = launch_rows<true>(p, entropy || entropy_coef != 0.0f);
     if (done != ZNN_OK) return done;
     policy_total_kernel<<<1, 1024, 0, stream()>>>(targets, weights, token_loss, loss, M, 1);
     ZNN_LAUNCH_OK("policy_total_kernel");
