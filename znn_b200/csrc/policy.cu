@@ -6,7 +6,6 @@
 #include <math_constants.h>
 
 #include <algorithm>
-#include <atomic>
 
 #include "common.cuh"
 #include "tc_ptx.cuh"
@@ -120,6 +119,11 @@ __device__ __forceinline__ double exp_of(double x)
 }
 __device__ __forceinline__ double expm1_of(double x) { return x > 80.0 ? exp_of(x) : (double)expm1f((float)x); }
 
+// A kernel that was launched with `overlap` may begin while the one before it still runs: it waits here before it reads what that
+// one writes.  That one lets it begin as soon as all of its own blocks run.
+__device__ __forceinline__ void wait_for_previous_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next_kernel_begin() { asm volatile("griddepcontrol.launch_dependents;"); }
+
 struct RowParams {
     const float* logits;
     long long ld;
@@ -172,7 +176,7 @@ __device__ __forceinline__ RowHead row_head(const RowParams& p, unsigned row, bo
 // gradient's coefficients for a walk over logits measured from `from`.  The log-probability, and the differences that ratio and
 // KL term are made of, are fp64: fp32 would leave a ratio of two probabilities of e^-10 an error of 1e-6.
 template <bool Policy>
-__device__ __forceinline__ RowGrad row_scalars(const RowParams& p, int row, const RowSums& r, const RowHead& in, float x_t, float w,
+__device__ __forceinline__ RowGrad row_scalars(const RowParams& p, int row, const RowSums& r, const RowHead& in, float x_t,
                                                bool write, float from)
 {
     const float total = r.ties + r.s;
@@ -187,6 +191,11 @@ __device__ __forceinline__ RowGrad row_scalars(const RowParams& p, int row, cons
     }
     RowGrad g{0.0f, 0.0f, 0.0f, from};
     if (Policy) {
+        float w = in.w;
+        if (!p.weights) {
+            wait_for_previous_kernel();   // which counts the rows while this one reads the logits
+            w = 1.0f / *p.count;
+        }
         const double A = in.advantage;
         double loss = 0.0, slope = 0.0;
         if (A != 0.0) {
@@ -264,44 +273,12 @@ struct RowPart {
         for (int k = 0; k < V; k++) {
             const int j = column(tid, k);
             if (whole(j)) {
-                const float4 q = __ldcs(reinterpret_cast<const float4*>(x + j));
+                const float4 q = __ldg(reinterpret_cast<const float4*>(x + j));
                 v[k][0] = q.x; v[k][1] = q.y; v[k][2] = q.z; v[k][3] = q.w;
             } else {
 #pragma unroll
-                for (int i = 0; i < 4; i++) v[k][i] = (!Aligned && j + i >= 0 && j + i < n) ? __ldcs(x + j + i) : -CUDART_INF_F;
+                for (int i = 0; i < 4; i++) v[k][i] = (!Aligned && j + i >= 0 && j + i < n) ? __ldg(x + j + i) : -CUDART_INF_F;
             }
-        }
-    }
-
-    // The part is copied to shared memory ahead of its use, every thread its own quads to places of its own (`mine`, `pitch`
-    // quads apart): only the thread itself waits for them, with no barrier.
-    __device__ __forceinline__ void fetch(const float* x, int tid, float4* mine, int pitch) const
-    {
-#pragma unroll
-        for (int k = 0; k < V; k++) {
-            const int j = column(tid, k);
-            const unsigned to = (unsigned)__cvta_generic_to_shared(mine + k * pitch);
-            if (whole(j)) {
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(x + j) : "memory");
-            } else if (Aligned) {
-                mine[k * pitch] = make_float4(-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F);
-            } else {
-#pragma unroll 1
-                for (int i = 0; i < 4; i++) {
-                    if (j + i >= 0 && j + i < n) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to + 4 * i), "l"(x + j + i) : "memory");
-                    else reinterpret_cast<float*>(mine + k * pitch)[i] = -CUDART_INF_F;
-                }
-            }
-        }
-    }
-
-    __device__ __forceinline__ void take(const float4* mine, int pitch)
-    {
-        asm volatile("cp.async.wait_all;" ::: "memory");
-#pragma unroll
-        for (int k = 0; k < V; k++) {
-            const float4 q = mine[k * pitch];
-            v[k][0] = q.x; v[k][1] = q.y; v[k][2] = q.z; v[k][3] = q.w;
         }
     }
 
@@ -316,11 +293,11 @@ struct RowPart {
         for (int k = 0; k < V; k++) {
             const int j = column(tid, k);
             if (quads && whole(j)) {
-                const float4 q = __ldcs(reinterpret_cast<const float4*>(y + j));
+                const float4 q = __ldg(reinterpret_cast<const float4*>(y + j));
                 o[k][0] = q.x; o[k][1] = q.y; o[k][2] = q.z; o[k][3] = q.w;
             } else {
 #pragma unroll
-                for (int i = 0; i < 4; i++) o[k][i] = (!Aligned && j + i >= 0 && j + i < n) ? __ldcs(y + j + i) : 0.0f;
+                for (int i = 0; i < 4; i++) o[k][i] = (!Aligned && j + i >= 0 && j + i < n) ? __ldg(y + j + i) : 0.0f;
             }
         }
     }
@@ -381,202 +358,109 @@ __device__ __forceinline__ int cluster_rank()
     return (int)r;
 }
 
-// The sums of every block's part of a row, written by the blocks themselves, with the target's logit from the one that has it.
-// Two such places take turns, so that a block may be one row ahead of another: it cannot be two ahead, since the row between
-// needs the other's word.
+__device__ __forceinline__ void cluster_store(double* place, int rank, double v)
+{
+    asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(mapa_shared(smem_u32(place), (uint32_t)rank)), "d"(v) : "memory");
+}
+
+// The sums of every block's part of a row, written by the blocks themselves.
 struct RowWord {
     RowSums sums[8];
-    float x_t;
     unsigned long long bar;
 };
 
-// Sends this block's sums (and x_t, where `has_target`) to every block of the cluster and waits for theirs; all lanes of one
-// warp call it.  The stores count on the receiver's barrier as they land: no fence waits for the gradients that are on their
-// way to memory.  parity: of the number of rows that have used this place.
-__device__ __forceinline__ void exchange(RowWord* word, const RowSums& mine, float x_t, bool has_target, int ranks, int rank, unsigned parity, int* status)
+// Sends this block's sums to every block of the cluster and waits for theirs; all lanes of one warp call it.  The stores count
+// on the receiver's barrier as they land.
+__device__ __forceinline__ void exchange(RowWord* word, const RowSums& mine, int ranks, int rank, int* status)
 {
     const int lane = threadIdx.x & 31;
-    const uint32_t bar = smem_u32(&word->bar), sums = smem_u32(&word->sums[rank]), target = smem_u32(&word->x_t);
-    if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)(ranks * sizeof(RowSums) + sizeof(float)));
+    const uint32_t bar = smem_u32(&word->bar), sums = smem_u32(&word->sums[rank]);
+    if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)(ranks * sizeof(RowSums)));
     if (lane < ranks) {
         const uint32_t there = mapa_shared(bar, lane);
         asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(mapa_shared(sums, lane)),
                      "f"(mine.mx), "f"(mine.ties), "f"(mine.s), "f"(mine.u), "r"(there)
                      : "memory");
-        if (has_target)
-            asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.f32 [%0], %1, [%2];" ::"r"(mapa_shared(target, lane)), "f"(x_t), "r"(there)
-                         : "memory");
     }
-    // (every block of the cluster runs and takes the same rows: the wait ends.  Its limit is there for what nobody foresees; the
+    // (every block of the cluster runs and comes here: the wait ends.  Its limit is there for what nobody foresees; the
     // row is then made of what has arrived, and the status word says so)
-    if (!mbar_wait_bounded_cluster(bar, parity, kWaitLimitCycles) && status) atomicOr(status, ZNN_DEV_TMA_WAIT_EXPIRED);
+    if (!mbar_wait_bounded_cluster(bar, 0, kWaitLimitCycles) && status) atomicOr(status, ZNN_DEV_TMA_WAIT_EXPIRED);
     __syncwarp();
 }
 
-// One pass over the logits: a group of threads (8 lanes, a warp, a block, or the blocks of a cluster, which take `part` columns
-// each) holds a whole row in registers from its arrival to the gradient's store.  The maximum (of a block's part) comes first,
-// so that every exponential is taken once, relative to it.  Groups stay and walk over the rows.  Ahead: the next row travels to
-// shared memory while this one is worked on, so that the memory does not wait for the reductions and the row's scalars.
-template <bool Policy, bool Entropy, bool Aligned, bool Ahead, int Group, int V>
-__global__ void __launch_bounds__(Group < 256 ? 128 : Group, Group < 256 ? 8 : 1024 / Group) rows_held_kernel(const RowParams p, int part)
+// Short rows: 8 lanes or a warp hold a whole row in registers from its load to the gradient's store.  The maximum comes first, so
+// that every exponential is taken once, relative to it.
+template <bool Policy, bool Entropy, bool Aligned, int Group, int V>
+__global__ void __launch_bounds__(128) rows_held_kernel(const RowParams p, int)
 {
-    constexpr int kThreads = Group < 256 ? 128 : Group, kWarps = kThreads / 32, kLanes = Group < 32 ? Group : 32;
-    using Part = RowPart<Group, V, Aligned>;
-    extern __shared__ float4 sh_quads[];
-    __shared__ float sh_max[kWarps], sh_target;
-    __shared__ RowSums sh_warps[kWarps];
-    __shared__ RowGrad sh_grad;
-    __shared__ __align__(16) RowWord sh_word[2];
-    const int ranks = Group < 512 ? 1 : cluster_size(), rank = Group < 512 ? 0 : cluster_rank();
-    const int tid = Group < 256 ? threadIdx.x % Group : threadIdx.x;
+    const int tid = threadIdx.x % Group;
     const unsigned mask = Group < 32 ? ((1u << (Group & 31)) - 1) << (threadIdx.x & 31 & ~(Group - 1)) : kAllLanes;
-    const unsigned stride = Group < 256 ? gridDim.x * (kThreads / Group) : gridDim.x / ranks;
-    const int first = rank * part;
-    float4* mine = sh_quads + threadIdx.x;
-    if (Group >= 512 && ranks > 1) {   // the barriers must be there before a block writes to another
-        if (threadIdx.x == 0) {
-            mbar_init(smem_u32(&sh_word[0].bar), 1);
-            mbar_init(smem_u32(&sh_word[1].bar), 1);
-            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        }
-        cluster_sync_all();
+    const unsigned row = blockIdx.x * (128 / Group) + threadIdx.x / Group;
+    if (row >= (unsigned)p.M) return;
+    const float* x = p.logits + (size_t)row * p.ld;
+    float* dx = Policy && p.dlogits ? p.dlogits + (size_t)row * p.ld_d : nullptr;
+    RowPart<Group, V, Aligned> r;
+    r.place(x, p.N);
+    const RowHead in = row_head<Policy>(p, row, tid == 0);
+    if (!in.used(p.N)) {
+        if (tid == 0) row_unused<Policy>(p, row, in.t >= p.N && in.w != 0.0f);
+        if (dx) r.clear(dx, tid);
+        return;
     }
-    unsigned row = Group < 256 ? blockIdx.x * (kThreads / Group) + threadIdx.x / Group : blockIdx.x / ranks;
-    unsigned uses = 0;   // rows of this group so far that are not left out
-    Part r;
-    RowHead cur = row_head<Policy>(p, row, tid == 0), nxt{-1, 0.0f, 0.0f, 0.0f, 0.0f};
-    if (Ahead) {
-        nxt = row_head<Policy>(p, row + stride, tid == 0);
-        const float* x = p.logits + (size_t)row * p.ld + first;
-        r.place(x, max(0, min(part, p.N - first)));
-        if (cur.used(p.N)) r.fetch(x, tid, mine, kThreads);
+    r.load(x, tid);
+    const float x_t = tid == 0 ? x[in.t] : 0.0f;   // before a gradient is written over it
+    float top = -CUDART_INF_F;
+#pragma unroll
+    for (int k = 0; k < V; k++) top = fmaxf(fmaxf(top, fmaxf(r.v[k][0], r.v[k][1])), fmaxf(r.v[k][2], r.v[k][3]));
+    RowSums sums{warp_max<Group>(top, mask), 0.0f, 0.0f, 0.0f};
+    const float base = base_of(sums.mx);
+#pragma unroll
+    for (int k = 0; k < V; k++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            // with an entropy term t is clamped (0 * -inf is to be 0), and kept for the gradient, which takes 2^t again
+            const float t2 = (r.v[k][i] - base) * p.c, te = Entropy ? max_nan(t2, kNothing) : t2, e = exp2_fast(te);
+            sums.s += e;
+            if (Entropy) sums.u += te * e;
+            r.v[k][i] = Entropy ? te : e;
+        }
+    if (top == base) {   // the few threads that hold the largest logit tell its ones from the rest
+        const float with_ones = sums.s;
+        sums.s = 0.0f;
+#pragma unroll
+        for (int k = 0; k < V; k++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float e = Entropy ? exp2_again(r.v[k][i]) : r.v[k][i];
+                if (!(e == 1.0f)) sums.s += e;
+            }
+        sums.ties = rintf(with_ones - sums.s);
     }
-    const float per_row = Policy && !p.weights ? 1.0f / *p.count : 0.0f;
-    for (; row < (unsigned)p.M; row += stride) {
-        const float* x = p.logits + (size_t)row * p.ld + first;
-        float* dx = Policy && p.dlogits ? p.dlogits + (size_t)row * p.ld_d + first : nullptr;
-        const int at = cur.t - first;      // the target's column in this block's part, if it is there
-        const bool used = cur.used(p.N);   // the same in every block of a cluster
-        r.place(x, max(0, min(part, p.N - first)));
-        float x_t = 0.0f, top = -CUDART_INF_F;
-        if (used) {
-            if (Ahead) {
-                r.take(mine, kThreads);
-                // the target's logit, from the thread that holds it
-                const int q = r.quad_of(at);
-                if (r.owns(at, tid)) x_t = reinterpret_cast<const float*>(mine + q / Group * kThreads)[(at - r.begin) & 3];
-                if (Group > 32) {
-                    if (r.owns(at, tid)) sh_target = x_t;
-                } else {
-                    x_t = __shfl_sync(mask, x_t, q % Group, kLanes);
-                }
-            } else {
-                r.load(x, tid);
-                if (tid == 0) x_t = p.logits[(size_t)row * p.ld + cur.t];   // before a gradient is written over it
-            }
+    const float from = sums.mx;
+    sums = join_lanes<Group>(sums, p.c, mask);
+    RowGrad g{};
+    if (tid == 0) g = row_scalars<Policy>(p, row, sums, in, x_t, true, from);
+    if (!dx) return;
+    g.a = __shfl_sync(mask, g.a, 0, Group);
+    g.b = __shfl_sync(mask, g.b, 0, Group);
+    g.at_target = __shfl_sync(mask, g.at_target, 0, Group);
 #pragma unroll
-            for (int k = 0; k < V; k++) top = fmaxf(fmaxf(top, fmaxf(r.v[k][0], r.v[k][1])), fmaxf(r.v[k][2], r.v[k][3]));
+    for (int k = 0; k < V; k++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if (Entropy) r.v[k][i] = exp2_again(r.v[k][i]) * (g.a + g.b * r.v[k][i]);
+            else r.v[k][i] *= g.a;
         }
-        RowHead after{-1, 0.0f, 0.0f, 0.0f, 0.0f};
-        if (Ahead) {
-            if (nxt.used(p.N)) {
-                Part f;
-                f.place(x + (size_t)stride * p.ld, r.n);
-                f.fetch(x + (size_t)stride * p.ld, tid, mine, kThreads);
-            }
-            after = row_head<Policy>(p, row + 2 * stride, tid == 0);
-        }
-        if (used) {
-            RowSums sums{warp_max<kLanes>(top, mask), 0.0f, 0.0f, 0.0f};
-            if (Group > 32) {
-                if ((tid & 31) == 0) sh_max[tid >> 5] = sums.mx;
-                __syncthreads();
-                sums.mx = sh_max[0];
-#pragma unroll
-                for (int i = 1; i < kWarps; i++) sums.mx = fmaxf(sums.mx, sh_max[i]);
-            }
-            const float base = base_of(sums.mx);
-#pragma unroll
-            for (int k = 0; k < V; k++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    // with an entropy term t is clamped (0 * -inf is to be 0), and kept for the gradient, which takes 2^t again
-                    const float t2 = (r.v[k][i] - base) * p.c, te = Entropy ? max_nan(t2, kNothing) : t2, e = exp2_fast(te);
-                    sums.s += e;
-                    if (Entropy) sums.u += te * e;
-                    r.v[k][i] = Entropy ? te : e;
-                }
-            if (top == base) {   // the few threads that hold the largest logit tell its ones from the rest
-                const float with_ones = sums.s;
-                sums.s = 0.0f;
-#pragma unroll
-                for (int k = 0; k < V; k++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const float e = Entropy ? exp2_again(r.v[k][i]) : r.v[k][i];
-                        if (!(e == 1.0f)) sums.s += e;
-                    }
-                sums.ties = rintf(with_ones - sums.s);
-            }
-            sums = join_lanes<kLanes>(sums, p.c, mask);
-            const float from = sums.mx;
-            RowGrad g{};
-            if (Group > 32) {
-                if ((tid & 31) == 0) sh_warps[tid >> 5] = sums;
-                __syncthreads();
-                if (tid < 32) {
-                    const RowSums none{-CUDART_INF_F, 0.0f, 0.0f, 0.0f};
-                    sums = join_lanes(tid < kWarps ? sh_warps[tid] : none, p.c);
-                    x_t = Ahead ? sh_target : __shfl_sync(kAllLanes, x_t, 0);
-                    if (Group >= 512 && ranks > 1) {
-                        RowWord* word = sh_word + (uses & 1);
-                        exchange(word, sums, x_t, Ahead ? at >= 0 && at < r.n : rank == 0, ranks, rank, (uses >> 1) & 1, p.status);
-                        sums = join_lanes(tid < ranks ? word->sums[tid] : none, p.c);
-                        x_t = word->x_t;
-                    }
-                }
-            }
-            uses++;
-            if (tid == 0) g = row_scalars<Policy>(p, row, sums, cur, x_t, p.weights ? cur.w : per_row, rank == 0, from);
-            if (dx) {
-                if (Group > 32) {
-                    if (tid == 0) sh_grad = g;
-                    __syncthreads();
-                    g = sh_grad;
-                } else {
-                    g.a = __shfl_sync(mask, g.a, 0, kLanes);
-                    g.b = __shfl_sync(mask, g.b, 0, kLanes);
-                    g.at_target = __shfl_sync(mask, g.at_target, 0, kLanes);
-                }
-#pragma unroll
-                for (int k = 0; k < V; k++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        if (Entropy) r.v[k][i] = exp2_again(r.v[k][i]) * (g.a + g.b * r.v[k][i]);
-                        else r.v[k][i] *= g.a;
-                    }
-                r.store(dx, tid);
-                if (r.owns(at, tid)) dx[at] = g.at_target;
-            }
-        } else {
-            if (tid == 0 && rank == 0) row_unused<Policy>(p, row, cur.t >= p.N && cur.w != 0.0f);
-            if (dx) r.clear(dx, tid);
-        }
-        if (Ahead) {
-            cur = nxt;
-            nxt = after;
-        } else {
-            cur = row_head<Policy>(p, row + stride, tid == 0);
-        }
-    }
+    r.store(dx, tid);
+    if (r.owns(in.t, tid)) dx[in.t] = g.at_target;
 }
 
 // Rows that need not be held (log-probabilities alone) or cannot be (longer than a cluster's registers): a block walks over the
 // row with running sums per thread, and a second time for the gradient; short calls give a row to a cluster of blocks.
-template <bool Policy, bool Entropy, bool Aligned, int Threads>
+template <bool Policy, bool Entropy, bool Aligned, int Threads, int kQuads>
 __global__ void __launch_bounds__(Threads) rows_walk_kernel(const RowParams p, int part)
 {
-    constexpr int kQuads = 4, kWarps = Threads / 32;
+    constexpr int kWarps = Threads / 32;
     using Part = RowPart<Threads, kQuads, Aligned>;
     __shared__ RowSums sh_warps[kWarps];
     __shared__ RowGrad sh_grad;
@@ -600,15 +484,15 @@ __global__ void __launch_bounds__(Threads) rows_walk_kernel(const RowParams p, i
             for (int j = tid; j < n; j += Threads) __stcs(dx + j, 0.0f);
         return;
     }
-    const float w = Policy && !p.weights ? 1.0f / *p.count : in.w;
     // before any gradient is written: dlogits may be the logits' own buffer
-    float x_t = tid == 0 ? p.logits[(size_t)row * p.ld + in.t] : 0.0f;
+    const float x_t = tid == 0 ? p.logits[(size_t)row * p.ld + in.t] : 0.0f;
 
     RowSums sums{-CUDART_INF_F, 0.0f, 0.0f, 0.0f};
     Part r;
     constexpr int kStep = 4 * Threads * kQuads;
+    r.place(x, n);
 #pragma unroll 1
-    for (r.place(x, n); r.begin < n; r.begin += kStep) {
+    for (;;) {
         r.load(x, tid);
         float mx = sums.mx;
 #pragma unroll
@@ -631,6 +515,8 @@ __global__ void __launch_bounds__(Threads) rows_walk_kernel(const RowParams p, i
                 else sums.s += e;
                 if (Entropy) sums.u += te * e;
             }
+        if (r.begin + kStep >= n) break;
+        r.begin += kStep;
     }
     sums = join_lanes(sums, p.c);
     if ((tid & 31) == 0) sh_warps[tid >> 5] = sums;
@@ -639,18 +525,18 @@ __global__ void __launch_bounds__(Threads) rows_walk_kernel(const RowParams p, i
         const RowSums none{-CUDART_INF_F, 0.0f, 0.0f, 0.0f};
         sums = join_lanes(tid < kWarps ? sh_warps[tid] : none, p.c);
         if (ranks > 1) {
-            exchange(&sh_word, sums, __shfl_sync(kAllLanes, x_t, 0), rank == 0, ranks, rank, 0, p.status);
+            exchange(&sh_word, sums, ranks, rank, p.status);
             sums = join_lanes(tid < ranks ? sh_word.sums[tid] : none, p.c);
         }
-        if (tid == 0) sh_grad = row_scalars<Policy>(p, row, sums, in, x_t, w, rank == 0, sums.mx);
+        if (tid == 0) sh_grad = row_scalars<Policy>(p, row, sums, in, x_t, rank == 0, sums.mx);
     }
     if (!dx) return;
     __syncthreads();
     const RowGrad g = sh_grad;
     const float base = base_of(g.mx);
+    // back from the end: the last step's logits are still here, the ones before it in the nearest caches
 #pragma unroll 1
-    for (r.place(x, n); r.begin < n; r.begin += kStep) {
-        r.load(x, tid);
+    for (;;) {
 #pragma unroll
         for (int k = 0; k < kQuads; k++)
 #pragma unroll
@@ -660,6 +546,9 @@ __global__ void __launch_bounds__(Threads) rows_walk_kernel(const RowParams p, i
             }
         r.store(dx, tid);
         if (r.owns(at, tid)) dx[at] = g.at_target;
+        r.begin -= kStep;
+        if (r.begin <= -kStep) break;
+        r.load(x, tid);
     }
 }
 
@@ -704,14 +593,19 @@ logprob_bwd_kernel(const float* logits, long long ld, const int32_t* __restrict_
     if (r.owns(t - first, tid)) dx[t - first] += G;
 }
 
-// loss[1] = rows in use; with_sum: loss[0] = sum of w_i token_loss_i as well.  One block, fixed order.
+// The number of rows that are not left out, and (with_sum) the sum of w_i token_loss_i; fixed order.  A cluster of blocks for
+// many rows.
 __global__ void __launch_bounds__(1024)
 policy_total_kernel(const int32_t* __restrict__ targets, const float* __restrict__ weights, const float* __restrict__ token_loss,
                     float* __restrict__ loss, int M, int with_sum)
 {
-    __shared__ double sh[32];
+    __shared__ double sh[32], sh_all[2][8];
+    const int ranks = cluster_size(), rank = cluster_rank();
+    if (ranks > 1) cluster_sync_all();   // a block must run before another writes to its memory
+    if (with_sum) wait_for_previous_kernel();
+    else let_next_kernel_begin();
     double count = 0.0, sum = 0.0;
-    for (int i = threadIdx.x; i < M; i += 1024) {
+    for (int i = rank * 1024 + threadIdx.x; i < M; i += ranks * 1024) {
         const float w = weights ? weights[i] : 1.0f;
         if (targets[i] < 0 || w == 0.0f) continue;
         count += 1.0;
@@ -719,7 +613,19 @@ policy_total_kernel(const int32_t* __restrict__ targets, const float* __restrict
     }
     count = block_sum(count, sh);
     if (with_sum) sum = block_sum(sum, sh);
-    if (threadIdx.x == 0) {
+    if (ranks > 1) {
+        if (threadIdx.x == 0) {
+            cluster_store(&sh_all[0][rank], 0, count);
+            cluster_store(&sh_all[1][rank], 0, sum);
+        }
+        cluster_sync_all();
+        count = sum = 0.0;
+        for (int i = 0; i < ranks; i++) {
+            count += sh_all[0][i];
+            sum += sh_all[1][i];
+        }
+    }
+    if (threadIdx.x == 0 && rank == 0) {
         loss[1] = (float)count;
         if (with_sum) loss[0] = (float)(weights ? sum : count > 0.0 ? sum / count : 0.0);
     }
@@ -797,103 +703,62 @@ using namespace znn;
 // Columns that a group can take whatever their alignment: up to three floats lie before the first column of a part.
 static constexpr int room(int group, int v, bool aligned) { return 4 * group * v - (aligned ? 0 : 3); }
 
-static int launch_rows_kernel(void (*kernel)(RowParams, int), const RowParams& p, long long blocks, int threads, int ranks, int part,
-                              size_t shared)
+// A launch in clusters of `ranks` blocks; overlap: it may begin while the kernel before it still runs.
+template <class... Params, class... Args>
+static int launch(void (*kernel)(Params...), const char* name, long long blocks, int threads, int ranks, bool overlap, Args... args)
 {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)blocks);
     cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = shared;
     cfg.stream = stream();
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim = {(unsigned)ranks, 1, 1};
-    cfg.attrs = &attr;
-    cfg.numAttrs = ranks > 1 ? 1 : 0;
-    ZNN_CUDA_OK(cudaLaunchKernelEx(&cfg, kernel, p, part));
-    ZNN_LAUNCH_OK("rows kernel");
-    return ZNN_OK;
-}
-
-// Blocks (or clusters of `ranks` blocks) of the kernel that run on the device at a time: asked of the driver once per device.
-template <class Kernel>
-static int resident(Kernel* kernel, int threads, size_t shared, int ranks, std::atomic<int> (&known)[16], int* out)
-{
-    int dev = 0;
-    ZNN_CUDA_OK(cudaGetDevice(&dev));
-    ZNN_REQUIRE(dev >= 0 && dev < 16, "device index %d out of range", dev);
-    int n = known[dev].load(std::memory_order_acquire);
-    if (n == 0) {
-        ZNN_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared));
-        if (ranks == 1) {
-            ZNN_CUDA_OK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, shared));
-            n *= sm_count();
-        } else {
-            cudaLaunchConfig_t cfg{};
-            cfg.gridDim = dim3((unsigned)(ranks * sm_count()));
-            cfg.blockDim = dim3(threads);
-            cfg.dynamicSmemBytes = shared;
-            cudaLaunchAttribute attr{};
-            attr.id = cudaLaunchAttributeClusterDimension;
-            attr.val.clusterDim = {(unsigned)ranks, 1, 1};
-            cfg.attrs = &attr;
-            cfg.numAttrs = 1;
-            ZNN_CUDA_OK(cudaOccupancyMaxActiveClusters(&n, kernel, &cfg));
-        }
-        if (n < 1) return fail(ZNN_ERR_CUDA, "the rows kernel does not fit the device");
-        known[dev].store(n, std::memory_order_release);
+    cudaLaunchAttribute attrs[2] = {};
+    if (ranks > 1) {
+        attrs[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        attrs[cfg.numAttrs++].val.clusterDim = {(unsigned)ranks, 1, 1};
     }
-    *out = n;
+    if (overlap) {
+        attrs[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attrs[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    cfg.attrs = attrs;
+    ZNN_CUDA_OK(cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...));
+    ZNN_LAUNCH_OK(name);
     return ZNN_OK;
 }
 
-#ifndef ZNN_AHEAD
-#define ZNN_AHEAD 1
-#endif
-template <bool Policy, bool Entropy, bool Aligned, int Group, int V, int Ranks>
-static int launch_held(const RowParams& p, int part)
+template <bool Policy, bool Entropy, bool Aligned, int Group, int V>
+static int launch_held(const RowParams& p)
 {
-    constexpr bool ahead = ZNN_AHEAD;
-    constexpr int threads = Group < 256 ? 128 : Group, rows = threads / Group;
-    constexpr size_t shared = ahead ? (size_t)threads * V * sizeof(float4) : 0;
-    static std::atomic<int> known[16];
-    auto kernel = rows_held_kernel<Policy, Entropy, Aligned, ahead, Group, V>;
-    const long long want = (p.M + (long long)rows - 1) / rows;
-    int most = 0;
-    const int rc = resident(kernel, threads, shared, Ranks, known, &most);
-    if (rc != ZNN_OK) return rc;
-    return launch_rows_kernel(kernel, p, (ahead ? std::min<long long>(want, most) : want) * Ranks, threads, Ranks, part, shared);
+    constexpr int rows = 128 / Group;
+    return launch(rows_held_kernel<Policy, Entropy, Aligned, Group, V>, "rows_held_kernel", (p.M + (long long)rows - 1) / rows, 128, 1,
+                  Policy && !p.weights, p, 0);
 }
 
-template <bool Policy, bool Entropy, bool Aligned, int Threads>
-static int launch_walk(const RowParams& p)
+template <bool Policy, bool Entropy, bool Aligned, int Threads, int Quads>
+static int launch_walk(const RowParams& p, int ranks)
 {
-    // a block per row, unless that leaves most of the device idle
-    int ranks = Policy ? 8 : 1;
-    while (ranks < 8 && (long long)p.M * ranks < 4 * sm_count()) ranks *= 2;
+    while (ranks < 8 && (long long)p.M * ranks < 4 * sm_count() && p.N > 4096 * ranks) ranks *= 2;   // few rows: all of the device for them
     const int part = (ceil_div(p.N, ranks) + 3) & ~3;   // parts start where the row's quads do
-    return launch_rows_kernel(rows_walk_kernel<Policy, Entropy, Aligned, Threads>, p, (long long)p.M * ranks, Threads, ranks, part, 0);
+    return launch(rows_walk_kernel<Policy, Entropy, Aligned, Threads, Quads>, "rows_walk_kernel", (long long)p.M * ranks, Threads, ranks,
+                  Policy && !p.weights, p, part);
 }
 
 template <bool Policy, bool Entropy, bool Aligned>
 static int launch_rows_as(const RowParams& p)
 {
-    // 8 lanes per row while a row fits them; then a warp; then a block; then a cluster of blocks; then two walks
-    if (p.N <= room(8, 2, Aligned)) return launch_held<Policy, Entropy, Aligned, 8, 2, 1>(p, p.N);
-    if (p.N <= room(8, 8, Aligned)) return launch_held<Policy, Entropy, Aligned, 8, 8, 1>(p, p.N);
-    if (p.N <= room(32, 8, Aligned)) return launch_held<Policy, Entropy, Aligned, 32, 8, 1>(p, p.N);
-    if constexpr (Policy) {   // (without a gradient as with one, so that the loss has the same bits)
-        auto part = [&](int ranks) { return (ceil_div(p.N, ranks) + 3) & ~3; };   // parts start where the row's quads do
-        if (p.N <= room(256, 4, Aligned)) return launch_held<Policy, Entropy, Aligned, 256, 4, 1>(p, p.N);
-        if (p.N <= room(256, 8, Aligned)) return launch_held<Policy, Entropy, Aligned, 256, 8, 1>(p, p.N);
-        if (part(1) <= room(512, 8, Aligned)) return launch_held<Policy, Entropy, Aligned, 512, 8, 1>(p, part(1));
-        if (part(2) <= room(512, 8, Aligned)) return launch_held<Policy, Entropy, Aligned, 512, 8, 2>(p, part(2));
-        if (part(4) <= room(512, 8, Aligned)) return launch_held<Policy, Entropy, Aligned, 512, 8, 4>(p, part(4));
-        if (part(8) <= room(512, 8, Aligned)) return launch_held<Policy, Entropy, Aligned, 512, 8, 8>(p, part(8));
+    if (p.N <= room(8, 2, Aligned)) return launch_held<Policy, Entropy, Aligned, 8, 2>(p);
+    if (p.N <= room(8, 8, Aligned)) return launch_held<Policy, Entropy, Aligned, 8, 8>(p);
+    if (p.N <= room(32, 8, Aligned)) return launch_held<Policy, Entropy, Aligned, 32, 8>(p);
+    if constexpr (!Policy) {
+        if (p.N <= 2048) return launch_walk<Policy, Entropy, Aligned, 64, 4>(p, 1);
+        if (p.N <= 4096) return launch_walk<Policy, Entropy, Aligned, 128, 4>(p, 1);
+        return launch_walk<Policy, Entropy, Aligned, 256, 4>(p, 1);
+    } else {
+        if (p.N <= 2048) return launch_walk<Policy, Entropy, Aligned, 64, 8>(p, 1);
+        if (p.N <= 8192) return launch_walk<Policy, Entropy, Aligned, 128, 8>(p, 1);
+        if (p.N <= 16384) return launch_walk<Policy, Entropy, Aligned, 256, 8>(p, 1);
+        return launch_walk<Policy, Entropy, Aligned, 512, 8>(p, p.N <= 32768 ? 1 : p.N <= 65536 ? 2 : p.N <= 131072 ? 4 : 8);
     }
-    if (!Policy && p.N <= 2048) return launch_walk<Policy, Entropy, Aligned, 64>(p);
-    if (!Policy && p.N <= 4096) return launch_walk<Policy, Entropy, Aligned, 128>(p);
-    return launch_walk<Policy, Entropy, Aligned, 256>(p);
 }
 
 // every row of the matrix starts with a 16-byte quad and has whole quads only
@@ -1005,15 +870,14 @@ int znn_policy_loss(const float* logits, long long ld, const int32_t* targets, f
     p.old_logp = old_logp; p.ref_logp = ref_logp; p.advantages = advantages; p.weights = weights;
     p.clip_low = clip_low; p.clip_high = clip_high; p.kl_coef = kl_coef; p.entropy_coef = entropy_coef;
     p.count = loss + 1; p.token_loss = token_loss; p.dlogits = dlogits; p.ld_d = ld_d;
+    const int total_ranks = M > 4096 ? 8 : 1;
     if (!weights) {   // the rows' weight 1 / count is needed before their gradients are written
-        policy_total_kernel<<<1, 1024, 0, stream()>>>(targets, weights, token_loss, loss, M, 0);
-        ZNN_LAUNCH_OK("policy_total_kernel");
+        const int counted = launch(policy_total_kernel, "policy_total_kernel", total_ranks, 1024, total_ranks, false, targets, weights, token_loss, loss, M, 0);
+        if (counted != ZNN_OK) return counted;
     }
     const int done = launch_rows<true>(p, entropy || entropy_coef != 0.0f);
     if (done != ZNN_OK) return done;
-    policy_total_kernel<<<1, 1024, 0, stream()>>>(targets, weights, token_loss, loss, M, 1);
-    ZNN_LAUNCH_OK("policy_total_kernel");
-    return ZNN_OK;
+    return launch(policy_total_kernel, "policy_total_kernel", total_ranks, 1024, total_ranks, true, targets, weights, token_loss, loss, M, 1);
 }
 
 int znn_preference_loss(const float* logp, const float* ref_logp, const int32_t* targets, const int32_t* seq_offsets, float beta,
