@@ -111,14 +111,6 @@ __device__ __forceinline__ double log_of_sum(float ties, float s)
     return (double)((bits >> 23) - 127) * 0.693147180559945309417 + (double)logf(__int_as_float((bits & 0x007fffff) | 0x3f800000)) + (total - total);
 }
 
-// exp(x), exp(x) - 1 of a difference of log-probabilities: fp32 has the accuracy that the difference leaves, fp64 the range
-__device__ __forceinline__ double exp_of(double x)
-{
-    const float z = (float)x, e = expf(z > 80.0f ? 0.5f * z : z);
-    return z > 80.0f ? (double)e * (double)e : (double)e;
-}
-__device__ __forceinline__ double expm1_of(double x) { return x > 80.0 ? exp_of(x) : (double)expm1f((float)x); }
-
 // A kernel that was launched with `overlap` may begin while the one before it still runs: it waits here before it reads what that
 // one writes.  That one lets it begin as soon as all of its own blocks run.
 __device__ __forceinline__ void wait_for_previous_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
@@ -174,60 +166,60 @@ __device__ __forceinline__ RowHead row_head(const RowParams& p, unsigned row, bo
 
 // The scalars of one row from its sums (one thread): writes logp, entropy, stats, token_loss (where `write`), returns the
 // gradient's coefficients for a walk over logits measured from `from`.  The log-probability, and the differences that ratio and
-// KL term are made of, are fp64: fp32 would leave a ratio of two probabilities of e^-10 an error of 1e-6.
-template <bool Policy>
+// KL term are made of, are fp64: fp32 would leave a ratio of two probabilities of e^-10 an error of 1e-6.  What follows from
+// them are products, which fp32 keeps.  (In short rows these few hundred operations of one lane are most of the work.)
+template <bool Policy, bool Entropy>
 __device__ __forceinline__ RowGrad row_scalars(const RowParams& p, int row, const RowSums& r, const RowHead& in, float x_t,
                                                bool write, float from)
 {
-    const float total = r.ties + r.s;
+    const float total = r.ties + r.s, inv_total = 1.0f / total;
     const bool empty = total == 0.0f;
     const double log_s = log_of_sum(r.ties, r.s);
     const double logp = empty ? -CUDART_INF : (double)p.it * ((double)x_t - (double)base_of(r.mx)) - log_s;
-    const double H = empty ? 0.0 : log_s - (double)(kLn2 * r.u / total);
+    const float U = Entropy ? kLn2 * r.u * inv_total : 0.0f;   // sum of p_j (log p_j + log s)
+    const float H = !Entropy || empty ? 0.0f : (float)(log_s - (double)U);
     if (write) {
         if (p.logp) p.logp[row] = (float)logp;
-        if (p.entropy) p.entropy[row] = (float)H;
+        if (Entropy && p.entropy) p.entropy[row] = H;
         if (p.stats) *reinterpret_cast<float2*>(p.stats + 2 * (size_t)row) = make_float2(r.mx, total);
     }
     RowGrad g{0.0f, 0.0f, 0.0f, from};
     if (Policy) {
-        float w = in.w;
-        if (!p.weights) {
-            wait_for_previous_kernel();   // which counts the rows while this one reads the logits
-            w = 1.0f / *p.count;
-        }
-        const double A = in.advantage;
-        double loss = 0.0, slope = 0.0;
-        if (A != 0.0) {
-            const double ratio = exp_of(logp - (double)in.old_logp);
-            const double lo = 1.0 - (double)p.clip_low, hi = 1.0 + (double)p.clip_high;
+        const float A = in.advantage;
+        float loss = 0.0f, slope = 0.0f;
+        if (A != 0.0f) {
+            const float ratio = expf((float)(logp - (double)in.old_logp));
+            const float border = A > 0.0f ? 1.0f + p.clip_high : 1.0f - p.clip_low;
             // a gain counts up to the upper border, a loss down to the lower one
-            const bool outside = A > 0.0 ? ratio > hi : ratio < lo;
-            loss = -A * (outside ? (A > 0.0 ? hi : lo) : ratio);
-            slope = outside ? 0.0 : loss;
+            const bool outside = A > 0.0f ? ratio > border : ratio < border;
+            loss = -A * (outside ? border : ratio);
+            slope = outside ? 0.0f : loss;
         }
         if (p.kl_coef != 0.0f) {
-            const double q = (double)in.ref_logp - logp, e = expm1_of(q);
+            const float q = (float)((double)in.ref_logp - logp), e = expm1f(q);
             // e - q loses what e and q share: for a small q the first terms of its series, q^2/2 + q^3/6 + q^4/24 + q^5/120 (the next
             // is below 1e-8 of the first for |q| < 1/32)
-            const double rest = fabs(q) < 0.03125 ? q * q * (0.5 + q * (1.0 / 6.0 + q * (1.0 / 24.0 + q * (1.0 / 120.0)))) : e - q;
-            loss += (double)p.kl_coef * rest;
-            slope -= (double)p.kl_coef * e;
+            const float rest = fabsf(q) < 0.03125f ? q * q * (0.5f + q * (1.0f / 6.0f + q * (1.0f / 24.0f + q * (1.0f / 120.0f)))) : e - q;
+            loss += p.kl_coef * rest;
+            slope -= p.kl_coef * e;
         }
-        double h = 0.0;
-        if (p.entropy_coef != 0.0f) {
-            loss -= (double)p.entropy_coef * H;
-            h = -(double)p.entropy_coef;
-        }
-        if (write) p.token_loss[row] = (float)loss;
+        if (Entropy) loss -= p.entropy_coef * H;
+        if (write) p.token_loss[row] = loss;
         if (!empty) {
-            const double G = (double)p.it * w * slope, E = (double)p.it * w * h;
-            const float rest = expm1f((float)logp);   // p_t - 1
-            g.at_target = (float)(-G * rest - (rest > -1.0f && E != 0.0 ? E * (1.0 + rest) * (logp + H) : 0.0));
-            // p_j (-G - E (log p_j + H)),  p_j = 2^(t + delta) / s,  log p_j = log(2) (t + delta) - log s
-            const float delta = from == r.mx ? 0.0f : fmaxf((from - r.mx) * p.c, kNothing), inv = exp2_fast(delta) / total;
-            g.a = inv * (float)(-G - E * (H + (double)(kLn2 * delta) - log_s));
-            g.b = inv * (float)(-E) * kLn2;
+            float w = in.w;
+            if (!p.weights) {
+                wait_for_previous_kernel();   // which counts the rows while this one reads the logits
+                w = 1.0f / *p.count;
+            }
+            const float G = p.it * w * slope, E = Entropy ? -p.it * w * p.entropy_coef : 0.0f;
+            // p_t, and 1 - p_t: where the target is the largest, what the others sum to; elsewhere p_t is at most 1/2
+            const float top = base_of(r.mx), e_t = x_t == top ? 1.0f : exp2_fast(fmaxf((x_t - top) * p.c, kNothing));
+            const float others = (x_t == top ? r.ties - 1.0f + r.s : total - e_t) * inv_total;
+            g.at_target = G * others - (Entropy && e_t > 0.0f ? E * e_t * inv_total * ((float)logp + H) : 0.0f);
+            // p_j (-G - E (log p_j + H)),  p_j = 2^(t + delta) / s,  log p_j + H = log(2) (t + delta) - U
+            const float delta = from == r.mx ? 0.0f : fmaxf((from - r.mx) * p.c, kNothing), inv = exp2_fast(delta) * inv_total;
+            g.a = inv * (-G - (Entropy ? E * (kLn2 * delta - U) : 0.0f));
+            g.b = Entropy ? -inv * E * kLn2 : 0.0f;
         }
     }
     return g;
@@ -436,10 +428,11 @@ __global__ void __launch_bounds__(128) rows_held_kernel(const RowParams p, int)
             }
         sums.ties = rintf(with_ones - sums.s);
     }
-    const float from = sums.mx;
-    sums = join_lanes<Group>(sums, p.c, mask);
+    sums.ties = warp_sum<Group>(sums.ties, mask);
+    sums.s = warp_sum<Group>(sums.s, mask);
+    if (Entropy) sums.u = warp_sum<Group>(sums.u, mask);
     RowGrad g{};
-    if (tid == 0) g = row_scalars<Policy>(p, row, sums, in, x_t, true, from);
+    if (tid == 0) g = row_scalars<Policy, Entropy>(p, row, sums, in, x_t, true, sums.mx);
     if (!dx) return;
     g.a = __shfl_sync(mask, g.a, 0, Group);
     g.b = __shfl_sync(mask, g.b, 0, Group);
@@ -528,7 +521,7 @@ __global__ void __launch_bounds__(Threads) rows_walk_kernel(const RowParams p, i
             exchange(&sh_word, sums, ranks, rank, p.status);
             sums = join_lanes(tid < ranks ? sh_word.sums[tid] : none, p.c);
         }
-        if (tid == 0) sh_grad = row_scalars<Policy>(p, row, sums, in, x_t, rank == 0, sums.mx);
+        if (tid == 0) sh_grad = row_scalars<Policy, Entropy>(p, row, sums, in, x_t, rank == 0, sums.mx);
     }
     if (!dx) return;
     __syncthreads();
