@@ -350,6 +350,9 @@ __device__ __forceinline__ int cluster_rank()
     return (int)r;
 }
 
+// (the barrier's own order is enough for mbarriers that are published by their fence: no memory fence on arrival)
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_store(double* place, int rank, double v)
 {
     asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(mapa_shared(smem_u32(place), (uint32_t)rank)), "d"(v) : "memory");
@@ -464,7 +467,8 @@ __global__ void __launch_bounds__(Threads) rows_walk_kernel(const RowParams p, i
             mbar_init(smem_u32(&sh_word.bar), 1);
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         }
-        cluster_sync_all();
+        __syncwarp();
+        cluster_arrive();   // waited for when the first walk is done: by then every block runs and has its barrier
     }
     const int row = blockIdx.x / ranks, first = rank * part, n = max(0, min(part, p.N - first));
     const float* x = p.logits + (size_t)row * p.ld + first;
@@ -511,6 +515,7 @@ __global__ void __launch_bounds__(Threads) rows_walk_kernel(const RowParams p, i
         if (r.begin + kStep >= n) break;
         r.begin += kStep;
     }
+    if (ranks > 1) cluster_wait();
     sums = join_lanes(sums, p.c);
     if ((tid & 31) == 0) sh_warps[tid >> 5] = sums;
     __syncthreads();
@@ -597,14 +602,16 @@ policy_total_kernel(const int32_t* __restrict__ targets, const float* __restrict
     if (ranks > 1) cluster_sync_all();   // a block must run before another writes to its memory
     if (with_sum) wait_for_previous_kernel();
     else let_next_kernel_begin();
-    double count = 0.0, sum = 0.0;
-    for (int i = rank * 1024 + threadIdx.x; i < M; i += ranks * 1024) {
-        const float w = weights ? weights[i] : 1.0f;
-        if (targets[i] < 0 || w == 0.0f) continue;
-        count += 1.0;
-        if (with_sum) sum += (double)w * (double)token_loss[i];
+    int rows = 0;
+    double sum = 0.0;
+#pragma unroll 8
+    for (int i = rank * 1024 + threadIdx.x; i < M; i += ranks * 1024) {   // no branch between the loads: all of a step's are under way at once
+        const float w = weights ? weights[i] : 1.0f, l = with_sum ? token_loss[i] : 0.0f;
+        const bool used = targets[i] >= 0 && w != 0.0f;
+        rows += used ? 1 : 0;
+        sum += used ? (double)w * (double)l : 0.0;
     }
-    count = block_sum(count, sh);
+    double count = block_sum((double)rows, sh);
     if (with_sum) sum = block_sum(sum, sh);
     if (ranks > 1) {
         if (threadIdx.x == 0) {
