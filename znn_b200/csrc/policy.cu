@@ -240,98 +240,103 @@ __device__ __forceinline__ void row_unused(const RowParams& p, int row, bool bad
     if (bad && p.status) atomicOr(p.status, ZNN_DEV_BAD_INDEX);
 }
 
-// ---- a row held in registers ----------------------------------------------------------------------------------------
-// Group threads hold V quads of four columns each of a row's part: thread k has the 16-byte quads k, k + Group, ... of memory
-// from the one that the part starts in, so rows may start at any float.  Aligned: every row starts with a quad and has whole
-// quads only; no code for the others then stands between the memory instructions.
+// ---- a row's columns among the threads ------------------------------------------------------------------------------
+// Group threads take V 16-byte quads each of a row's part in a step: thread k the quads k, k + Group, ... of the step.  A part
+// may start and end at any float: up to three columns lie before its first quad and after its last, one each for a few threads
+// (`extra`), so that nothing stands between the quads' memory instructions.  Aligned: there are none of those.
 template <int Group, int V, bool Aligned>
 struct RowPart {
     float v[V][4];
-    int begin;   // column that the first thread's first quad begins at: that is on a multiple of 16 bytes, so it may be negative
-    int n;       // columns of the part
-
-    __device__ __forceinline__ int column(int tid, int k) const { return begin + 4 * (tid + k * Group); }
-    __device__ __forceinline__ bool whole(int j) const { return Aligned ? j < n : j >= 0 && j + 4 <= n; }
+    float extra;
+    int n, head, quads;   // columns of the part, those before the first quad, quads
+    int step;             // first quad of the step
 
     __device__ __forceinline__ void place(const float* x, int columns)
     {
         n = columns;
-        begin = Aligned ? 0 : -((int)((uintptr_t)x >> 2) & 3);
+        head = Aligned ? 0 : min(n, (int)(0u - (unsigned)((uintptr_t)x >> 2)) & 3);
+        quads = (n - head) >> 2;
+        step = 0;
+    }
+    __device__ __forceinline__ bool has(int tid, int k) const { return step + tid + k * Group < quads; }
+    __device__ __forceinline__ int column(int tid, int k) const { return head + 4 * (step + tid + k * Group); }
+    // the thread's extra column: the first threads have those before the quads, from the fifth on those after them
+    __device__ __forceinline__ int extra_column(int tid) const
+    {
+        if (Aligned || step > 0) return -1;
+        const int after = head + 4 * quads + tid - 4;
+        return tid < head ? tid : tid >= 4 && after < n ? after : -1;
     }
 
     __device__ __forceinline__ void load(const float* x, int tid)
     {
 #pragma unroll
         for (int k = 0; k < V; k++) {
-            const int j = column(tid, k);
-            if (whole(j)) {
-                const float4 q = __ldg(reinterpret_cast<const float4*>(x + j));
-                v[k][0] = q.x; v[k][1] = q.y; v[k][2] = q.z; v[k][3] = q.w;
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; i++) v[k][i] = (!Aligned && j + i >= 0 && j + i < n) ? __ldg(x + j + i) : -CUDART_INF_F;
-            }
+            float4 q = make_float4(-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F);
+            if (has(tid, k)) q = *reinterpret_cast<const float4*>(x + column(tid, k));
+            v[k][0] = q.x; v[k][1] = q.y; v[k][2] = q.z; v[k][3] = q.w;
         }
+        const int c = extra_column(tid);
+        extra = c >= 0 ? x[c] : -CUDART_INF_F;
     }
 
-    // whether the columns of a quad lie in one 16-byte quad of the row y as well
-    __device__ __forceinline__ bool same_quads(const float* y) const { return Aligned || (((uintptr_t)(y + begin) >> 2) & 3) == 0; }
+    // whether the part's quads are quads of the row y as well
+    __device__ __forceinline__ bool same_quads(const float* y) const { return Aligned || ((uintptr_t)(y + head) & 15) == 0; }
 
-    // the same columns of another row, whatever its alignment, to hold beside this part's
-    __device__ __forceinline__ void load_beside(const float* y, int tid, float (&o)[V][4]) const
+    // adds the same columns of a row of any alignment to what v holds
+    __device__ __forceinline__ void load_beside(const float* y, int tid, float (&o)[V][4], float& o_extra) const
     {
-        const bool quads = same_quads(y);
+        const bool quad = same_quads(y);
 #pragma unroll
         for (int k = 0; k < V; k++) {
-            const int j = column(tid, k);
-            if (quads && whole(j)) {
-                const float4 q = __ldg(reinterpret_cast<const float4*>(y + j));
-                o[k][0] = q.x; o[k][1] = q.y; o[k][2] = q.z; o[k][3] = q.w;
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; i++) o[k][i] = (!Aligned && j + i >= 0 && j + i < n) ? __ldg(y + j + i) : 0.0f;
+            float4 q = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (has(tid, k)) {
+                const float* from = y + column(tid, k);
+                if (quad) q = __ldcs(reinterpret_cast<const float4*>(from));
+                else q = make_float4(__ldcs(from), __ldcs(from + 1), __ldcs(from + 2), __ldcs(from + 3));
             }
+            o[k][0] = q.x; o[k][1] = q.y; o[k][2] = q.z; o[k][3] = q.w;
         }
+        const int c = extra_column(tid);
+        o_extra = c >= 0 ? y[c] : 0.0f;
     }
 
-    // the quad, in the order of the threads, that holds column c, and whether it is one of this thread's
-    __device__ __forceinline__ int quad_of(int c) const { return (c - begin) >> 2; }
+    // whether this thread is the one that holds (and stores) column c in this step
     __device__ __forceinline__ bool owns(int c, int tid) const
     {
-        const int q = quad_of(c);
-        return c >= 0 && c < n && q >= 0 && q < Group * V && q % Group == tid;
+        if (c < 0 || c >= n) return false;
+        if (!Aligned && (c < head || c >= head + 4 * quads)) return extra_column(tid) == c;
+        const int q = ((c - head) >> 2) - step;
+        return q >= 0 && q < Group * V && q % Group == tid;
     }
 
     // writes what the caller has put into v to a row of any alignment
     __device__ __forceinline__ void store(float* y, int tid) const
     {
-        const bool quads = same_quads(y);
+        const bool quad = same_quads(y);
 #pragma unroll
         for (int k = 0; k < V; k++) {
-            const int j = column(tid, k);
-            if (quads && whole(j)) {
-                __stcs(reinterpret_cast<float4*>(y + j), make_float4(v[k][0], v[k][1], v[k][2], v[k][3]));
-            } else if (!Aligned) {
+            if (!has(tid, k)) continue;
+            float* to = y + column(tid, k);
+            if (quad) {
+                __stcs(reinterpret_cast<float4*>(to), make_float4(v[k][0], v[k][1], v[k][2], v[k][3]));
+            } else {
 #pragma unroll
-                for (int i = 0; i < 4; i++)
-                    if (j + i >= 0 && j + i < n) __stcs(y + j + i, v[k][i]);
+                for (int i = 0; i < 4; i++) __stcs(to + i, v[k][i]);
             }
         }
+        const int c = extra_column(tid);
+        if (c >= 0) __stcs(y + c, extra);
     }
 
-    __device__ __forceinline__ void clear(float* y, int tid) const
+    // zeros for the whole part
+    __device__ __forceinline__ static void clear(float* y, int columns, int tid)
     {
-        const bool quads = same_quads(y);
-#pragma unroll 1
-        for (int k = 0; k < V; k++) {
-            const int j = column(tid, k);
-            if (quads && whole(j)) {
-                __stcs(reinterpret_cast<float4*>(y + j), make_float4(0.0f, 0.0f, 0.0f, 0.0f));
-            } else if (!Aligned) {
-#pragma unroll 1
-                for (int i = 0; i < 4; i++)
-                    if (j + i >= 0 && j + i < n) __stcs(y + j + i, 0.0f);
-            }
+        const int before = Aligned ? 0 : min(columns, (int)(0u - (unsigned)((uintptr_t)y >> 2)) & 3), whole = (columns - before) >> 2;
+        for (int q = tid; q < whole; q += Group) __stcs(reinterpret_cast<float4*>(y + before) + q, make_float4(0.0f, 0.0f, 0.0f, 0.0f));
+        if (!Aligned) {
+            if (tid < before) y[tid] = 0.0f;
+            if (before + 4 * whole + tid < columns) y[before + 4 * whole + tid] = 0.0f;
         }
     }
 };
@@ -399,36 +404,40 @@ __global__ void __launch_bounds__(128) rows_held_kernel(const RowParams p, int)
     const RowHead in = row_head<Policy>(p, row, tid == 0);
     if (!in.used(p.N)) {
         if (tid == 0) row_unused<Policy>(p, row, in.t >= p.N && in.w != 0.0f);
-        if (dx) r.clear(dx, tid);
+        if (dx) r.clear(dx, p.N, tid);
         return;
     }
     r.load(x, tid);
     const float x_t = tid == 0 ? x[in.t] : 0.0f;   // before a gradient is written over it
-    float top = -CUDART_INF_F;
+    float top = r.extra;
 #pragma unroll
     for (int k = 0; k < V; k++) top = fmaxf(fmaxf(top, fmaxf(r.v[k][0], r.v[k][1])), fmaxf(r.v[k][2], r.v[k][3]));
     RowSums sums{warp_max<Group>(top, mask), 0.0f, 0.0f, 0.0f};
     const float base = base_of(sums.mx);
+    // with an entropy term t is clamped (0 * -inf is to be 0), and kept for the gradient, which takes 2^t again
+    auto take = [&](float& x) {
+        const float t2 = (x - base) * p.c, te = Entropy ? max_nan(t2, kNothing) : t2, e = exp2_fast(te);
+        sums.s += e;
+        if (Entropy) sums.u += te * e;
+        x = Entropy ? te : e;
+    };
 #pragma unroll
     for (int k = 0; k < V; k++)
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            // with an entropy term t is clamped (0 * -inf is to be 0), and kept for the gradient, which takes 2^t again
-            const float t2 = (r.v[k][i] - base) * p.c, te = Entropy ? max_nan(t2, kNothing) : t2, e = exp2_fast(te);
-            sums.s += e;
-            if (Entropy) sums.u += te * e;
-            r.v[k][i] = Entropy ? te : e;
-        }
+        for (int i = 0; i < 4; i++) take(r.v[k][i]);
+    if (!Aligned) take(r.extra);
     if (top == base) {   // the few threads that hold the largest logit tell its ones from the rest
         const float with_ones = sums.s;
         sums.s = 0.0f;
+        auto add = [&](float x) {
+            const float e = Entropy ? exp2_again(x) : x;
+            if (!(e == 1.0f)) sums.s += e;
+        };
 #pragma unroll
         for (int k = 0; k < V; k++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float e = Entropy ? exp2_again(r.v[k][i]) : r.v[k][i];
-                if (!(e == 1.0f)) sums.s += e;
-            }
+            for (int i = 0; i < 4; i++) add(r.v[k][i]);
+        if (!Aligned) add(r.extra);
         sums.ties = rintf(with_ones - sums.s);
     }
     sums.ties = warp_sum<Group>(sums.ties, mask);
@@ -440,13 +449,12 @@ __global__ void __launch_bounds__(128) rows_held_kernel(const RowParams p, int)
     g.a = __shfl_sync(mask, g.a, 0, Group);
     g.b = __shfl_sync(mask, g.b, 0, Group);
     g.at_target = __shfl_sync(mask, g.at_target, 0, Group);
+    auto slope = [&](float& x) { x = Entropy ? exp2_again(x) * (g.a + g.b * x) : x * g.a; };
 #pragma unroll
     for (int k = 0; k < V; k++)
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            if (Entropy) r.v[k][i] = exp2_again(r.v[k][i]) * (g.a + g.b * r.v[k][i]);
-            else r.v[k][i] *= g.a;
-        }
+        for (int i = 0; i < 4; i++) slope(r.v[k][i]);
+    if (!Aligned) slope(r.extra);
     r.store(dx, tid);
     if (r.owns(in.t, tid)) dx[in.t] = g.at_target;
 }
@@ -477,8 +485,7 @@ __global__ void __launch_bounds__(Threads) rows_walk_kernel(const RowParams p, i
     const int at = in.t - first;
     if (!in.used(p.N)) {
         if (tid == 0 && rank == 0) row_unused<Policy>(p, row, in.t >= p.N && in.w != 0.0f);
-        if (dx)
-            for (int j = tid; j < n; j += Threads) __stcs(dx + j, 0.0f);
+        if (dx) Part::clear(dx, n, tid);
         return;
     }
     // before any gradient is written: dlogits may be the logits' own buffer
@@ -486,12 +493,12 @@ __global__ void __launch_bounds__(Threads) rows_walk_kernel(const RowParams p, i
 
     RowSums sums{-CUDART_INF_F, 0.0f, 0.0f, 0.0f};
     Part r;
-    constexpr int kStep = 4 * Threads * kQuads;
+    constexpr int kStep = Threads * kQuads;
     r.place(x, n);
 #pragma unroll 1
     for (;;) {
         r.load(x, tid);
-        float mx = sums.mx;
+        float mx = fmaxf(sums.mx, r.extra);
 #pragma unroll
         for (int k = 0; k < kQuads; k++)
             mx = fmaxf(fmaxf(mx, fmaxf(r.v[k][0], r.v[k][1])), fmaxf(r.v[k][2], r.v[k][3]));
@@ -503,17 +510,19 @@ __global__ void __launch_bounds__(Threads) rows_walk_kernel(const RowParams p, i
             sums.mx = mx;
         }
         const float base = base_of(mx);
+        auto take = [&](float x) {
+            const float t2 = (x - base) * p.c, te = Entropy ? max_nan(t2, kNothing) : t2, e = exp2_fast(te);
+            if (e == 1.0f) sums.ties += 1.0f;
+            else sums.s += e;
+            if (Entropy) sums.u += te * e;
+        };
 #pragma unroll
         for (int k = 0; k < kQuads; k++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float t2 = (r.v[k][i] - base) * p.c, te = Entropy ? max_nan(t2, kNothing) : t2, e = exp2_fast(te);
-                if (e == 1.0f) sums.ties += 1.0f;
-                else sums.s += e;
-                if (Entropy) sums.u += te * e;
-            }
-        if (r.begin + kStep >= n) break;
-        r.begin += kStep;
+            for (int i = 0; i < 4; i++) take(r.v[k][i]);
+        if (!Aligned) take(r.extra);
+        if (r.step + kStep >= r.quads) break;
+        r.step += kStep;
     }
     if (ranks > 1) cluster_wait();
     sums = join_lanes(sums, p.c);
@@ -535,17 +544,19 @@ __global__ void __launch_bounds__(Threads) rows_walk_kernel(const RowParams p, i
     // back from the end: the last step's logits are still here, the ones before it in the nearest caches
 #pragma unroll 1
     for (;;) {
+        auto slope = [&](float& x) {
+            const float te = max_nan((x - base) * p.c, kNothing);
+            x = exp2_fast(te) * (g.a + g.b * te);
+        };
 #pragma unroll
         for (int k = 0; k < kQuads; k++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float te = max_nan((r.v[k][i] - base) * p.c, kNothing);
-                r.v[k][i] = exp2_fast(te) * (g.a + g.b * te);
-            }
+            for (int i = 0; i < 4; i++) slope(r.v[k][i]);
+        if (!Aligned) slope(r.extra);
         r.store(dx, tid);
         if (r.owns(at, tid)) dx[at] = g.at_target;
-        r.begin -= kStep;
-        if (r.begin <= -kStep) break;
+        if (r.step == 0) break;
+        r.step -= kStep;
         r.load(x, tid);
     }
 }
@@ -567,26 +578,27 @@ logprob_bwd_kernel(const float* logits, long long ld, const int32_t* __restrict_
     const int t = targets[row];
     const float s = stats[2 * (size_t)row + 1];
     if (t < 0 || t >= N || s == 0.0f) {
-        if (!Accumulate)
-            for (int j = tid; j < n; j += Group) __stcs(dx + j, 0.0f);
+        if (!Accumulate) RowPart<Group, V, Aligned>::clear(dx, n, tid);
         return;
     }
     RowPart<Group, V, Aligned> r;
-    float old[V][4];
+    float old[V][4], old_extra = 0.0f;
     r.place(x, n);
     r.load(x, tid);
-    if (Accumulate) r.load_beside(dx, tid, old);
+    if (Accumulate) r.load_beside(dx, tid, old, old_extra);
     // p_j (-G - E (log p_j + H)) with p_j = 2^t / s, log p_j = log(2) t - log s
     const float G = it * (dlogp ? dlogp[row] : 0.0f), E = it * (dentropy ? dentropy[row] : 0.0f);
     const float base = base_of(stats[2 * (size_t)row]), c = it * kLog2e, inv = 1.0f / s;
     const float a = inv * (-G - (E != 0.0f ? E * (entropy[row] - logf(s)) : 0.0f)), b = -inv * E * kLn2;
+    auto slope = [&](float& x, float before) {
+        const float te = max_nan((x - base) * c, kNothing), o = exp2_fast(te) * (a + b * te);
+        x = Accumulate ? before + o : o;
+    };
 #pragma unroll
     for (int k = 0; k < V; k++)
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const float te = max_nan((r.v[k][i] - base) * c, kNothing), o = exp2_fast(te) * (a + b * te);
-            r.v[k][i] = Accumulate ? old[k][i] + o : o;
-        }
+        for (int i = 0; i < 4; i++) slope(r.v[k][i], Accumulate ? old[k][i] : 0.0f);
+    if (!Aligned) slope(r.extra, old_extra);
     r.store(dx, tid);
     if (r.owns(t - first, tid)) dx[t - first] += G;
 }
@@ -700,9 +712,6 @@ using namespace znn;
     } while (0)
 
 // ---- launches
-// Columns that a group can take whatever their alignment: up to three floats lie before the first column of a part.
-static constexpr int room(int group, int v, bool aligned) { return 4 * group * v - (aligned ? 0 : 3); }
-
 // A launch in clusters of `ranks` blocks; overlap: it may begin while the kernel before it still runs.
 template <class... Params, class... Args>
 static int launch(void (*kernel)(Params...), const char* name, long long blocks, int threads, int ranks, bool overlap, Args... args)
@@ -746,9 +755,9 @@ static int launch_walk(const RowParams& p, int ranks)
 template <bool Policy, bool Entropy, bool Aligned>
 static int launch_rows_as(const RowParams& p)
 {
-    if (p.N <= room(8, 2, Aligned)) return launch_held<Policy, Entropy, Aligned, 8, 2>(p);
-    if (p.N <= room(8, 8, Aligned)) return launch_held<Policy, Entropy, Aligned, 8, 8>(p);
-    if (p.N <= room(32, 8, Aligned)) return launch_held<Policy, Entropy, Aligned, 32, 8>(p);
+    if (p.N <= 64) return launch_held<Policy, Entropy, Aligned, 8, 2>(p);
+    if (p.N <= 256) return launch_held<Policy, Entropy, Aligned, 8, 8>(p);
+    if (p.N <= 1024) return launch_held<Policy, Entropy, Aligned, 32, 8>(p);
     if constexpr (!Policy) {
         if (p.N <= 2048) return launch_walk<Policy, Entropy, Aligned, 64, 4>(p, 1);
         if (p.N <= 4096) return launch_walk<Policy, Entropy, Aligned, 128, 4>(p, 1);
@@ -787,7 +796,8 @@ template <bool Accumulate, bool Aligned, int Group, int V>
 static int launch_bwd(const BwdArgs& b)
 {
     constexpr int rows = Group < 256 ? 128 / Group : 1;
-    const int fit = room(Group, V, Aligned) & ~3, part = (ceil_div(b.N, ceil_div(b.N, fit)) + 3) & ~3, parts = ceil_div(b.N, part);
+    constexpr int fit = 4 * Group * V;
+    const int part = (ceil_div(b.N, ceil_div(b.N, fit)) + 3) & ~3, parts = ceil_div(b.N, part);
     const long long units = (long long)b.M * parts;
     logprob_bwd_kernel<Accumulate, Aligned, Group, V><<<(unsigned)((units + rows - 1) / rows), Group < 256 ? 128 : Group, 0, stream()>>>(
         b.logits, b.ld, b.targets, b.it, b.stats, b.entropy, b.dlogp, b.dentropy, b.dlogits, b.ld_d, b.M, b.N, parts, part);
@@ -798,11 +808,11 @@ static int launch_bwd(const BwdArgs& b)
 template <bool Accumulate, bool Aligned>
 static int launch_bwd_as(const BwdArgs& b)
 {
-    if (b.N <= (room(8, 2, Aligned) & ~3)) return launch_bwd<Accumulate, Aligned, 8, 2>(b);
-    if (b.N <= (room(8, 4, Aligned) & ~3)) return launch_bwd<Accumulate, Aligned, 8, 4>(b);
-    if (b.N <= (room(32, 4, Aligned) & ~3)) return launch_bwd<Accumulate, Aligned, 32, 4>(b);
-    if (b.N <= (room(32, 8, Aligned) & ~3)) return launch_bwd<Accumulate, Aligned, 32, 8>(b);
-    if (b.N <= (room(256, 2, Aligned) & ~3)) return launch_bwd<Accumulate, Aligned, 256, 2>(b);
+    if (b.N <= 64) return launch_bwd<Accumulate, Aligned, 8, 2>(b);
+    if (b.N <= 128) return launch_bwd<Accumulate, Aligned, 8, 4>(b);
+    if (b.N <= 512) return launch_bwd<Accumulate, Aligned, 32, 4>(b);
+    if (b.N <= 1024) return launch_bwd<Accumulate, Aligned, 32, 8>(b);
+    if (b.N <= 2048) return launch_bwd<Accumulate, Aligned, 256, 2>(b);
     return launch_bwd<Accumulate, Aligned, 256, 4>(b);
 }
 
