@@ -126,7 +126,7 @@ struct RowParams {
     // policy loss only
     const float *old_logp, *ref_logp, *advantages, *weights;
     float clip_low, clip_high, kl_coef, entropy_coef;
-    const float* count;   // 1 / *count is the weight where weights is NULL
+    const float* count;   // 1 / *count is the weight where weights is NULL; NULL: every group counts the (few) rows itself
     float* token_loss;
     float* dlogits;
     long long ld_d;
@@ -169,7 +169,7 @@ __device__ __forceinline__ RowHead row_head(const RowParams& p, unsigned row, bo
 // KL term are made of, are fp64: fp32 would leave a ratio of two probabilities of e^-10 an error of 1e-6.  What follows from
 // them are products, which fp32 keeps.  (In short rows these few hundred operations of one lane are most of the work.)
 template <bool Policy, bool Entropy>
-__device__ __forceinline__ RowGrad row_scalars(const RowParams& p, int row, const RowSums& r, const RowHead& in, float x_t,
+__device__ __forceinline__ RowGrad row_scalars(const RowParams& p, int row, const RowSums& r, const RowHead& in, float x_t, int rows,
                                                bool write, float from)
 {
     const float total = r.ties + r.s, inv_total = 1.0f / total;
@@ -208,8 +208,8 @@ __device__ __forceinline__ RowGrad row_scalars(const RowParams& p, int row, cons
         if (!empty) {
             float w = in.w;
             if (!p.weights) {
-                wait_for_previous_kernel();   // which counts the rows while this one reads the logits
-                w = 1.0f / *p.count;
+                if (p.count) wait_for_previous_kernel();   // which counts the rows while this one reads the logits
+                w = 1.0f / (p.count ? *p.count : (float)rows);
             }
             const float G = p.it * w * slope, E = Entropy ? -p.it * w * p.entropy_coef : 0.0f;
             // p_t, and 1 - p_t: where the target is the largest, what the others sum to; elsewhere p_t is at most 1/2
@@ -223,6 +223,17 @@ __device__ __forceinline__ RowGrad row_scalars(const RowParams& p, int row, cons
         }
     }
     return g;
+}
+
+// rows that are not left out, the share of one of `Lanes` neighbouring lanes: small calls count them on the way, where a kernel of
+// its own would cost more than all the rest
+template <int Lanes>
+__device__ __forceinline__ int count_rows(const RowParams& p, int tid)
+{
+    int rows = 0;
+#pragma unroll 4
+    for (int i = tid; i < p.M; i += Lanes) rows += p.targets[i] >= 0 ? 1 : 0;
+    return rows;
 }
 
 // a row that is left out (bad = false) or whose target is outside the vocabulary (bad = true)
@@ -409,6 +420,7 @@ __global__ void __launch_bounds__(128) rows_held_kernel(const RowParams p, int)
     }
     r.load(x, tid);
     const float x_t = tid == 0 ? x[in.t] : 0.0f;   // before a gradient is written over it
+    const int rows = Policy && !p.weights && !p.count ? __reduce_add_sync(mask, count_rows<Group>(p, tid)) : 0;
     float top = r.extra;
 #pragma unroll
     for (int k = 0; k < V; k++) top = fmaxf(fmaxf(top, fmaxf(r.v[k][0], r.v[k][1])), fmaxf(r.v[k][2], r.v[k][3]));
@@ -444,7 +456,7 @@ __global__ void __launch_bounds__(128) rows_held_kernel(const RowParams p, int)
     sums.s = warp_sum<Group>(sums.s, mask);
     if (Entropy) sums.u = warp_sum<Group>(sums.u, mask);
     RowGrad g{};
-    if (tid == 0) g = row_scalars<Policy, Entropy>(p, row, sums, in, x_t, true, sums.mx);
+    if (tid == 0) g = row_scalars<Policy, Entropy>(p, row, sums, in, x_t, rows, true, sums.mx);
     if (!dx) return;
     g.a = __shfl_sync(mask, g.a, 0, Group);
     g.b = __shfl_sync(mask, g.b, 0, Group);
@@ -467,6 +479,7 @@ __global__ void __launch_bounds__(Threads) rows_walk_kernel(const RowParams p, i
     constexpr int kWarps = Threads / 32;
     using Part = RowPart<Threads, kQuads, Aligned>;
     __shared__ RowSums sh_warps[kWarps];
+    __shared__ int sh_rows[kWarps];
     __shared__ RowGrad sh_grad;
     __shared__ __align__(16) RowWord sh_word;
     const int ranks = cluster_size(), rank = cluster_rank(), tid = threadIdx.x;
@@ -524,6 +537,10 @@ __global__ void __launch_bounds__(Threads) rows_walk_kernel(const RowParams p, i
         if (r.step + kStep >= r.quads) break;
         r.step += kStep;
     }
+    if (Policy && !p.weights && !p.count) {
+        const int rows = __reduce_add_sync(kAllLanes, count_rows<Threads>(p, tid));
+        if ((tid & 31) == 0) sh_rows[tid >> 5] = rows;
+    }
     if (ranks > 1) cluster_wait();
     sums = join_lanes(sums, p.c);
     if ((tid & 31) == 0) sh_warps[tid >> 5] = sums;
@@ -535,7 +552,12 @@ __global__ void __launch_bounds__(Threads) rows_walk_kernel(const RowParams p, i
             exchange(&sh_word, sums, ranks, rank, p.status);
             sums = join_lanes(tid < ranks ? sh_word.sums[tid] : none, p.c);
         }
-        if (tid == 0) sh_grad = row_scalars<Policy, Entropy>(p, row, sums, in, x_t, rank == 0, sums.mx);
+        if (tid == 0) {
+            int rows = 0;
+            if (Policy && !p.weights && !p.count)
+                for (int i = 0; i < kWarps; i++) rows += sh_rows[i];
+            sh_grad = row_scalars<Policy, Entropy>(p, row, sums, in, x_t, rows, rank == 0, sums.mx);
+        }
     }
     if (!dx) return;
     __syncthreads();
@@ -617,7 +639,7 @@ policy_total_kernel(const int32_t* __restrict__ targets, const float* __restrict
     int rows = 0;
     double sum = 0.0;
 #pragma unroll 8
-    for (int i = rank * 1024 + threadIdx.x; i < M; i += ranks * 1024) {   // no branch between the loads: all of a step's are under way at once
+    for (unsigned i = rank * 1024 + threadIdx.x; i < (unsigned)M; i += ranks * 1024) {   // no branch between the loads: all of a step's are under way at once
         const float w = weights ? weights[i] : 1.0f, l = with_sum ? token_loss[i] : 0.0f;
         const bool used = targets[i] >= 0 && w != 0.0f;
         rows += used ? 1 : 0;
@@ -643,60 +665,155 @@ policy_total_kernel(const int32_t* __restrict__ targets, const float* __restrict
     }
 }
 
-// One block per pair: the two sums, the pair's loss, the gradient of its rows.
-__global__ void __launch_bounds__(256)
+// What a pair's margin makes of it: its loss, and the slope of the mean loss by the margin.
+struct PairTerms {
+    double loss, slope;
+};
+
+__device__ __forceinline__ PairTerms pair_terms(double m, double eps, int P)
+{
+    const double e = exp(-fabs(m)), soft = log1p(e), inv = 1.0 / (1.0 + e);   // log(1 + e^-|m|), sigmoid(|m|): no overflow either way
+    PairTerms t;
+    t.loss = (1.0 - eps) * (soft + fmax(-m, 0.0)) + eps * (soft + fmax(m, 0.0));
+    t.slope = (eps - (m >= 0.0 ? e * inv : inv)) / (double)P;   // -(1 - eps) sigmoid(-m) + eps sigmoid(m)
+    return t;
+}
+
+// A block (or a cluster of blocks, for long sequences) per pair: the two sums, the pair's loss, the gradient of its rows.
+// Small: one block has every pair, a warp each, and the mean as well.  The gradient is the same for all rows of a sequence, so the
+// second walk reads nothing but which rows are left out.  Bound by HBM where there is enough: 12 to 16 bytes per row.
+template <bool Small, int Threads>
+__global__ void __launch_bounds__(Threads)
 preference_pair_kernel(const float* __restrict__ logp, const float* __restrict__ ref_logp, const int32_t* __restrict__ targets,
                        const int32_t* __restrict__ offsets, float beta, float smoothing, float margin, int by_length,
-                       float* __restrict__ pair_loss, float* __restrict__ rewards, float* __restrict__ dlogp, int P, int M,
-                       int* __restrict__ status)
+                       float* __restrict__ loss, float* __restrict__ pair_loss, float* __restrict__ rewards, float* __restrict__ dlogp,
+                       int P, int M, int* __restrict__ status)
 {
-    __shared__ double sh[8];
-    const int pair = blockIdx.x;
-    const int o[3] = {offsets[2 * pair], offsets[2 * pair + 1], offsets[2 * pair + 2]};
-    if (o[0] < 0 || o[1] < o[0] || o[2] < o[1] || o[2] > M) {
+    constexpr int kBatch = 8;   // rows per thread whose loads are under way at once
+    __shared__ double sh[Threads / 32][4], sh_all[8][4];
+    __shared__ float sh_slope[2];
+    const int ranks = cluster_size(), rank = cluster_rank(), tid = Small ? threadIdx.x & 31 : threadIdx.x;
+    if (ranks > 1) cluster_sync_all();   // a block must run before another writes to its memory
+    const int pair = Small ? threadIdx.x >> 5 : blockIdx.x / ranks;
+    const unsigned step = Small ? 32 : Threads * ranks, start = Small ? tid : rank * Threads + tid;
+    int o[3];
+    for (int k = 0; k < 3; k++) o[k] = offsets[2 * pair + k];
+    const bool usable = o[0] >= 0 && o[1] >= o[0] && o[2] >= o[1] && o[2] <= M;   // the same in every block of the pair
+    // of the ratios and of the rows, for both sequences: their rows lie one after the other, so one walk makes all four
+    double sums[4] = {0.0, 0.0, 0.0, 0.0};
+    // (an unusable pair's range is empty, whatever its offsets say)
+    const unsigned begin = usable ? o[0] : 0, middle = usable ? o[1] : 0, end = usable ? o[2] : 0;
+    int rows[2] = {0, 0};
+    for (unsigned i0 = begin + start; i0 < end; i0 += kBatch * step) {
+        float a[kBatch], b[kBatch];
+        int t[kBatch];
+#pragma unroll
+        for (int q = 0; q < kBatch; q++) {
+            const unsigned i = i0 + q * step;
+            const bool in = i < end;
+            a[q] = in ? logp[i] : 0.0f;
+            b[q] = in && ref_logp ? ref_logp[i] : 0.0f;
+            t[q] = !in ? -1 : targets ? targets[i] : 0;
+        }
+#pragma unroll
+        for (int q = 0; q < kBatch; q++) {
+            const bool first = i0 + q * step < middle;
+            const double d = t[q] >= 0 ? (double)a[q] - (double)b[q] : 0.0;
+            const int one = t[q] >= 0 ? 1 : 0;
+            if (first) {
+                sums[0] += d;
+                rows[0] += one;
+            } else {
+                sums[1] += d;
+                rows[1] += one;
+            }
+        }
+    }
+    sums[2] = rows[0];
+    sums[3] = rows[1];
+#pragma unroll
+    for (int k = 0; k < 4; k++)
+#pragma unroll
+        for (int l = 16; l > 0; l >>= 1) sums[k] += __shfl_xor_sync(kAllLanes, sums[k], l);
+    if (!Small) {
+        if ((tid & 31) == 0)
+            for (int k = 0; k < 4; k++) sh[tid >> 5][k] = sums[k];
+        __syncthreads();
+        if (tid < 32) {
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                sums[k] = tid < Threads / 32 ? sh[tid][k] : 0.0;
+#pragma unroll
+                for (int l = 16; l > 0; l >>= 1) sums[k] += __shfl_xor_sync(kAllLanes, sums[k], l);
+            }
+        }
+        if (ranks > 1) {
+            if (tid < ranks)
+                for (int k = 0; k < 4; k++) cluster_store(&sh_all[rank][k], tid, sums[k]);
+            cluster_sync_all();
+            if (tid == 0)
+                for (int k = 0; k < 4; k++) {
+                    sums[k] = 0.0;
+                    for (int i = 0; i < ranks; i++) sums[k] += sh_all[i][k];
+                }
+        }
+    }
+    float slopes[2] = {0.0f, 0.0f};
+    if (tid == 0) {
+        double share[2], reward[2];
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            share[k] = !by_length ? (double)beta : sums[2 + k] > 0.0 ? (double)beta / sums[2 + k] : 0.0;
+            reward[k] = usable ? share[k] * sums[k] : CUDART_NAN;
+        }
+        const PairTerms t = pair_terms(reward[0] - reward[1] - (double)margin, (double)smoothing, P);
+        slopes[0] = (float)(t.slope * share[0]);
+        slopes[1] = (float)(-t.slope * share[1]);
+        if (rank == 0) {
+            pair_loss[pair] = (float)t.loss;
+            rewards[2 * pair] = (float)reward[0];
+            rewards[2 * pair + 1] = (float)reward[1];
+            if (!usable && status) atomicOr(status, ZNN_DEV_BAD_INDEX);
+        }
+        if (Small) sh[pair][0] = (double)(float)t.loss;   // the mean is that of the losses as rounded
+        sh_slope[0] = slopes[0];
+        sh_slope[1] = slopes[1];
+    }
+    __syncthreads();
+    if (Small) {
         if (threadIdx.x == 0) {
-            pair_loss[pair] = rewards[2 * pair] = rewards[2 * pair + 1] = CUDART_NAN_F;
-            if (status) atomicOr(status, ZNN_DEV_BAD_INDEX);
+            double sum = 0.0;
+            for (int i = 0; i < P; i++) sum += sh[i][0];
+            *loss = (float)(sum / (double)P);
         }
-        return;
+        slopes[0] = __shfl_sync(kAllLanes, slopes[0], 0);
+        slopes[1] = __shfl_sync(kAllLanes, slopes[1], 0);
+    } else {
+        slopes[0] = sh_slope[0];
+        slopes[1] = sh_slope[1];
     }
-    double reward[2], share[2];
+    if (!usable || !dlogp) return;
+    for (unsigned i0 = begin + start; i0 < end; i0 += kBatch * step) {
+        int t[kBatch];
 #pragma unroll
-    for (int k = 0; k < 2; k++) {
-        double sum = 0.0, n = 0.0;
-        for (int i = o[k] + threadIdx.x; i < o[k + 1]; i += 256) {
-            if (targets && targets[i] < 0) continue;
-            sum += (double)logp[i] - (ref_logp ? (double)ref_logp[i] : 0.0);
-            n += 1.0;
+        for (int q = 0; q < kBatch; q++) {
+            const unsigned i = i0 + q * step;
+            t[q] = targets && i < end ? targets[i] : 0;
         }
-        sum = block_sum(sum, sh);
-        share[k] = beta;
-        if (by_length) {
-            n = block_sum(n, sh);
-            share[k] = n > 0.0 ? (double)beta / n : 0.0;
-        }
-        reward[k] = share[k] * sum;
-    }
-    const double m = reward[0] - reward[1] - (double)margin, eps = smoothing;
-    const double soft = log1p(exp(-fabs(m)));   // log(1 + exp(-|m|)): -log sigmoid(+-m) without overflow
-    if (threadIdx.x == 0) {
-        pair_loss[pair] = (float)((1.0 - eps) * (soft + fmax(-m, 0.0)) + eps * (soft + fmax(m, 0.0)));
-        rewards[2 * pair] = (float)reward[0];
-        rewards[2 * pair + 1] = (float)reward[1];
-    }
-    if (!dlogp) return;
-    const double slope = (eps - 1.0 / (1.0 + exp(m))) / (double)P;   // -(1 - eps) sigmoid(-m) + eps sigmoid(m)
 #pragma unroll
-    for (int k = 0; k < 2; k++) {
-        const float g = (float)((k ? -slope : slope) * share[k]);
-        for (int i = o[k] + threadIdx.x; i < o[k + 1]; i += 256) dlogp[i] = (targets && targets[i] < 0) ? 0.0f : g;
+        for (int q = 0; q < kBatch; q++) {
+            const unsigned i = i0 + q * step;
+            if (i < end) dlogp[i] = t[q] < 0 ? 0.0f : i < middle ? slopes[0] : slopes[1];
+        }
     }
 }
 
 __global__ void __launch_bounds__(1024) mean_kernel(const float* __restrict__ v, float* __restrict__ out, int n)
 {
     __shared__ double sh[32];
+    wait_for_previous_kernel();
     double s = 0.0;
+#pragma unroll 8
     for (int i = threadIdx.x; i < n; i += 1024) s += (double)v[i];
     s = block_sum(s, sh);
     if (threadIdx.x == 0) out[0] = (float)(s / (double)n);
@@ -740,34 +857,42 @@ static int launch_held(const RowParams& p)
 {
     constexpr int rows = 128 / Group;
     return launch(rows_held_kernel<Policy, Entropy, Aligned, Group, V>, "rows_held_kernel", (p.M + (long long)rows - 1) / rows, 128, 1,
-                  Policy && !p.weights, p, 0);
+                  Policy && p.count, p, 0);
 }
 
-template <bool Policy, bool Entropy, bool Aligned, int Threads, int Quads>
+template <bool Policy, bool Entropy, bool Aligned, int Threads>
 static int launch_walk(const RowParams& p, int ranks)
 {
-    while (ranks < 8 && (long long)p.M * ranks < 4 * sm_count() && p.N > 4096 * ranks) ranks *= 2;   // few rows: all of the device for them
     const int part = (ceil_div(p.N, ranks) + 3) & ~3;   // parts start where the row's quads do
-    return launch(rows_walk_kernel<Policy, Entropy, Aligned, Threads, Quads>, "rows_walk_kernel", (long long)p.M * ranks, Threads, ranks,
-                  Policy && !p.weights, p, part);
+    return launch(rows_walk_kernel<Policy, Entropy, Aligned, Threads, 8>, "rows_walk_kernel", (long long)p.M * ranks, Threads, ranks,
+                  Policy && p.count, p, part);
 }
 
+// Which kernel: 8 lanes per row up to 256 columns, a warp up to 1024, then blocks that walk.  A block costs the same few
+// reductions whatever its size, so the smallest one that a few steps suffice wins; the policy loss, which walks twice, wants its
+// rows in flight to stay in L2 between the walks and so spreads long rows over clusters.  Measured (us, 32 / 64 / 128 / 256 threads):
+//   policy   40000 x 2000: 111 / 125 / 183 / 339,  20000 x 4096: 133 / 114 / 120 / 185,  10000 x 8192: - / 135 / 112 / 124,
+//            4000 x 20000: - / - / 140 / 120;  256 threads in clusters of 1 / 2 / 4 / 8: 2500 x 32000: 133 / 117 / 139 / -,
+//            1500 x 65536: 180 / 162 / 143 / 165,  700 x 131072: - / - / 152 / 136
+//   logprob  40000 x 2000: 54 / 66 / 105 / 220,  20000 x 4099: 54 / 55 / 58 / 117,  4000 x 20000: - / 59 / 54 / 59,
+//            500 x 200001 (512 threads: 67): - / - / 74 / 69
+// Few rows are spread over clusters whatever they cost: 32 x 131072 takes 7.4 us with eight blocks per row, 8.7 with four.
 template <bool Policy, bool Entropy, bool Aligned>
 static int launch_rows_as(const RowParams& p)
 {
     if (p.N <= 64) return launch_held<Policy, Entropy, Aligned, 8, 2>(p);
     if (p.N <= 256) return launch_held<Policy, Entropy, Aligned, 8, 8>(p);
     if (p.N <= 1024) return launch_held<Policy, Entropy, Aligned, 32, 8>(p);
-    if constexpr (!Policy) {
-        if (p.N <= 2048) return launch_walk<Policy, Entropy, Aligned, 64, 4>(p, 1);
-        if (p.N <= 4096) return launch_walk<Policy, Entropy, Aligned, 128, 4>(p, 1);
-        return launch_walk<Policy, Entropy, Aligned, 256, 4>(p, 1);
-    } else {
-        if (p.N <= 2048) return launch_walk<Policy, Entropy, Aligned, 64, 8>(p, 1);
-        if (p.N <= 8192) return launch_walk<Policy, Entropy, Aligned, 128, 8>(p, 1);
-        if (p.N <= 16384) return launch_walk<Policy, Entropy, Aligned, 256, 8>(p, 1);
-        return launch_walk<Policy, Entropy, Aligned, 512, 8>(p, p.N <= 32768 ? 1 : p.N <= 65536 ? 2 : p.N <= 131072 ? 4 : 8);
+    if (p.M < 2 * sm_count() && p.N > 2048) {
+        int ranks = Policy && p.N > 102400 ? 8 : 1;
+        while (ranks < 8 && p.N > 4096 * ranks && (long long)p.M * ranks < 2 * sm_count()) ranks *= 2;
+        return launch_walk<Policy, Entropy, Aligned, 256>(p, ranks);
     }
+    if (p.N <= (Policy ? 2048 : 4096)) return launch_walk<Policy, Entropy, Aligned, 32>(p, 1);
+    if (p.N <= (Policy ? 5120 : 8192)) return launch_walk<Policy, Entropy, Aligned, 64>(p, 1);
+    if (p.N <= (Policy ? 12288 : 32768)) return launch_walk<Policy, Entropy, Aligned, 128>(p, 1);
+    if constexpr (Policy) return launch_walk<Policy, Entropy, Aligned, 256>(p, p.N <= 25600 ? 1 : p.N <= 51200 ? 2 : p.N <= 102400 ? 4 : 8);
+    else return launch_walk<Policy, Entropy, Aligned, 512>(p, 1);
 }
 
 // every row of the matrix starts with a 16-byte quad and has whole quads only
@@ -879,9 +1004,10 @@ int znn_policy_loss(const float* logits, long long ld, const int32_t* targets, f
     p.logp = logp; p.entropy = entropy; p.status = device_status_word();
     p.old_logp = old_logp; p.ref_logp = ref_logp; p.advantages = advantages; p.weights = weights;
     p.clip_low = clip_low; p.clip_high = clip_high; p.kl_coef = kl_coef; p.entropy_coef = entropy_coef;
-    p.count = loss + 1; p.token_loss = token_loss; p.dlogits = dlogits; p.ld_d = ld_d;
+    p.token_loss = token_loss; p.dlogits = dlogits; p.ld_d = ld_d;
     const int total_ranks = M > 4096 ? 8 : 1;
-    if (!weights) {   // the rows' weight 1 / count is needed before their gradients are written
+    if (!weights && M > 512) {   // the rows' weight 1 / count is needed before their gradients are written
+        p.count = loss + 1;
         const int counted = launch(policy_total_kernel, "policy_total_kernel", total_ranks, 1024, total_ranks, false, targets, weights, token_loss, loss, M, 0);
         if (counted != ZNN_OK) return counted;
     }
@@ -900,12 +1026,20 @@ int znn_preference_loss(const float* logp, const float* ref_logp, const int32_t*
     ZNN_REQUIRE(isfinite(beta) && isfinite(margin), "beta and margin must be finite");
     ZNN_REQUIRE(label_smoothing >= 0.0f && label_smoothing < 1.0f, "label_smoothing must lie in [0, 1)");
     ZNN_NEED_DEVICE();
-    preference_pair_kernel<<<P, 256, 0, stream()>>>(logp, ref_logp, targets, seq_offsets, beta, label_smoothing, margin,
-                                                    length_normalize, pair_loss, rewards, dlogp, P, M, device_status_word());
-    ZNN_LAUNCH_OK("preference_pair_kernel");
-    mean_kernel<<<1, 1024, 0, stream()>>>(pair_loss, loss, P);
-    ZNN_LAUNCH_OK("mean_kernel");
-    return ZNN_OK;
+#define ZNN_PAIRS(small, threads, blocks, used, ranks)                                                                                    \
+    launch(preference_pair_kernel<small, threads>, "preference_pair_kernel", blocks, used, ranks, false, logp, ref_logp, targets, seq_offsets, \
+           beta, label_smoothing, margin, length_normalize, loss, pair_loss, rewards, dlogp, P, M, device_status_word())
+    // A warp per pair in one launch for small calls.  Few pairs of long sequences: eight blocks each, where one block's own bandwidth
+    // (about 100 GB/s) would be the limit.  Many short ones: small blocks.
+    if (P <= 32 && M <= 8192) return ZNN_PAIRS(true, 1024, 1, 32 * P, 1);
+    const int rows = M / P;
+    const int rc = rows > 8192 && P <= 32              ? ZNN_PAIRS(false, 1024, 8LL * P, 1024, 8)
+                   : rows > 8192 && P < 2 * sm_count() ? ZNN_PAIRS(false, 256, 8LL * P, 256, 8)
+                   : rows > 1024                       ? ZNN_PAIRS(false, 256, P, 256, 1)
+                                                       : ZNN_PAIRS(false, 64, P, 64, 1);
+#undef ZNN_PAIRS
+    if (rc != ZNN_OK) return rc;
+    return launch(mean_kernel, "mean_kernel", 1, 1024, 1, true, (const float*)pair_loss, loss, P);
 }
 
 }  // extern "C"
