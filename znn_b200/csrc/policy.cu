@@ -885,7 +885,7 @@ static int launch_rows_as(const RowParams& p)
     if (p.N <= 1024) return launch_held<Policy, Entropy, Aligned, 32, 8>(p);
     if (p.M < 2 * sm_count() && p.N > 2048) {
         int ranks = Policy && p.N > 102400 ? 8 : 1;
-        while (ranks < 8 && p.N > 4096 * ranks && (long long)p.M * ranks < 2 * sm_count()) ranks *= 2;
+        while (ranks < 8 && p.N > 8192 * ranks && (long long)p.M * ranks < 2 * sm_count()) ranks *= 2;
         return launch_walk<Policy, Entropy, Aligned, 256>(p, ranks);
     }
     if (p.N <= (Policy ? 2048 : 4096)) return launch_walk<Policy, Entropy, Aligned, 32>(p, 1);
