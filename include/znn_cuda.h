@@ -83,6 +83,9 @@ int znn_param_slab_total(znn_param_slab* s, size_t* total_floats);
 int znn_param_slab_tensor(znn_param_slab* s, int i, float** value, float** grad, float** velocity, size_t* offset);
 int znn_param_slab_zero_grad(znn_param_slab* s);
 int znn_param_slab_sgd_step(znn_param_slab* s, float lr, float momentum, float grad_scale);
+/* the same with the gradients clipped to the global norm max_norm: znn_grad_norm of the slab into result, then
+ * znn_sgd_step_clipped (both below) */
+int znn_param_slab_sgd_step_clipped(znn_param_slab* s, float lr, float momentum, float grad_scale, float max_norm, float* result);
 int znn_param_slab_allreduce_grads(znn_param_slab* s);   /* in-place sum over the data-parallel ranks */
 int znn_param_slab_destroy(znn_param_slab* s);
 int znn_last_error(char* buf, size_t buflen);

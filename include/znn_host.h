@@ -9,7 +9,7 @@
  *    ("matmul", "addBias", "relu", "gelu", "softmaxCrossEntropy", "reshape",
  *    "transposeND", "mulScalar", "add", "conv2d", "maxpool2d", "softmax",
  *    "rmsNorm", "batchMatMul", "embedding", plus the additions "causalSoftmax", "layerNorm", "linear", "causalAttention"
- *    (args: B, T, heads, scale)).
+ *    (args: B, T, heads, scale), and the fine-tuning losses "tokenLogProb", "policyLoss", "preferenceLoss").
  *  - znn_model_*: the example programs' models (examples/fashion_mnist.zig,
  *    examples/cnn.zig, examples/transformer_block.zig, examples/transformer_gpt.zig)
  *    with their training step: new graph -> forward -> SoftmaxCrossEntropy ->
@@ -33,7 +33,13 @@ int znn_graph_destroy(znn_graph* g);
 int znn_graph_array(znn_graph* g, const long long* dims, int rank, const float* host_data, int requires_grad, int* id);
 /* args: reshape -> new dims; transposeND -> dim0, dim1; mulScalar -> value; maxpool2d -> pool, stride;
  * rmsNorm/layerNorm -> eps; conv2d -> pad (optional); causalSoftmax -> scale;
- * softmaxCrossEntropy -> the M integer class labels */
+ * softmaxCrossEntropy -> the M integer class labels;
+ * tokenLogProb (input logits; result [M, 1]) -> inv_temp, M targets;
+ * policyLoss (inputs logits, old_logp, advantages[, ref_logp][, weights]; result [1, 2] = loss, rows) -> clip_low, clip_high,
+ *   kl_coef, entropy_coef, inv_temp, 1 if ref_logp is given, 1 if weights is, M targets;
+ * preferenceLoss (inputs logp[, ref_logp]; result [1, 1]) -> beta, label_smoothing, margin, length_normalize, P, 2P + 1 row
+ *   numbers where the sequences start and end, and M targets or none.  Meaning: znn_policy_loss, znn_preference_loss.  Like
+ *   softmaxCrossEntropy the two losses are roots: the gradient that arrives at them from above is not used. */
 int znn_graph_op(znn_graph* g, const char* name, const int* inputs, int n_inputs, const double* args, int n_args, int* id);
 int znn_graph_backward(znn_graph* g, int id, int seed_one);  /* seed_one=1: Graph.backward, 0: backwardWithGrad */
 int znn_graph_forward(znn_graph* g);                         /* Graph.forward: re-execute the tape */
@@ -93,6 +99,8 @@ int znn_model_get_velocities(znn_model* m, float* host_slab);
  * a fused_* option changes, or when one of the shim's scratch blocks has moved since),
  * "optimizer" (0 = SGD with "lr" / "momentum" as the example programs use, 1 = Adam, src/optim.zig:69-152, with "lr",
  * "beta1", "beta2", "eps" and the step count "adam_t"; no CUDA-graph replay with Adam: the step size changes per step),
+ * "max_grad_norm" (above 0: every step's gradients, after the data-parallel sum, are clipped to this global norm, and a step whose
+ * norm is not finite leaves parameters and optimizer state as they are; 0, the default, is off),
  * "targets_u8" (1/0: the targets pointer of znn_model_train_step holds byte labels, the reference's label type,
  * e.g. the y_dest of znn_loader_next_into; default 0 = int32) */
 int znn_model_set_option(znn_model* m, const char* key, double value);
@@ -101,6 +109,25 @@ int znn_model_set_option(znn_model* m, const char* key, double value);
  * loss_host may be NULL (no read-back, no synchronisation). */
 int znn_model_train_step(znn_model* m, const float* x, const int32_t* targets, int batch, int seq, int on_device,
                          float* loss_host);
+/* Fine-tuning of a GPT (additions; the losses are znn_token_logprob_fwd, znn_policy_loss and znn_preference_loss of znn_cuda.h).  ids:
+ * [batch, seq] fp32 token ids; targets: batch * seq int32, the token that follows each position, negative where a position
+ * (prompt, padding) is left out.  on_device = 1: all arrays are device memory and used in place, results of
+ * znn_model_token_logprobs included; loss_host and rewards_host are host memory and may be NULL (no read-back).
+ * znn_model_token_logprobs: log-probabilities (and entropies, may be NULL) of the targets under the model as it is: what a
+ *   policy step calls old_logp or ref_logp, what a preference step calls ref_logp.
+ * znn_model_policy_step, znn_model_preference_step: one training step each, as znn_model_train_step (forward, loss, zeroGrad,
+ *   backward, gradient all-reduce, clipping where max_grad_norm is set, optimizer).  Preference: 2 * pairs sequences of seq ids,
+ *   the preferred and the other one of each pair in turn; rewards_host receives 2 * pairs values.
+ * znn_model_grad_norm: norm and clip factor (may be NULL) of the latest step, while the option max_grad_norm is set. */
+int znn_model_token_logprobs(znn_model* m, const float* ids, const int32_t* targets, int batch, int seq, int on_device, float inv_temp,
+                             float* logp, float* entropy);
+int znn_model_policy_step(znn_model* m, const float* ids, const int32_t* targets, const float* old_logp, const float* ref_logp,
+                          const float* advantages, const float* weights, int batch, int seq, int on_device, float inv_temp,
+                          float clip_low, float clip_high, float kl_coef, float entropy_coef, float* loss_host);
+int znn_model_preference_step(znn_model* m, const float* ids, const int32_t* targets, const float* ref_logp, int pairs, int seq,
+                              int on_device, float beta, float label_smoothing, float margin, int length_normalize, float* loss_host,
+                              float* rewards_host);
+int znn_model_grad_norm(znn_model* m, float* norm, float* factor);
 /* One evaluation batch as the example programs' evaluateModel runs it (examples/cnn.zig:212-256): forward, mean
  * cross-entropy loss, and computeAccuracy (:193-205) = fraction of rows whose argmax equals the byte label.  MLP / CNN
  * models; x and labels are host memory, or device memory used in place when on_device = 1 (e.g. a loader's batch). */

@@ -83,6 +83,7 @@ pub extern fn znn_param_slab_total(s: ?*znn_param_slab, total_floats: ?*usize) c
 pub extern fn znn_param_slab_tensor(s: ?*znn_param_slab, i: c_int, value: *?[*]f32, grad: *?[*]f32, velocity: *?[*]f32, offset: ?*usize) c_int;
 pub extern fn znn_param_slab_zero_grad(s: ?*znn_param_slab) c_int;
 pub extern fn znn_param_slab_sgd_step(s: ?*znn_param_slab, lr: f32, momentum: f32, grad_scale: f32) c_int;
+pub extern fn znn_param_slab_sgd_step_clipped(s: ?*znn_param_slab, lr: f32, momentum: f32, grad_scale: f32, max_norm: f32, result: ?[*]f32) c_int;
 pub extern fn znn_param_slab_allreduce_grads(s: ?*znn_param_slab) c_int;
 pub extern fn znn_param_slab_destroy(s: ?*znn_param_slab) c_int;
 pub extern fn znn_last_error(buf: [*]u8, buflen: usize) c_int;

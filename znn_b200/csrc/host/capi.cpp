@@ -48,6 +48,19 @@ static Shape shape_from(const long long* dims, int rank)
     return Shape(d, (size_t)rank);
 }
 
+// args[from .. n_args) as int32 in the graph's arena; there must be `want` of them
+static const int32_t* upload_ints(znn_graph* zg, const std::string& op, const double* args, int from, int n_args, size_t want)
+{
+    if (n_args < from || (size_t)(n_args - from) != want)
+        throw Error(ZNN_ERR_INVALID, op + ": " + std::to_string(want) + " integers expected, " + std::to_string(n_args - from) + " given");
+    std::vector<int32_t> v(want);
+    for (size_t i = 0; i < want; i++) v[i] = (int32_t)args[from + i];
+    int32_t* dev = (int32_t*)zg->arena->alloc(want * sizeof(int32_t));
+    check(znn_memcpy_h2d(dev, v.data(), want * sizeof(int32_t)), "upload integers");
+    check(znn_sync(), "znn_sync");
+    return dev;
+}
+
 extern "C" {
 
 int znn_graph_create(size_t arena_bytes, znn_graph** out)
@@ -129,7 +142,34 @@ int znn_graph_op(znn_graph* zg, const char* name, const int* inputs, int n_input
     else if (op == "causalAttention")
         out = g.causalAttention(in(0), in(1), in(2), (size_t)arg(0), (size_t)arg(1), (size_t)arg(2), (float)arg(3));
     else if (op == "embedding") out = g.embedding(in(0), in(1));
-    else throw Error(ZNN_ERR_INVALID, "unknown op '" + op + "'");
+    else if (op == "tokenLogProb") {
+        Tensor* logits = in(0);
+        out = g.tokenLogProb(logits, upload_ints(zg, op, args, 1, n_args, logits->shape.dims[0]), (float)arg(0));
+    } else if (op == "policyLoss") {
+        PolicyArgs a;
+        a.clip_low = (float)arg(0);
+        a.clip_high = (float)arg(1);
+        a.kl_coef = (float)arg(2);
+        a.entropy_coef = (float)arg(3);
+        a.inv_temp = (float)arg(4);
+        int next = 3;
+        Tensor* ref = arg(5) != 0.0 ? in(next++) : nullptr;
+        Tensor* weights = arg(6) != 0.0 ? in(next++) : nullptr;
+        Tensor* logits = in(0);
+        out = g.policyLoss(logits, upload_ints(zg, op, args, 7, n_args, logits->shape.dims[0]), in(1), in(2), ref, weights, a);
+    } else if (op == "preferenceLoss") {
+        PreferenceArgs a;
+        a.beta = (float)arg(0);
+        a.label_smoothing = (float)arg(1);
+        a.margin = (float)arg(2);
+        a.length_normalize = arg(3) != 0.0;
+        const double pairs = arg(4);
+        if (!(pairs >= 1.0 && pairs < 1e9)) throw Error(ZNN_ERR_INVALID, "preferenceLoss: at least one pair is needed");
+        const int n_off = 2 * (int)pairs + 1, rest = n_args - 5 - n_off;
+        const int32_t* offsets = upload_ints(zg, op, args, 5, n_args - (rest > 0 ? rest : 0), (size_t)n_off);
+        const int32_t* targets = rest > 0 ? upload_ints(zg, op, args, 5 + n_off, n_args, in(0)->numel()) : nullptr;
+        out = g.preferenceLoss(in(0), n_inputs > 1 ? in(1) : nullptr, targets, offsets, (int)pairs, a);
+    } else throw Error(ZNN_ERR_INVALID, "unknown op '" + op + "'");
     zg->handles.push_back(out);
     if (id) *id = (int)zg->handles.size() - 1;
     ZNN_HOST_CATCH
@@ -464,6 +504,12 @@ int znn_model_set_option(znn_model* m, const char* key, double value)
     else if (k == "eps") m->adam.eps = (float)value;
     else if (k == "adam_t") m->adam.t = (float)value;
     else if (k == "momentum") m->opt.momentum = (float)value;
+    else if (k == "max_grad_norm") {
+        if (!(value >= 0.0)) throw Error(ZNN_ERR_INVALID, "max_grad_norm: a norm, or 0 to leave gradients as they are");
+        if (value > 0.0) m->ps.norm_result();   // allocated here, not inside a step that may be under capture
+        m->opt.max_norm = m->adam.max_norm = (float)value;
+        drop_graph(m);
+    }
     else if (k == "fused_softmax") {
         m->gpt.set_fused_softmax(value != 0.0);
         m->block.attn.fused_softmax = (value != 0.0);
@@ -490,23 +536,9 @@ int znn_model_set_option(znn_model* m, const char* key, double value)
     ZNN_HOST_CATCH
 }
 
-// One training step as the example programs run it (examples/fashion_mnist.zig:131-167); returns the device
-// address of the loss scalar.
-static float* run_train_step(znn_model* m, const float* x, const int32_t* targets, int batch, int seq, bool on_device)
+// Gradients of `loss` into the (zeroed) parameter slab, summed over the ranks, and the optimizer step.
+static void finish_step(znn_model* m, Graph& g, Tensor* loss)
 {
-    m->arena->reset();                       // Graph.init / graph.deinit of the previous batch
-    Graph g(m->arena.get());
-    const size_t rows = (m->kind == ZNN_MODEL_GPT) ? (size_t)batch * seq : (size_t)batch;
-    const int32_t* dev_targets = targets;
-    if (!on_device) {
-        const size_t bytes = rows * (m->targets_u8 ? 1 : sizeof(int32_t));
-        int32_t* t = (int32_t*)m->arena->alloc(bytes);
-        check(znn_memcpy_h2d(t, targets, bytes), "upload targets");
-        dev_targets = t;  // the stream synchronisation of the input upload below covers this copy
-    }
-    Tensor* logits = model_forward(*m, g, x, batch, seq, on_device);
-    Tensor* loss = m->targets_u8 ? g.softmaxCrossEntropyU8(logits, reinterpret_cast<const uint8_t*>(dev_targets))
-                                 : g.softmaxCrossEntropy(logits, dev_targets);
     m->ps.zeroGrad();                        // model.zeroGrad() (fashion_mnist.zig:155)
     int world = 1;
     znn_dp_world(&world, nullptr);
@@ -526,7 +558,145 @@ static float* run_train_step(znn_model* m, const float* x, const int32_t* target
     if (m->use_adam) m->adam.step(1.0f / (float)world);
     else m->opt.step(1.0f / (float)world);
     m->last_ops = (int)g.ops().size();
+}
+
+// One training step as the example programs run it (examples/fashion_mnist.zig:131-167); returns the device
+// address of the loss scalar.
+static float* run_train_step(znn_model* m, const float* x, const int32_t* targets, int batch, int seq, bool on_device)
+{
+    m->arena->reset();                       // Graph.init / graph.deinit of the previous batch
+    Graph g(m->arena.get());
+    const size_t rows = (m->kind == ZNN_MODEL_GPT) ? (size_t)batch * seq : (size_t)batch;
+    const int32_t* dev_targets = targets;
+    if (!on_device) {
+        const size_t bytes = rows * (m->targets_u8 ? 1 : sizeof(int32_t));
+        int32_t* t = (int32_t*)m->arena->alloc(bytes);
+        check(znn_memcpy_h2d(t, targets, bytes), "upload targets");
+        dev_targets = t;  // the stream synchronisation of the input upload below covers this copy
+    }
+    Tensor* logits = model_forward(*m, g, x, batch, seq, on_device);
+    Tensor* loss = m->targets_u8 ? g.softmaxCrossEntropyU8(logits, reinterpret_cast<const uint8_t*>(dev_targets))
+                                 : g.softmaxCrossEntropy(logits, dev_targets);
+    finish_step(m, g, loss);
     return loss->data;
+}
+
+// ---- fine-tuning steps of a GPT
+static size_t gpt_rows(znn_model* m, const char* what, int batch, int seq)
+{
+    if (!m || m->kind != ZNN_MODEL_GPT) throw Error(ZNN_ERR_INVALID, std::string(what) + ": not a GPT model");
+    if (batch <= 0 || seq <= 0) throw Error(ZNN_ERR_INVALID, std::string(what) + ": batch and seq must be positive");
+    if ((size_t)batch * seq > 0x7fffffff) throw Error(ZNN_ERR_INVALID, std::string(what) + ": more than 2^31 - 1 rows");
+    return (size_t)batch * seq;
+}
+
+// an array of the caller as device memory: itself, or a copy in the arena, which the upload of the ids behind it waits for
+static const void* device_bytes(znn_model* m, const void* p, size_t bytes, bool on_device)
+{
+    if (!p || on_device) return p;
+    void* d = m->arena->alloc(bytes);
+    check(znn_memcpy_h2d(d, p, bytes), "upload");
+    return d;
+}
+static const float* device_floats(znn_model* m, const float* p, size_t n, bool on_device)
+{
+    return (const float*)device_bytes(m, p, n * sizeof(float), on_device);
+}
+static const int32_t* device_ints(znn_model* m, const int32_t* p, size_t n, bool on_device)
+{
+    return (const int32_t*)device_bytes(m, p, n * sizeof(int32_t), on_device);
+}
+
+int znn_model_token_logprobs(znn_model* m, const float* ids, const int32_t* targets, int batch, int seq, int on_device, float inv_temp,
+                             float* logp, float* entropy)
+{
+    ZNN_HOST_TRY
+    const size_t rows = gpt_rows(m, "token_logprobs", batch, seq);
+    if (!ids || !targets || !logp) throw Error(ZNN_ERR_INVALID, "token_logprobs: ids, targets or logp is NULL");
+    m->arena->reset();
+    Graph g(m->arena.get());
+    const int32_t* t = device_ints(m, targets, rows, on_device != 0);
+    float* lp = on_device ? logp : (float*)m->arena->alloc(rows * sizeof(float));
+    float* en = on_device || !entropy ? entropy : (float*)m->arena->alloc(rows * sizeof(float));
+    Tensor* logits = model_forward(*m, g, ids, batch, seq, on_device != 0);
+    const int V = (int)m->classes;
+    check(znn_token_logprob_fwd(logits->data, V, t, inv_temp, lp, en, nullptr, (int)rows, V), "token log-probabilities");
+    if (!on_device) {
+        check(znn_memcpy_d2h(logp, lp, rows * sizeof(float)), "read log-probabilities");
+        if (entropy) check(znn_memcpy_d2h(entropy, en, rows * sizeof(float)), "read entropies");
+    }
+    ZNN_HOST_CATCH
+}
+
+int znn_model_policy_step(znn_model* m, const float* ids, const int32_t* targets, const float* old_logp, const float* ref_logp,
+                          const float* advantages, const float* weights, int batch, int seq, int on_device, float inv_temp,
+                          float clip_low, float clip_high, float kl_coef, float entropy_coef, float* loss_host)
+{
+    ZNN_HOST_TRY
+    const size_t rows = gpt_rows(m, "policy_step", batch, seq);
+    if (!ids || !targets || !old_logp || !advantages) throw Error(ZNN_ERR_INVALID, "policy_step: ids, targets, old_logp or advantages is NULL");
+    m->arena->reset();
+    Graph g(m->arena.get());
+    const bool dev = on_device != 0;
+    const int32_t* t = device_ints(m, targets, rows, dev);
+    const Shape s{rows};
+    auto column = [&](const float* p) { return p ? wrap_device(g, s, device_floats(m, p, rows, dev)) : nullptr; };
+    Tensor *old = column(old_logp), *ref = column(ref_logp), *adv = column(advantages), *w = column(weights);
+    Tensor* logits = model_forward(*m, g, ids, batch, seq, dev);
+    PolicyArgs a;
+    a.clip_low = clip_low;
+    a.clip_high = clip_high;
+    a.kl_coef = kl_coef;
+    a.entropy_coef = entropy_coef;
+    a.inv_temp = inv_temp;
+    Tensor* loss = g.policyLoss(logits, t, old, adv, ref, w, a);
+    finish_step(m, g, loss);
+    if (loss_host) check(znn_memcpy_d2h(loss_host, loss->data, sizeof(float)), "read loss");
+    ZNN_HOST_CATCH
+}
+
+int znn_model_preference_step(znn_model* m, const float* ids, const int32_t* targets, const float* ref_logp, int pairs, int seq,
+                              int on_device, float beta, float label_smoothing, float margin, int length_normalize, float* loss_host,
+                              float* rewards_host)
+{
+    ZNN_HOST_TRY
+    if (pairs <= 0 || pairs > (1 << 29)) throw Error(ZNN_ERR_INVALID, "preference_step: pairs must be positive");
+    const size_t rows = gpt_rows(m, "preference_step", 2 * pairs, seq);
+    if (!ids || !targets) throw Error(ZNN_ERR_INVALID, "preference_step: ids or targets is NULL");
+    m->arena->reset();
+    Graph g(m->arena.get());
+    const bool dev = on_device != 0;
+    const int32_t* t = device_ints(m, targets, rows, dev);
+    Tensor* ref = ref_logp ? wrap_device(g, Shape{rows}, device_floats(m, ref_logp, rows, dev)) : nullptr;
+    std::vector<int32_t> bounds(2 * (size_t)pairs + 1);   // sequence s has the rows s * seq .. (s + 1) * seq
+    for (size_t i = 0; i < bounds.size(); i++) bounds[i] = (int32_t)(i * (size_t)seq);
+    const int32_t* offsets = device_ints(m, bounds.data(), bounds.size(), false);
+    check(znn_sync(), "znn_sync");   // `bounds` is a temporary
+    Tensor* logits = model_forward(*m, g, ids, 2 * pairs, seq, dev);
+    Tensor* logp = g.tokenLogProb(logits, t, 1.0f);
+    PreferenceArgs a;
+    a.beta = beta;
+    a.label_smoothing = label_smoothing;
+    a.margin = margin;
+    a.length_normalize = length_normalize != 0;
+    float* rewards = nullptr;
+    Tensor* loss = g.preferenceLoss(logp, ref, t, offsets, pairs, a, &rewards);
+    finish_step(m, g, loss);
+    if (loss_host) check(znn_memcpy_d2h(loss_host, loss->data, sizeof(float)), "read loss");
+    if (rewards_host) check(znn_memcpy_d2h(rewards_host, rewards, 2 * (size_t)pairs * sizeof(float)), "read rewards");
+    ZNN_HOST_CATCH
+}
+
+int znn_model_grad_norm(znn_model* m, float* norm, float* factor)
+{
+    ZNN_HOST_TRY
+    if (!m || !norm) throw Error(ZNN_ERR_INVALID, "grad_norm: model or norm is NULL");
+    if (!(m->opt.max_norm > 0.0f)) throw Error(ZNN_ERR_INVALID, "grad_norm: set the option max_grad_norm first (steps measure no norm without it)");
+    float both[2];
+    check(znn_memcpy_d2h(both, m->ps.norm_result(), sizeof(both)), "read gradient norm");
+    *norm = both[0];
+    if (factor) *factor = both[1];
+    ZNN_HOST_CATCH
 }
 
 int znn_model_train_step(znn_model* m, const float* x, const int32_t* targets, int batch, int seq, int on_device,
@@ -1097,6 +1267,16 @@ int znn_param_slab_sgd_step(znn_param_slab* s, float lr, float momentum, float g
     ZNN_HOST_TRY
     if (!s) throw Error(ZNN_ERR_INVALID, "slab is NULL");
     check(znn_sgd_step(s->w, s->g, momentum > 0.0f ? s->v : nullptr, lr, momentum, grad_scale, s->total), "SGD step");
+    ZNN_HOST_CATCH
+}
+
+int znn_param_slab_sgd_step_clipped(znn_param_slab* s, float lr, float momentum, float grad_scale, float max_norm, float* result)
+{
+    ZNN_HOST_TRY
+    if (!s) throw Error(ZNN_ERR_INVALID, "slab is NULL");
+    const float* g = s->g;
+    check(znn_grad_norm(&g, &s->total, 1, grad_scale, max_norm, result), "gradient norm");
+    check(znn_sgd_step_clipped(s->w, s->g, momentum > 0.0f ? s->v : nullptr, lr, momentum, grad_scale, result, s->total), "SGD step");
     ZNN_HOST_CATCH
 }
 

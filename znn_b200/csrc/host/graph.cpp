@@ -400,6 +400,66 @@ Tensor* Graph::layerNorm(Tensor* X, Tensor* G, Tensor* B, float eps)
     return Y;
 }
 
+static int rows_of(const Tensor* logits, const char* what)
+{
+    if (logits->shape.len != 2 || logits->shape.dims[0] == 0 || logits->shape.dims[1] == 0)
+        throw Error(ZNN_ERR_INVALID, std::string(what) + ": needs 2-D logits");
+    return (int)logits->shape.dims[0];
+}
+
+Tensor* Graph::tokenLogProb(Tensor* logits, const int32_t* dev_targets, float inv_temp)
+{
+    const int M = rows_of(logits, "tokenLogProb");
+    Tensor* C = new_tensor(Shape{(size_t)M, 1}, logits->requires_grad, false);
+    Op* o = new_op(OpType::TokenLogProb, {logits}, C);
+    o->targets = const_cast<int32_t*>(dev_targets);
+    o->policy.inv_temp = inv_temp;
+    o->scratch = (float*)arena_->alloc((size_t)M * 2 * sizeof(float));
+    o->forward();
+    return C;
+}
+
+Tensor* Graph::policyLoss(Tensor* logits, const int32_t* dev_targets, Tensor* old, Tensor* advantages, Tensor* ref, Tensor* weights,
+                          const PolicyArgs& args)
+{
+    const size_t M = (size_t)rows_of(logits, "policyLoss");
+    for (const Tensor* t : {old, advantages, ref, weights})
+        if (t && t->numel() != M) throw Error(ZNN_ERR_INVALID, "policyLoss: old, advantages, ref and weights need one value per row");
+    if (!old || !advantages) throw Error(ZNN_ERR_INVALID, "policyLoss: old and advantages are needed");
+    Tensor* loss = new_tensor(Shape{1, 2}, logits->requires_grad, false);
+    Op* o = new_op(OpType::PolicyLoss, {logits, old, advantages}, loss);
+    o->targets = const_cast<int32_t*>(dev_targets);
+    o->ref = ref ? ref->data : nullptr;
+    o->weights = weights ? weights->data : nullptr;
+    o->policy = args;
+    o->arena = arena_;
+    o->scratch = (float*)arena_->alloc(M * 3 * sizeof(float));
+    o->forward();
+    return loss;
+}
+
+Tensor* Graph::preferenceLoss(Tensor* logp, Tensor* ref, const int32_t* dev_targets, const int32_t* dev_offsets, int pairs,
+                              const PreferenceArgs& args, float** rewards)
+{
+    const size_t M = logp->numel();
+    if (pairs < 1) throw Error(ZNN_ERR_INVALID, "preferenceLoss: at least one pair is needed");
+    if (M == 0 || M > 0x7fffffff) throw Error(ZNN_ERR_INVALID, "preferenceLoss: between 1 and 2^31 - 1 rows are needed");
+    if (ref && ref->numel() != M) throw Error(ZNN_ERR_INVALID, "preferenceLoss: ref needs one value per row");
+    Tensor* loss = new_tensor(Shape{1, 1}, logp->requires_grad, false);
+    Op* o = new_op(OpType::PreferenceLoss, {logp}, loss);
+    o->targets = const_cast<int32_t*>(dev_targets);
+    o->offsets = dev_offsets;
+    o->ref = ref ? ref->data : nullptr;
+    o->pairs = pairs;
+    o->preference = args;
+    const size_t n = 3 * (size_t)pairs + M;
+    o->scratch = (float*)arena_->alloc(n * sizeof(float));
+    check(znn_memset(o->scratch, 0, n * sizeof(float)), "znn_memset");   // rows of no sequence keep a gradient of 0
+    if (rewards) *rewards = o->scratch + pairs;
+    o->forward();
+    return loss;
+}
+
 Tensor* Graph::linear(Tensor* X, Tensor* W, Tensor* bias)
 {
     if (X->shape.len < 2 || W->shape.len < 2 || X->shape.dims[1] != W->shape.dims[0] || bias->numel() != W->shape.dims[1])
@@ -639,6 +699,25 @@ void Op::forward()
               "Embedding forward");
         break;
     }
+    case OpType::TokenLogProb: {
+        const int M = (int)A->shape.dims[0], N = (int)A->shape.dims[1];
+        check(znn_token_logprob_fwd(A->data, N, targets, policy.inv_temp, C->data, nullptr, scratch, M, N), "TokenLogProb forward");
+        break;
+    }
+    case OpType::PolicyLoss: {
+        // One pass makes the loss and the gradient: it goes where it belongs at once, unless something is there already.
+        const bool store = A->grad && grad_is_fresh(A);
+        if (store) grad_root(A)->grad_stored_by = this;
+        policy_loss(store ? A->grad : nullptr);
+        break;
+    }
+    case OpType::PreferenceLoss: {
+        float *pair_loss = scratch, *rewards = scratch + pairs, *dlogp = scratch + 3 * (size_t)pairs;
+        check(znn_preference_loss(A->data, ref, targets, offsets, preference.beta, preference.label_smoothing, preference.margin,
+                                  preference.length_normalize ? 1 : 0, C->data, pair_loss, rewards, dlogp, pairs, (int)A->numel()),
+              "PreferenceLoss forward");
+        break;
+    }
     case OpType::CausalAttention: {
         const long long Cw = (long long)A->shape.dims[1], hs = Cw / att_nh;
         check(znn_attn_fwd(A->data, inputs[1]->data, inputs[2]->data, C->data, scratch, att_B, att_nh, att_T, (int)hs, Cw, hs,
@@ -647,6 +726,17 @@ void Op::forward()
         break;
     }
     }
+}
+
+void Op::policy_loss(float* dlogits)
+{
+    const Tensor* A = inputs[0];
+    const int M = (int)A->shape.dims[0], N = (int)A->shape.dims[1];
+    float *token_loss = scratch, *logp = scratch + M, *entropy = scratch + 2 * (size_t)M;
+    check(znn_policy_loss(A->data, N, targets, policy.inv_temp, inputs[1]->data, ref, inputs[2]->data, weights, policy.clip_low, policy.clip_high,
+                          policy.kl_coef, policy.entropy_coef, outputs[0]->data, token_loss, logp, policy.entropy_coef != 0.0f ? entropy : nullptr,
+                          dlogits, N, M, N),
+          "PolicyLoss");
 }
 
 void Op::backward()
@@ -664,7 +754,8 @@ void Op::backward()
     const bool can_store = type == OpType::MatMul || type == OpType::BatchMatMul || type == OpType::BatchMatMulNT ||
                            type == OpType::LinearBias || type == OpType::CausalAttention ||
                            type == OpType::Gelu || type == OpType::CausalSoftmax || type == OpType::Add ||
-                           type == OpType::MulScalar || type == OpType::Reshape || type == OpType::Transpose;
+                           type == OpType::MulScalar || type == OpType::Reshape || type == OpType::Transpose ||
+                           type == OpType::TokenLogProb || type == OpType::PolicyLoss || type == OpType::PreferenceLoss;
     if (!can_store)
         for (Tensor* in : inputs) ensure_grad(in);
     switch (type) {
@@ -955,6 +1046,33 @@ void Op::backward()
                   "Embedding backward");
         break;
     }
+    case OpType::TokenLogProb:
+        if (A->requires_grad) {
+            const int M = (int)A->shape.dims[0], N = (int)A->shape.dims[1];
+            const int add = claim_grad_overwrite(A) ? 0 : 1;
+            check(znn_token_logprob_bwd(A->data, N, targets, policy.inv_temp, scratch, nullptr, C->grad, nullptr, A->grad, N, add, M, N),
+                  "TokenLogProb backward");
+        }
+        break;
+    case OpType::PolicyLoss:
+        if (A->grad) {
+            if (grad_is_fresh(A) && grad_root(A)->grad_stored_by == this) {
+                mark_grad_written(A);
+            } else {   // another op or arm was here: make the gradient once more and add it
+                float* dlogits = (float*)arena->alloc(A->numel() * sizeof(float));
+                policy_loss(dlogits);
+                ensure_grad(A);
+                check(znn_accumulate(dlogits, A->grad, A->numel()), "PolicyLoss backward");
+            }
+        }
+        break;
+    case OpType::PreferenceLoss:
+        if (A->grad) {
+            const float* dlogp = scratch + 3 * (size_t)pairs;
+            if (claim_grad_overwrite(A)) check(znn_memcpy_d2d(A->grad, dlogp, A->numel() * sizeof(float)), "PreferenceLoss backward");
+            else check(znn_accumulate(dlogp, A->grad, A->numel()), "PreferenceLoss backward");
+        }
+        break;
     case OpType::CausalAttention: {
         Tensor* Kt = inputs[1];
         Tensor* Vt = inputs[2];

@@ -54,6 +54,7 @@ struct Tensor {
     // A Reshape view that shares its input's buffer points at the owner, whose flag counts.
     bool grad_valid = true;
     Tensor* grad_owner = nullptr;
+    const Op* grad_stored_by = nullptr;   // PolicyLoss op whose forward put its gradient into the untouched buffer, the latest of them
     int consumers = 0;   // ops that read this tensor (counted while the tape is built)
     Op* last_consumer = nullptr;   // the latest of them
     size_t numel() const { return shape.numel(); }
@@ -95,9 +96,21 @@ enum class OpType {
     LayerNorm,      // extension, no reference counterpart
     LinearBias,     // fused matmul + addBias of Linear.forward (src/nn.zig:44-51), an addition
     BatchMatMulNT,  // C = A.B^T per (batch, head) slice: transposeND(K) + batchMatMul of src/nn.zig:796-835 in one op, an addition
-    CausalAttention // the whole chain of src/nn.zig:796-906 (head split, Q.K^T, scale, mask, softmax, P.V, head merge) as one
+    CausalAttention, // the whole chain of src/nn.zig:796-906 (head split, Q.K^T, scale, mask, softmax, P.V, head merge) as one
                     // fused op on the [B*T, C] projections (znn_attn_fwd / znn_attn_bwd), an addition
+    TokenLogProb, PolicyLoss, PreferenceLoss   // fine-tuning losses (znn_token_logprob_*, znn_policy_loss, znn_preference_loss), additions
 };
+
+// Settings of the fine-tuning losses, as in include/znn_cuda.h.
+struct PolicyArgs {
+    float clip_low = 0.2f, clip_high = 0.2f, kl_coef = 0.0f, entropy_coef = 0.0f, inv_temp = 1.0f;
+};
+struct PreferenceArgs {
+    float beta = 0.1f, label_smoothing = 0.0f, margin = 0.0f;
+    bool length_normalize = false;
+};
+
+class Arena;
 
 // src/autodiff.zig:100-105 (OpContext flattened)
 struct Op {
@@ -115,8 +128,20 @@ struct Op {
     float* probs = nullptr;     // SoftmaxCrossEntropy: device M x N
     int32_t* targets = nullptr; // SoftmaxCrossEntropy: device int32 labels (device bytes when targets_u8)
     bool targets_u8 = false;
+    // TokenLogProb (targets, policy.inv_temp; scratch = the rows' statistics), PolicyLoss (inputs logits, old, advantages; ref and
+    // weights below; scratch = token losses, log-probabilities, entropies), PreferenceLoss (inputs logp; ref below; scratch = pair
+    // losses, rewards, gradient)
+    PolicyArgs policy;
+    PreferenceArgs preference;
+    const float *ref = nullptr, *weights = nullptr;
+    const int32_t* offsets = nullptr;
+    int pairs = 0;
+    Arena* arena = nullptr;
     void forward();             // src/autodiff.zig:107-575
     void backward();            // src/autodiff.zig:579-1231
+
+private:
+    void policy_loss(float* dlogits);
 };
 
 // Reshape views share their input's gradient buffer (default on; off = a separate, zeroed gradient and an adding
@@ -184,6 +209,17 @@ public:
     // of C / nh columns each (src/nn.zig:796-906 in one op; no score matrix, no head split / merge copies)
     Tensor* causalAttention(Tensor* q, Tensor* k, Tensor* v, size_t B, size_t T, size_t nh, float scale);
     Tensor* layerNorm(Tensor* X, Tensor* G, Tensor* B, float eps);          // extension
+    // Log-probabilities [M, 1] of the targets under the logits [M, V]; a negative target leaves its row out.
+    Tensor* tokenLogProb(Tensor* logits, const int32_t* dev_targets, float inv_temp);
+    // Clipped policy loss on logits [M, V]; old, advantages, ref (may be null where kl_coef is 0) and weights (may be null) have M
+    // values each and get no gradient.  The result is [1, 2]: the loss, and the number of rows it was made of.  Like
+    // softmaxCrossEntropy this op (and preferenceLoss) is a root: the gradient that arrives at its output is not used.
+    Tensor* policyLoss(Tensor* logits, const int32_t* dev_targets, Tensor* old, Tensor* advantages, Tensor* ref, Tensor* weights,
+                       const PolicyArgs& args);
+    // Preference loss [1, 1] on the log-probabilities of `pairs` pairs of sequences; dev_targets and ref may be null.  `rewards`
+    // (may be null) receives the address of the 2 * pairs rewards.
+    Tensor* preferenceLoss(Tensor* logp, Tensor* ref, const int32_t* dev_targets, const int32_t* dev_offsets, int pairs,
+                           const PreferenceArgs& args, float** rewards = nullptr);
     Tensor* linear(Tensor* X, Tensor* W, Tensor* bias);                     // fused addBias(matmul(X, W), bias)
     // act(linear(X, W, bias)) with act = Relu or Gelu: the tape gets the Linear and the activation op, one GEMM fills both
     // outputs (pre-activation and activation) when the epilogue form applies

@@ -16,6 +16,7 @@ ParamStore::~ParamStore()
     if (g_) znn_free(g_);
     if (v_) znn_free(v_);
     if (v2_) znn_free(v2_);
+    if (norm_) znn_free(norm_);
 }
 
 Tensor* ParamStore::add(const std::string& name, const Shape& shape, size_t fan_in)
@@ -60,6 +61,23 @@ float* ParamStore::second_moments()
         check(znn_memset(v2_, 0, total_ * sizeof(float)), "znn_memset");
     }
     return v2_;
+}
+
+float* ParamStore::norm_result()
+{
+    if (!norm_) {
+        void* p = nullptr;
+        check(znn_malloc(&p, ZNN_GRAD_NORM_FLOATS * sizeof(float)), "gradient norm");
+        norm_ = (float*)p;
+        check(znn_memset(norm_, 0, ZNN_GRAD_NORM_FLOATS * sizeof(float)), "znn_memset");
+    }
+    return norm_;
+}
+
+void ParamStore::grad_norm(float grad_scale, float max_norm)
+{
+    const float* g = g_;
+    check(znn_grad_norm(&g, &total_, 1, grad_scale, max_norm, norm_result()), "gradient norm");   // the slab's padding is zeros
 }
 
 void ParamStore::zeroGrad()
@@ -334,14 +352,25 @@ Tensor* CnnNet::forward(Graph& g, Tensor* x) const
 
 void SGDOptimizer::step(float grad_scale) const
 {
-    check(znn_sgd_step(ps->values(), ps->grads(), momentum > 0.0f ? ps->velocities() : nullptr, lr, momentum, grad_scale,
-                       ps->total()),
-          "SGD step");
+    float* v = momentum > 0.0f ? ps->velocities() : nullptr;
+    if (max_norm > 0.0f) {
+        ps->grad_norm(grad_scale, max_norm);
+        check(znn_sgd_step_clipped(ps->values(), ps->grads(), v, lr, momentum, grad_scale, ps->norm_result(), ps->total()), "SGD step");
+        return;
+    }
+    check(znn_sgd_step(ps->values(), ps->grads(), v, lr, momentum, grad_scale, ps->total()), "SGD step");
 }
 
 void AdamOptimizer::step(float grad_scale)
 {
     t += 1.0f;
+    if (max_norm > 0.0f) {
+        ps->grad_norm(grad_scale, max_norm);
+        check(znn_adam_step_clipped(ps->values(), ps->grads(), ps->velocities(), ps->second_moments(), lr, beta1, beta2, eps, t, grad_scale,
+                                    ps->norm_result(), ps->total()),
+              "Adam step");
+        return;
+    }
     check(znn_adam_step(ps->values(), ps->grads(), ps->velocities(), ps->second_moments(), lr, beta1, beta2, eps, t,
                         grad_scale, ps->total()),
           "Adam step");

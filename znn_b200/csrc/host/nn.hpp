@@ -37,12 +37,15 @@ public:
     float* grads() { return g_; }
     float* velocities() { return v_; }
     float* second_moments();         // Adam's v slab, allocated and zeroed on first use
+    float* norm_result();            // what znn_grad_norm writes (ZNN_GRAD_NORM_FLOATS), allocated on first use
+    // the global norm of the gradients (times grad_scale) into norm_result(), with the factor that clips it to max_norm
+    void grad_norm(float grad_scale, float max_norm);
     const std::vector<ParamInfo>& params() const { return params_; }
 
 private:
     std::vector<ParamInfo> params_;
     size_t total_ = 0;
-    float *w_ = nullptr, *g_ = nullptr, *v_ = nullptr, *v2_ = nullptr;
+    float *w_ = nullptr, *g_ = nullptr, *v_ = nullptr, *v2_ = nullptr, *norm_ = nullptr;
 };
 
 // Linear.forward runs the fused matmul+addBias op by default; false = the reference's two ops.
@@ -171,6 +174,7 @@ struct CnnNet {
 struct SGDOptimizer {
     ParamStore* ps = nullptr;
     float lr = 0.01f, momentum = 0.0f;
+    float max_norm = 0.0f;   // above 0: the gradient is clipped to this global norm (an addition)
     void step(float grad_scale = 1.0f) const;
 };
 
@@ -180,6 +184,7 @@ struct AdamOptimizer {
     ParamStore* ps = nullptr;
     float lr = 0.001f, beta1 = 0.9f, beta2 = 0.999f, eps = 1e-8f;
     float t = 0.0f;
+    float max_norm = 0.0f;   // as SGDOptimizer's
     void step(float grad_scale = 1.0f);
 };
 

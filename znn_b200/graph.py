@@ -92,6 +92,20 @@ class Graph:
     def embedding(self, W, X): return self._op("embedding", [W, X])
     def linear(self, X, W, b): return self._op("linear", [X, W, b])
 
+    # fine-tuning losses (additions): see znn_policy_loss / znn_preference_loss in include/znn_cuda.h
+    def tokenLogProb(self, logits, targets, inv_temp=1.0):
+        return self._op("tokenLogProb", [logits], [inv_temp] + list(np.asarray(targets).reshape(-1)))
+
+    def policyLoss(self, logits, targets, old, advantages, ref=None, weights=None, clip=(0.2, 0.2), kl_coef=0.0, entropy_coef=0.0, inv_temp=1.0):
+        """[1, 2]: the loss and the number of rows it is made of."""
+        return self._op("policyLoss", [logits, old, advantages] + [t for t in (ref, weights) if t is not None],
+                        [clip[0], clip[1], kl_coef, entropy_coef, inv_temp, ref is not None, weights is not None] + list(np.asarray(targets).reshape(-1)))
+
+    def preferenceLoss(self, logp, offsets, ref=None, targets=None, beta=0.1, label_smoothing=0.0, margin=0.0, length_normalize=False):
+        return self._op("preferenceLoss", [logp] + ([ref] if ref is not None else []),
+                        [beta, label_smoothing, margin, length_normalize, (len(offsets) - 1) // 2] + list(offsets) +
+                        ([] if targets is None else list(np.asarray(targets).reshape(-1))))
+
     def backward(self, t): lib().call("znn_graph_backward", self.h, t.id, 1)
     def backwardWithGrad(self, t): lib().call("znn_graph_backward", self.h, t.id, 0)
     def forward(self): lib().call("znn_graph_forward", self.h)

@@ -97,6 +97,48 @@ class Model:
     def train_step_device(self, x_ptr, t_ptr, batch, seq=0, loss_ptr=None):
         lib().call("znn_model_train_step", self.h, x_ptr, t_ptr, batch, seq, 1, loss_ptr)
 
+    # ---- fine-tuning of a GPT (host arrays; the C entry points take device memory as well)
+    def token_logprobs(self, ids, targets, inv_temp=1.0, want_entropy=False):
+        """Log-probabilities [batch, seq] of the targets (negative = left out), and their entropies where asked for."""
+        ids = np.ascontiguousarray(ids, np.float32)
+        t = np.ascontiguousarray(targets, np.int32)
+        assert ids.shape == t.shape and ids.ndim == 2, (ids.shape, t.shape)
+        lp = np.empty(ids.shape, np.float32)
+        en = np.empty(ids.shape, np.float32) if want_entropy else None
+        lib().call("znn_model_token_logprobs", self.h, ids.ctypes.data, t.ctypes.data, ids.shape[0], ids.shape[1], 0, inv_temp,
+                   lp.ctypes.data, en.ctypes.data if want_entropy else None)
+        return (lp, en) if want_entropy else lp
+
+    def policy_step(self, ids, targets, old_logp, advantages, ref_logp=None, weights=None, clip=(0.2, 0.2), kl_coef=0.0,
+                    entropy_coef=0.0, inv_temp=1.0):
+        """One training step on the clipped policy loss; every array is [batch, seq].  Returns the loss."""
+        ids = np.ascontiguousarray(ids, np.float32)
+        t = np.ascontiguousarray(targets, np.int32)
+        cols = [None if a is None else np.ascontiguousarray(a, np.float32) for a in (old_logp, ref_logp, advantages, weights)]
+        assert ids.ndim == 2 and all(a is None or a.shape == ids.shape for a in [t] + cols)
+        loss = C.c_float()
+        lib().call("znn_model_policy_step", self.h, ids.ctypes.data, t.ctypes.data, *[None if a is None else a.ctypes.data for a in cols],
+                   ids.shape[0], ids.shape[1], 0, inv_temp, clip[0], clip[1], kl_coef, entropy_coef, C.byref(loss))
+        return loss.value
+
+    def preference_step(self, ids, targets, ref_logp=None, beta=0.1, label_smoothing=0.0, margin=0.0, length_normalize=False):
+        """One training step on the preference loss; ids, targets and ref_logp are [2 * pairs, seq], preferred sequences in the even rows.
+        Returns (loss, rewards [pairs, 2])."""
+        ids = np.ascontiguousarray(ids, np.float32)
+        t = np.ascontiguousarray(targets, np.int32)
+        ref = None if ref_logp is None else np.ascontiguousarray(ref_logp, np.float32)
+        assert ids.ndim == 2 and ids.shape[0] % 2 == 0 and t.shape == ids.shape and (ref is None or ref.shape == ids.shape)
+        loss, rewards = C.c_float(), np.empty((ids.shape[0] // 2, 2), np.float32)
+        lib().call("znn_model_preference_step", self.h, ids.ctypes.data, t.ctypes.data, None if ref is None else ref.ctypes.data,
+                   ids.shape[0] // 2, ids.shape[1], 0, beta, label_smoothing, margin, int(length_normalize), C.byref(loss), rewards.ctypes.data)
+        return loss.value, rewards
+
+    def grad_norm(self):
+        """(norm, clip factor) of the latest step; needs the option max_grad_norm."""
+        norm, factor = C.c_float(), C.c_float()
+        lib().call("znn_model_grad_norm", self.h, C.byref(norm), C.byref(factor))
+        return norm.value, factor.value
+
     def evaluate(self, x, labels):
         """(loss, accuracy) of one batch: host arrays, labels as bytes."""
         x = np.ascontiguousarray(x, np.float32)
