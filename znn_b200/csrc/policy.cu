@@ -875,7 +875,7 @@ static int launch_walk(const RowParams& p, int ranks)
 //            4000 x 20000: - / - / 140 / 120;  256 threads in clusters of 1 / 2 / 4 / 8: 2500 x 32000: 133 / 117 / 139 / -,
 //            1500 x 65536: 180 / 162 / 143 / 165,  700 x 131072: - / - / 152 / 136
 //   logprob  40000 x 2000: 54 / 66 / 105 / 220,  20000 x 4099: 54 / 55 / 58 / 117,  4000 x 20000: - / 59 / 54 / 59,
-//            1200 x 50257: - / 45 / 43 / 49,  1000 x 100000: - / - / 66 / 67
+//            1000 x 100000: - / - / 66 / 67,  2045 x 50257 (1.7 times the blocks of 128 threads that are resident at once): - / 57 / 60 / 58
 // Few rows are spread over clusters whatever they cost: 32 x 131072 takes 7.4 us with eight blocks per row, 8.7 with four.
 template <bool Policy, bool Entropy, bool Aligned>
 static int launch_rows_as(const RowParams& p)
@@ -890,7 +890,14 @@ static int launch_rows_as(const RowParams& p)
     }
     if (p.N <= (Policy ? 2048 : 4096)) return launch_walk<Policy, Entropy, Aligned, 32>(p, 1);
     if (p.N <= (Policy ? 5120 : 8192)) return launch_walk<Policy, Entropy, Aligned, 64>(p, 1);
-    if (!Policy || p.N <= 12288) return launch_walk<Policy, Entropy, Aligned, 128>(p, 1);
+    if constexpr (!Policy) {
+        // long rows: where the blocks of a size smaller or larger are all resident at once, that size (an SM has 1024 threads of them)
+        const int slots = sm_count() * (1024 / 64);
+        if (p.M <= slots / 4) return launch_walk<Policy, Entropy, Aligned, 256>(p, 1);
+        if (p.M > slots / 2 && p.M <= slots) return launch_walk<Policy, Entropy, Aligned, 64>(p, 1);
+        return launch_walk<Policy, Entropy, Aligned, 128>(p, 1);
+    }
+    if (p.N <= 12288) return launch_walk<Policy, Entropy, Aligned, 128>(p, 1);
     return launch_walk<Policy, Entropy, Aligned, 256>(p, p.N <= 25600 ? 1 : p.N <= 51200 ? 2 : p.N <= 102400 ? 4 : 8);
 }
 
