@@ -30,7 +30,8 @@ FWD = dict(logits=P, ld=8, targets=P, inv_temp=1.0, logp=P, entropy=P, stats=P, 
 
 @pytest.mark.parametrize("change,word", [(dict(logits=None), "NULL"), (dict(targets=None), "NULL"), (dict(logp=None), "NULL"), (dict(ld=7), "ld"),
                                          (dict(M=-1), "M"), (dict(N=0), "N"), (dict(inv_temp=0.0), "inv_temp"), (dict(inv_temp=-1.0), "inv_temp"),
-                                         (dict(inv_temp=float("nan")), "inv_temp"), (dict(inv_temp=float("inf")), "inv_temp")])
+                                         (dict(inv_temp=float("nan")), "inv_temp"), (dict(inv_temp=float("inf")), "inv_temp"),
+                                         (dict(inv_temp=3e38), "inv_temp"), (dict(logits=P + 2), "aligned")])
 def test_token_logprob_fwd(L, change, word):
     assert word in refused(L, "znn_token_logprob_fwd", *{**FWD, **change}.values())
 
@@ -40,7 +41,7 @@ BWD = dict(logits=P, ld=8, targets=P, inv_temp=1.0, stats=P, entropy=P, dlogp=P,
 
 @pytest.mark.parametrize("change,word", [(dict(logits=None), "NULL"), (dict(stats=None), "NULL"), (dict(dlogits=None), "NULL"), (dict(ld_d=7), "ld_d"),
                                          (dict(entropy=None), "entropy"), (dict(dlogits=P, accumulate=1), "own buffer"),
-                                         (dict(dlogits=P, ld_d=9), "own buffer"), (dict(M=-2), "M")])
+                                         (dict(dlogits=P, ld_d=9), "own buffer"), (dict(M=-2), "M"), (dict(dlogits=P + 3), "aligned")])
 def test_token_logprob_bwd(L, change, word):
     assert word in refused(L, "znn_token_logprob_bwd", *{**BWD, **change}.values())
 
@@ -53,7 +54,8 @@ POLICY = dict(logits=P, ld=8, targets=P, inv_temp=1.0, old=P, ref=P, adv=P, weig
                                          (dict(ref=None), "ref_logp"), (dict(lo=-0.1), "clip"), (dict(lo=1.5), "clip"), (dict(hi=-0.1), "clip"),
                                          (dict(hi=float("inf")), "clip"), (dict(lo=float("nan")), "clip"), (dict(kl=float("nan")), "finite"),
                                          (dict(ent=float("inf")), "finite"), (dict(ld_d=7), "ld_d"), (dict(dlogits=P, ld_d=9), "own buffer"),
-                                         (dict(M=0), "M"), (dict(N=-3), "N"), (dict(ld=2), "ld")])
+                                         (dict(M=0), "M"), (dict(N=-3), "N"), (dict(ld=2), "ld"), (dict(dlogits=P + 1), "aligned"),
+                                         (dict(logits=P + 1), "aligned")])
 def test_policy_loss(L, change, word):
     assert word in refused(L, "znn_policy_loss", *{**POLICY, **change}.values())
 
@@ -103,3 +105,19 @@ def test_clipped_steps(L):
     assert "step count" in refused(L, "znn_adam_step_clipped", P, P, P, P, 0.1, 0.9, 0.99, 1e-8, 0.0, 1.0, P, 5)
     refused(L, "znn_adam_step_clipped", P, P, None, P, 0.1, 0.9, 0.99, 1e-8, 1.0, 1.0, P, 5)
     assert L.call("znn_sgd_step_clipped", None, None, None, 0.1, 0.0, 1.0, None, 0) == 0   # nothing to do
+
+
+def test_arrays_of_the_wrong_size():
+    """The numpy front end: a shorter array is refused before anything is uploaded."""
+    import numpy as np
+    from znn_b200 import ops
+    x, t, v, short = np.zeros((4, 7), np.float32), np.zeros(4, np.int32), np.zeros(4, np.float32), np.zeros(3, np.float32)
+    bad = [lambda: ops.token_logprob_fwd(x, t[:3]), lambda: ops.token_logprob_fwd(v, t), lambda: ops.token_logprob_bwd(x, t, np.zeros((3, 2)), v),
+           lambda: ops.token_logprob_bwd(x, t, np.zeros((4, 2)), short), lambda: ops.token_logprob_bwd(x, t, np.zeros((4, 2)), v, dlogits=x[:3].copy()),
+           lambda: ops.policy_loss(x, t, short, v), lambda: ops.policy_loss(x, t, v, short), lambda: ops.policy_loss(x, t, v, v, short),
+           lambda: ops.policy_loss(x, t, v, v, None, short), lambda: ops.preference_loss(v, [0, 2]), lambda: ops.preference_loss(v, [0, 2, 4], short),
+           lambda: ops.preference_loss(v, [0, 2, 4], None, t[:2]), lambda: ops.preference_loss(v, [0, 2, 4], dlogp=short),
+           lambda: ops.sgd_step_clipped(v, short, None, 0.1, 0.0, 1.0), lambda: ops.adam_step_clipped(v, v, short, v, 0.1, 0.9, 0.9, 1e-8, 1.0, 1.0)]
+    for f in bad:
+        with pytest.raises(ValueError):
+            f()

@@ -642,3 +642,77 @@ def test_a_run_of_them_on_another_stream_and_captured(ops, L):
                 np.testing.assert_array_equal(a, b)
     finally:
         L.call("znn_set_stream", None)
+
+
+@pytest.mark.parametrize("M,N", [(61, 700), (700, 40), (600, 9001), (20, 40000)])
+def test_policy_loss_captured_and_on_two_streams(ops, L, M, N):
+    """Two policy losses with buffers of their own, captured on two streams and replayed at the same time, and eager ones that follow
+    one another without a wait while the inputs change in between: every result is the one of a call alone."""
+    torch = pytest.importorskip("torch")
+
+    class Call:
+        def __init__(self, seed):
+            r = np.random.default_rng(seed)
+            self.r = r
+            self.host = []
+            for _ in range(3):
+                x, t = logits(r, M, N)
+                self.host.append((np.nan_to_num(x, nan=0.0, neginf=-np.inf), t))
+            self.old, self.adv = np.full(M, -4, np.float32), r.standard_normal(M).astype(np.float32)
+            up = ops.DevBuf.from_host
+            self.xs = [up(h[0]) for h in self.host]
+            self.ts = [up(h[1]) for h in self.host]
+            self.x, self.t, self.o, self.a = ops.DevBuf(4 * M * N), ops.DevBuf(4 * M), up(self.old), up(self.adv)
+            self.loss, self.tl, self.lp, self.dx = ops.DevBuf(8), ops.DevBuf(4 * M), ops.DevBuf(4 * M), ops.DevBuf(4 * M * N)
+            self.keep = [[ops.DevBuf(8), ops.DevBuf(4 * M * N)] for _ in range(3)]
+
+        def load(self, k):
+            L.call("znn_memcpy_d2d", self.x.ptr, self.xs[k].ptr, 4 * M * N)
+            L.call("znn_memcpy_d2d", self.t.ptr, self.ts[k].ptr, 4 * M)
+
+        def run(self):
+            L.call("znn_policy_loss", self.x.ptr, N, self.t.ptr, 1.0, self.o.ptr, None, self.a.ptr, None, 0.2, 0.2, 0.0, 0.0, self.loss.ptr,
+                   self.tl.ptr, self.lp.ptr, None, self.dx.ptr, N, M, N)
+
+        def save(self, k):
+            L.call("znn_memcpy_d2d", self.keep[k][0].ptr, self.loss.ptr, 8)
+            L.call("znn_memcpy_d2d", self.keep[k][1].ptr, self.dx.ptr, 4 * M * N)
+
+        def check(self, k):
+            want = ops.policy_loss(*self.host[k], self.old, self.adv)
+            got = self.keep[k][0].to_host((2,))
+            assert got[0] == want["loss"] and got[1] == want["rows"]
+            np.testing.assert_array_equal(self.keep[k][1].to_host((M, N)), want["dlogits"])
+    calls, streams, graphs = [Call(1), Call(2)], [torch.cuda.Stream() for _ in range(2)], []
+    torch.cuda.synchronize()
+    try:
+        for k in range(3):
+            for c, st in zip(calls, streams):
+                L.call("znn_set_stream", st.cuda_stream)
+                c.load(k)
+                c.run()
+                c.save(k)
+        torch.cuda.synchronize()
+        L.call("znn_set_stream", None)
+        for c in calls:
+            for k in range(3):
+                c.check(k)
+        for c, st in zip(calls, streams):
+            L.call("znn_set_stream", st.cuda_stream)
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=st, capture_error_mode="thread_local"):
+                c.run()
+            graphs.append(g)
+        for k in (2, 0, 1):
+            for c, st, g in zip(calls, streams, graphs):
+                L.call("znn_set_stream", st.cuda_stream)
+                c.load(k)
+                with torch.cuda.stream(st):
+                    g.replay()
+                c.save(k)
+        torch.cuda.synchronize()
+    finally:
+        L.call("znn_set_stream", None)
+    for c in calls:
+        for k in range(3):
+            c.check(k)

@@ -133,6 +133,13 @@ struct RowParams {
     int* status;
 };
 
+// The kernel that counts the rows runs while this one reads the logits.  One thread of every row waits for it, of rows that are left
+// out too: when this kernel has ended, that one has, for whatever comes next on the stream.
+__device__ __forceinline__ void wait_for_count(const RowParams& p)
+{
+    if (p.count) wait_for_previous_kernel();
+}
+
 // What a row's gradient is made of: dx_j = 2^t * (a + b * t) for j != target, and dx at the target as it is.  t is measured
 // from `mx`.
 struct __align__(16) RowGrad {
@@ -181,10 +188,14 @@ __device__ __forceinline__ RowGrad row_scalars(const RowParams& p, int row, cons
     if (write) {
         if (p.logp) p.logp[row] = (float)logp;
         if (Entropy && p.entropy) p.entropy[row] = H;
-        if (p.stats) *reinterpret_cast<float2*>(p.stats + 2 * (size_t)row) = make_float2(r.mx, total);
+        if (p.stats) {
+            p.stats[2 * (size_t)row] = r.mx;
+            p.stats[2 * (size_t)row + 1] = total;
+        }
     }
     RowGrad g{0.0f, 0.0f, 0.0f, from};
     if (Policy) {
+        wait_for_count(p);
         const float A = in.advantage;
         float loss = 0.0f, slope = 0.0f;
         if (A != 0.0f) {
@@ -207,10 +218,7 @@ __device__ __forceinline__ RowGrad row_scalars(const RowParams& p, int row, cons
         if (write) p.token_loss[row] = loss;
         if (!empty) {
             float w = in.w;
-            if (!p.weights) {
-                if (p.count) wait_for_previous_kernel();   // which counts the rows while this one reads the logits
-                w = 1.0f / (p.count ? *p.count : (float)rows);
-            }
+            if (!p.weights) w = 1.0f / (p.count ? *p.count : (float)rows);
             const float G = p.it * w * slope, E = Entropy ? -p.it * w * p.entropy_coef : 0.0f;
             // p_t, and 1 - p_t: where the target is the largest, what the others sum to; elsewhere p_t is at most 1/2
             const float top = base_of(r.mx), e_t = x_t == top ? 1.0f : exp2_fast(fmaxf((x_t - top) * p.c, kNothing));
@@ -241,6 +249,7 @@ template <bool Policy>
 __device__ __forceinline__ void row_unused(const RowParams& p, int row, bool bad)
 {
     const float v = bad ? CUDART_NAN_F : 0.0f;
+    if (Policy) wait_for_count(p);
     if (p.logp) p.logp[row] = v;
     if (p.entropy) p.entropy[row] = 0.0f;
     if (p.stats) {
@@ -952,7 +961,8 @@ static int check_rows(const float* logits, long long ld, const int32_t* targets,
     ZNN_REQUIRE(M >= 0 && N > 0, "M must not be negative and N must be positive");
     ZNN_REQUIRE(M == 0 || (logits && targets), "NULL pointer");
     ZNN_REQUIRE(ld >= N, "ld = %lld is smaller than N = %d", ld, N);
-    ZNN_REQUIRE(inv_temp > 0.0f && isfinite(inv_temp), "inv_temp must be positive and finite");
+    ZNN_REQUIRE(((uintptr_t)logits & 3) == 0, "logits are not aligned to 4 bytes");
+    ZNN_REQUIRE(inv_temp > 0.0f && inv_temp < 1e38f, "inv_temp must be positive and finite (below 1e38)");
     return ZNN_OK;
 }
 
@@ -980,6 +990,7 @@ int znn_token_logprob_bwd(const float* logits, long long ld, const int32_t* targ
     if (rc != ZNN_OK) return rc;
     if (M == 0) return ZNN_OK;
     ZNN_REQUIRE(stats && dlogits, "stats/dlogits is NULL");
+    ZNN_REQUIRE(((uintptr_t)dlogits & 3) == 0, "dlogits are not aligned to 4 bytes");
     ZNN_REQUIRE(!dentropy || entropy, "dentropy needs the forward's entropy");
     ZNN_REQUIRE(ld_d >= N, "ld_d = %lld is smaller than N = %d", ld_d, N);
     ZNN_REQUIRE(dlogits != logits || (ld_d == ld && !accumulate), "dlogits may be the logits' own buffer only with ld_d == ld and accumulate = 0");
@@ -998,6 +1009,7 @@ int znn_policy_loss(const float* logits, long long ld, const int32_t* targets, f
     if (rc != ZNN_OK) return rc;
     ZNN_REQUIRE(M > 0, "M must be positive");
     ZNN_REQUIRE(old_logp && advantages && loss && token_loss, "NULL pointer");
+    ZNN_REQUIRE(((uintptr_t)dlogits & 3) == 0, "dlogits are not aligned to 4 bytes");
     ZNN_REQUIRE(isfinite(kl_coef) && isfinite(entropy_coef), "kl_coef and entropy_coef must be finite");
     ZNN_REQUIRE(ref_logp || kl_coef == 0.0f, "kl_coef needs ref_logp");
     ZNN_REQUIRE(clip_low >= 0.0f && clip_low <= 1.0f && clip_high >= 0.0f && isfinite(clip_high),

@@ -621,11 +621,26 @@ def sgd_step(w, g, v, lr, momentum, grad_scale=1.0):
 
 
 # ---- fine-tuning losses and clipping by the global gradient norm (include/znn_cuda.h) ----
+def _sizes(n, **arrays):
+    """Refuses arrays that do not have n values: the calls below take pointers and would read past the end of a shorter one."""
+    for name, a in arrays.items():
+        if a is not None and np.size(a) != n:
+            raise ValueError(f"{name} has {np.size(a)} values, {n} are needed")
+
+
+def _matrix(logits):
+    logits = _f(logits)
+    if logits.ndim != 2:
+        raise ValueError(f"logits have {logits.ndim} dimensions, 2 are needed")
+    return logits
+
+
 def token_logprob_fwd(logits, targets, inv_temp=1.0, want_entropy=True):
     """(logp[M], entropy[M] or None, stats[M, 2]) of the target tokens; a negative target leaves its row out."""
-    _ensure()
-    logits = _f(logits)
+    logits = _matrix(logits)
     M, N = logits.shape
+    _sizes(M, targets=targets)
+    _ensure()
     x, t = _up(logits), _up(targets, np.int32)
     lp, st = DevBuf(M * 4), DevBuf(M * 8)
     en = DevBuf(M * 4) if want_entropy else None
@@ -635,9 +650,12 @@ def token_logprob_fwd(logits, targets, inv_temp=1.0, want_entropy=True):
 
 def token_logprob_bwd(logits, targets, stats, dlogp, dlogits=None, entropy=None, dentropy=None, inv_temp=1.0):
     """Gradient of the logits; added to dlogits in place where that is given, returned as a fresh array otherwise."""
-    _ensure()
-    logits = _f(logits)
+    logits = _matrix(logits)
     M, N = logits.shape
+    _sizes(M, targets=targets, dlogp=dlogp, entropy=entropy, dentropy=dentropy)
+    _sizes(2 * M, stats=stats)
+    _sizes(M * N, dlogits=dlogits)
+    _ensure()
     x, t, st, g = _up(logits), _up(targets, np.int32), _up(stats), _up(dlogp)
     en, h = _up(entropy), _up(dentropy)
     out = _up(dlogits) if dlogits is not None else DevBuf(logits.nbytes)
@@ -652,9 +670,10 @@ def token_logprob_bwd(logits, targets, stats, dlogp, dlogits=None, entropy=None,
 def policy_loss(logits, targets, old_logp, advantages, ref_logp=None, weights=None, clip=(0.2, 0.2), kl_coef=0.0,
                 entropy_coef=0.0, inv_temp=1.0, want_grad=True):
     """Clipped policy loss: dict with loss, rows, token_loss[M], logp[M], entropy[M] and dlogits[M, N] (None without want_grad)."""
-    _ensure()
-    logits = _f(logits)
+    logits = _matrix(logits)
     M, N = logits.shape
+    _sizes(M, targets=targets, old_logp=old_logp, advantages=advantages, ref_logp=ref_logp, weights=weights)
+    _ensure()
     x, t, old, adv = _up(logits), _up(targets, np.int32), _up(old_logp), _up(advantages)
     ref, w = _up(ref_logp), _up(weights)
     loss, tl, lp, en = DevBuf(8), DevBuf(M * 4), DevBuf(M * 4), DevBuf(M * 4)
@@ -670,9 +689,11 @@ def preference_loss(logp, seq_offsets, ref_logp=None, targets=None, beta=0.1, la
                     length_normalize=False, dlogp=None):
     """Preference loss on the pairs of sequences that seq_offsets (2P + 1 row numbers) cut out of logp: dict with loss,
     pair_loss[P], rewards[2P] and dlogp[M] (rows of no sequence keep what `dlogp` gives them, 0 by default)."""
-    _ensure()
     logp = _f(logp)
     M, P = logp.size, (len(seq_offsets) - 1) // 2
+    _sizes(2 * P + 1, seq_offsets=seq_offsets)
+    _sizes(M, ref_logp=ref_logp, targets=targets, dlogp=dlogp)
+    _ensure()
     lp, ref, t, off = _up(logp), _up(ref_logp), _up(targets, np.int32), _up(seq_offsets, np.int32)
     loss, pl, rw = DevBuf(4), DevBuf(P * 4), DevBuf(2 * P * 4)
     g = _up(np.zeros(M, np.float32) if dlogp is None else dlogp)
@@ -716,6 +737,7 @@ def clip_grads(grads, max_norm, grad_scale=1.0):
 
 def sgd_step_clipped(w, g, v, lr, momentum, max_norm, grad_scale=1.0):
     """One SGD step on w (and v), in place, with the gradient clipped to max_norm; returns (norm, factor)."""
+    _sizes(w.size, g=g, v=v)
     _ensure()
     dw, dv = _up(w), _up(v)
     bufs, ptrs, counts = _grad_set([g])
@@ -731,6 +753,7 @@ def sgd_step_clipped(w, g, v, lr, momentum, max_norm, grad_scale=1.0):
 
 def adam_step_clipped(w, g, m, v, lr, beta1, beta2, eps, t, max_norm, grad_scale=1.0):
     """One Adam step on w, m, v, in place, with the gradient clipped to max_norm; returns (norm, factor)."""
+    _sizes(w.size, g=g, m=m, v=v)
     _ensure()
     dw, dm, dv = _up(w), _up(m), _up(v)
     bufs, ptrs, counts = _grad_set([g])
