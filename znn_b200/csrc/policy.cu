@@ -780,6 +780,7 @@ preference_pair_kernel(const float* __restrict__ logp, const float* __restrict__
         slopes[1] = (float)(-t.slope * share[1]);
         if (rank == 0) {
             pair_loss[pair] = (float)t.loss;
+            if (!Small && P == 1) *loss = (float)t.loss;
             rewards[2 * pair] = (float)reward[0];
             rewards[2 * pair + 1] = (float)reward[1];
             if (!usable && status) atomicOr(status, ZNN_DEV_BAD_INDEX);
@@ -1056,7 +1057,7 @@ int znn_preference_loss(const float* logp, const float* ref_logp, const int32_t*
                    : rows > 1024                       ? ZNN_PAIRS(false, 256, P, 256, 1)
                                                        : ZNN_PAIRS(false, 64, P, 64, 1);
 #undef ZNN_PAIRS
-    if (rc != ZNN_OK) return rc;
+    if (rc != ZNN_OK || P == 1) return rc;   // (a single pair's loss is the mean)
     return launch(mean_kernel, "mean_kernel", 1, 1024, 1, true, (const float*)pair_loss, loss, P);
 }
 
