@@ -111,8 +111,9 @@ __device__ __forceinline__ double log_of_sum(float ties, float s)
     return (double)((bits >> 23) - 127) * 0.693147180559945309417 + (double)logf(__int_as_float((bits & 0x007fffff) | 0x3f800000)) + (total - total);
 }
 
-// A kernel that was launched with `overlap` may begin while the one before it still runs: it waits here before it reads what that
-// one writes.  That one lets it begin as soon as all of its own blocks run.
+// Every kernel here may begin while the one before it on the stream still runs, and waits here for that one's end and for what it
+// wrote: the launch itself then costs no time between them.  Only the rows of a policy loss begin without, beside the kernel that
+// counts them, which has waited before it let them begin.
 __device__ __forceinline__ void wait_for_previous_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void let_next_kernel_begin() { asm volatile("griddepcontrol.launch_dependents;"); }
 
@@ -417,6 +418,7 @@ __global__ void __launch_bounds__(128) rows_held_kernel(const RowParams p, int)
     const unsigned mask = Group < 32 ? ((1u << (Group & 31)) - 1) << (threadIdx.x & 31 & ~(Group - 1)) : kAllLanes;
     const unsigned row = blockIdx.x * (128 / Group) + threadIdx.x / Group;
     if (row >= (unsigned)p.M) return;
+    if (!Policy || !p.count) wait_for_previous_kernel();
     const float* x = p.logits + (size_t)row * p.ld;
     float* dx = Policy && p.dlogits ? p.dlogits + (size_t)row * p.ld_d : nullptr;
     RowPart<Group, V, Aligned> r;
@@ -500,6 +502,7 @@ __global__ void __launch_bounds__(Threads) rows_walk_kernel(const RowParams p, i
         __syncwarp();
         cluster_arrive();   // waited for when the first walk is done: by then every block runs and has its barrier
     }
+    if (!Policy || !p.count) wait_for_previous_kernel();
     const int row = blockIdx.x / ranks, first = rank * part, n = max(0, min(part, p.N - first));
     const float* x = p.logits + (size_t)row * p.ld + first;
     float* dx = Policy && p.dlogits ? p.dlogits + (size_t)row * p.ld_d + first : nullptr;
@@ -604,6 +607,7 @@ logprob_bwd_kernel(const float* logits, long long ld, const int32_t* __restrict_
     const unsigned unit = Group < 256 ? blockIdx.x * (128 / Group) + threadIdx.x / Group : blockIdx.x;
     const int row = (int)(unit / (unsigned)parts), first = (int)(unit % (unsigned)parts) * part, n = min(part, N - first);
     if (row >= M) return;
+    wait_for_previous_kernel();
     const float* x = logits + (size_t)row * ld + first;
     float* dx = dlogits + (size_t)row * ld_d + first;
     const int t = targets[row];
@@ -643,8 +647,8 @@ policy_total_kernel(const int32_t* __restrict__ targets, const float* __restrict
     __shared__ double sh[32], sh_all[2][8];
     const int ranks = cluster_size(), rank = cluster_rank();
     if (ranks > 1) cluster_sync_all();   // a block must run before another writes to its memory
-    if (with_sum) wait_for_previous_kernel();
-    else let_next_kernel_begin();
+    wait_for_previous_kernel();
+    if (!with_sum) let_next_kernel_begin();
     int rows = 0;
     double sum = 0.0;
 #pragma unroll 8
@@ -703,6 +707,7 @@ preference_pair_kernel(const float* __restrict__ logp, const float* __restrict__
     __shared__ float sh_slope[2];
     const int ranks = cluster_size(), rank = cluster_rank(), tid = Small ? threadIdx.x & 31 : threadIdx.x;
     if (ranks > 1) cluster_sync_all();   // a block must run before another writes to its memory
+    wait_for_previous_kernel();
     const int pair = Small ? threadIdx.x >> 5 : blockIdx.x / ranks;
     const unsigned step = Small ? 32 : Threads * ranks, start = Small ? tid : rank * Threads + tid;
     int o[3];
@@ -839,9 +844,9 @@ using namespace znn;
     } while (0)
 
 // ---- launches
-// A launch in clusters of `ranks` blocks; overlap: it may begin while the kernel before it still runs.
+// A launch in clusters of `ranks` blocks that may begin while the kernel before it still runs.
 template <class... Params, class... Args>
-static int launch(void (*kernel)(Params...), const char* name, long long blocks, int threads, int ranks, bool overlap, Args... args)
+static int launch(void (*kernel)(Params...), const char* name, long long blocks, int threads, int ranks, Args... args)
 {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)blocks);
@@ -852,10 +857,8 @@ static int launch(void (*kernel)(Params...), const char* name, long long blocks,
         attrs[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
         attrs[cfg.numAttrs++].val.clusterDim = {(unsigned)ranks, 1, 1};
     }
-    if (overlap) {
-        attrs[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attrs[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
-    }
+    attrs[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attrs[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attrs;
     ZNN_CUDA_OK(cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...));
     ZNN_LAUNCH_OK(name);
@@ -867,7 +870,7 @@ static int launch_held(const RowParams& p)
 {
     constexpr int rows = 128 / Group;
     return launch(rows_held_kernel<Policy, Entropy, Aligned, Group, V>, "rows_held_kernel", (p.M + (long long)rows - 1) / rows, 128, 1,
-                  Policy && p.count, p, 0);
+                  p, 0);
 }
 
 template <bool Policy, bool Entropy, bool Aligned, int Threads>
@@ -875,7 +878,7 @@ static int launch_walk(const RowParams& p, int ranks)
 {
     const int part = (ceil_div(p.N, ranks) + 3) & ~3;   // parts start where the row's quads do
     return launch(rows_walk_kernel<Policy, Entropy, Aligned, Threads, 8>, "rows_walk_kernel", (long long)p.M * ranks, Threads, ranks,
-                  Policy && p.count, p, part);
+                  p, part);
 }
 
 // Which kernel: 8 lanes per row up to 256 columns, a warp up to 1024, then blocks that walk.  A block costs the same few
@@ -940,10 +943,8 @@ static int launch_bwd(const BwdArgs& b)
     constexpr int fit = 4 * Group * V;
     const int part = (ceil_div(b.N, ceil_div(b.N, fit)) + 3) & ~3, parts = ceil_div(b.N, part);
     const long long units = (long long)b.M * parts;
-    logprob_bwd_kernel<Accumulate, Aligned, Group, V><<<(unsigned)((units + rows - 1) / rows), Group < 256 ? 128 : Group, 0, stream()>>>(
-        b.logits, b.ld, b.targets, b.it, b.stats, b.entropy, b.dlogp, b.dentropy, b.dlogits, b.ld_d, b.M, b.N, parts, part);
-    ZNN_LAUNCH_OK("logprob_bwd_kernel");
-    return ZNN_OK;
+    return launch(logprob_bwd_kernel<Accumulate, Aligned, Group, V>, "logprob_bwd_kernel", (units + rows - 1) / rows, Group < 256 ? 128 : Group, 1,
+                  b.logits, b.ld, b.targets, b.it, b.stats, b.entropy, b.dlogp, b.dentropy, b.dlogits, b.ld_d, b.M, b.N, parts, part);
 }
 
 template <bool Accumulate, bool Aligned>
@@ -1027,12 +1028,12 @@ int znn_policy_loss(const float* logits, long long ld, const int32_t* targets, f
     const int total_ranks = M > 4096 ? 8 : 1;
     if (!weights && M > 512) {   // the rows' weight 1 / count is needed before their gradients are written
         p.count = loss + 1;
-        const int counted = launch(policy_total_kernel, "policy_total_kernel", total_ranks, 1024, total_ranks, false, targets, weights, token_loss, loss, M, 0);
+        const int counted = launch(policy_total_kernel, "policy_total_kernel", total_ranks, 1024, total_ranks, targets, weights, token_loss, loss, M, 0);
         if (counted != ZNN_OK) return counted;
     }
     const int done = launch_rows<true>(p, entropy || entropy_coef != 0.0f);
     if (done != ZNN_OK) return done;
-    return launch(policy_total_kernel, "policy_total_kernel", total_ranks, 1024, total_ranks, true, targets, weights, token_loss, loss, M, 1);
+    return launch(policy_total_kernel, "policy_total_kernel", total_ranks, 1024, total_ranks, targets, weights, token_loss, loss, M, 1);
 }
 
 int znn_preference_loss(const float* logp, const float* ref_logp, const int32_t* targets, const int32_t* seq_offsets, float beta,
@@ -1046,7 +1047,7 @@ int znn_preference_loss(const float* logp, const float* ref_logp, const int32_t*
     ZNN_REQUIRE(label_smoothing >= 0.0f && label_smoothing < 1.0f, "label_smoothing must lie in [0, 1)");
     ZNN_NEED_DEVICE();
 #define ZNN_PAIRS(small, threads, blocks, used, ranks)                                                                                    \
-    launch(preference_pair_kernel<small, threads>, "preference_pair_kernel", blocks, used, ranks, false, logp, ref_logp, targets, seq_offsets, \
+    launch(preference_pair_kernel<small, threads>, "preference_pair_kernel", blocks, used, ranks, logp, ref_logp, targets, seq_offsets, \
            beta, label_smoothing, margin, length_normalize, loss, pair_loss, rewards, dlogp, P, M, device_status_word())
     // A warp per pair in one launch for small calls.  Few pairs of long sequences: eight blocks each, where one block's own bandwidth
     // (about 100 GB/s) would be the limit.  Many short ones: small blocks.
@@ -1058,7 +1059,7 @@ int znn_preference_loss(const float* logp, const float* ref_logp, const int32_t*
                                                        : ZNN_PAIRS(false, 64, P, 64, 1);
 #undef ZNN_PAIRS
     if (rc != ZNN_OK || P == 1) return rc;   // (a single pair's loss is the mean)
-    return launch(mean_kernel, "mean_kernel", 1, 1024, 1, true, (const float*)pair_loss, loss, P);
+    return launch(mean_kernel, "mean_kernel", 1, 1024, 1, (const float*)pair_loss, loss, P);
 }
 
 }  // extern "C"
