@@ -1,7 +1,9 @@
 // Global gradient norm over a set of tensors, clipping by it, and the optimizer steps that take the factor from device
 // memory.  Compiled with -fmad=false like rowops.cu: the steps round where znn_sgd_step and znn_adam_step do.
 //
-// Bound by HBM: 4 bytes per gradient for the norm, 20 (SGD with momentum) or 28 (Adam) for a step.
+// Bound by HBM: 4 bytes per gradient for the norm, 20 (SGD with momentum) or 28 (Adam) for a step.  Measured on a B200 whose copies
+// run at 6548 GB/s: norm of 98 million floats 61 us, 6.5 TB/s; Adam step on them 395 us, 6.8 TB/s of the 2.69 GB that cross HBM (the
+// gradients that the norm read last come from L2); both as called 470 us.
 #include <cooperative_groups.h>
 #include <math.h>
 
@@ -77,8 +79,9 @@ struct Tile {
 };
 
 // Squares of the tiles first, first + step, ...: fp64 from the first product on, so that no finite gradient overflows or vanishes
-// and sums of any length keep their digits.  (A conversion and a fused multiply-add per float: a fifth of what the fp64 pipe can
-// do at the rate at which the floats arrive.)
+// and sums of any length keep their digits.  A conversion and a fused multiply-add per float cost nothing beside the loads (the
+// schedulers issue in 37 % of the cycles); what counts is that the next tile's loads are under way meanwhile (24 layers of width
+// 1000: 148 us without, 135 us with).
 template <int Cap>
 __device__ __forceinline__ double squares(const TensorTable<Cap>& t, int first, int step)
 {

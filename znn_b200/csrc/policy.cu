@@ -1,7 +1,13 @@
 // Fine-tuning losses on a language model's logits: token log-probabilities (forward, backward), the clipped policy loss
 // with its gradient, the preference loss on pairs of sequences.  Formulas: include/znn_cuda.h.
 //
-// Every operator is bound by HBM: 10 to 20 operations per logit against 4 to 12 bytes.
+// Bound by HBM where there is enough to do (10 to 20 operations per logit against 4 to 12 bytes), by launch and reduction latency
+// where there is not.  Measured on a B200 whose copies run at 6548 GB/s, the whole call, inputs in turn from three sets:
+//   log-probabilities and entropies 2045 x 50257, a fifth left out  58 us  5.7 TB/s     (floor 50 us)
+//   their gradient with entropy term 8192 x 8192, a tenth left out  79 us  6.4 TB/s     (78 us)
+//   policy loss 8192 x 8192, KL term                                92 us  5.8 TB/s     (82 us)
+//   policy loss 2048 x 131000, KL and entropy, 0.15 left out       342 us  5.8 TB/s     (303 us)
+//   preference loss 700 pairs, 1.4 million rows                     12 us               (3.4 us: latency)
 #include <math.h>
 #include <math_constants.h>
 
@@ -18,9 +24,9 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 // Where exp2() is 0 in fp32 whatever comes after the point.  Exponents are clamped to it, so that no 0 * inf arises.
 constexpr float kNothing = -150.0f;
 
-// 2^x as the special-function unit gives it (2 units in the last place, subnormal results 0).  The exponentials of this file
+// 2^x as the special-function unit gives it (relative error below 2^-22, subnormal results 0).  The exponentials of this file
 // are 2^t with t = (x - xm) * inv_temp * log2(e): a subtraction, a product and this, where expf() would take twice as many
-// operations after the same two roundings, and the kernels here are as near to the issue rate as to the memory's.
+// operations after the same two roundings, and the kernels issue in half to two thirds of all cycles as it is.
 __device__ __forceinline__ float exp2_fast(float x)
 {
     float y;
@@ -148,8 +154,7 @@ struct __align__(16) RowGrad {
 };
 
 // What decides whether a row is used: its target and (policy loss) its weight.  With them, in the thread that makes the row's
-// scalars (`inputs`), the row's entries of the other inputs.  All of it is fetched well ahead: behind the rows that are on
-// their way, a single load takes microseconds.
+// scalars (`inputs`), the row's entries of the other inputs: they are on their way while the row is walked over, instead of behind it.
 struct RowHead {
     int t;
     float w, old_logp, ref_logp, advantage;
@@ -289,12 +294,15 @@ struct RowPart {
         return tid < head ? tid : tid >= 4 && after < n ? after : -1;
     }
 
+    // Last: nobody reads these logits again, so that they leave L2 before those that are read once more
+    template <bool Last = false>
     __device__ __forceinline__ void load(const float* x, int tid)
     {
 #pragma unroll
         for (int k = 0; k < V; k++) {
             float4 q = make_float4(-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F);
-            if (has(tid, k)) q = *reinterpret_cast<const float4*>(x + column(tid, k));
+            const float4* from = reinterpret_cast<const float4*>(x + column(tid, k));
+            if (has(tid, k)) q = Last ? __ldcs(from) : *from;
             v[k][0] = q.x; v[k][1] = q.y; v[k][2] = q.z; v[k][3] = q.w;
         }
         const int c = extra_column(tid);
@@ -304,7 +312,7 @@ struct RowPart {
     // whether the part's quads are quads of the row y as well
     __device__ __forceinline__ bool same_quads(const float* y) const { return Aligned || ((uintptr_t)(y + head) & 15) == 0; }
 
-    // adds the same columns of a row of any alignment to what v holds
+    // the same columns of a row of any alignment
     __device__ __forceinline__ void load_beside(const float* y, int tid, float (&o)[V][4], float& o_extra) const
     {
         const bool quad = same_quads(y);
@@ -410,7 +418,9 @@ __device__ __forceinline__ void exchange(RowWord* word, const RowSums& mine, int
 }
 
 // Short rows: 8 lanes or a warp hold a whole row in registers from its load to the gradient's store.  The maximum comes first, so
-// that every exponential is taken once, relative to it.
+// that every exponential is taken once, relative to it.  Log-probabilities 65536 x 1000: 40 us, 6.5 TB/s; policy loss with KL term
+// 100 us, 5.3 TB/s: the row's scalars and reductions show, and are most of the work below a few hundred columns (1000000 x 100:
+// 369 us, 2.3 TB/s).
 template <bool Policy, bool Entropy, bool Aligned, int Group, int V>
 __global__ void __launch_bounds__(128) rows_held_kernel(const RowParams p, int)
 {
@@ -482,8 +492,14 @@ __global__ void __launch_bounds__(128) rows_held_kernel(const RowParams p, int)
     if (r.owns(in.t, tid)) dx[in.t] = g.at_target;
 }
 
-// Rows that need not be held (log-probabilities alone) or cannot be (longer than a cluster's registers): a block walks over the
-// row with running sums per thread, and a second time for the gradient; short calls give a row to a cluster of blocks.
+// Longer rows: a block (or the blocks of a cluster, which take `part` columns each) walks over the row with running sums per thread,
+// and for the gradient a second time, back from the end, through the L2 cache: 8 bytes per logit cross HBM, not 12 (2048 x 131000:
+// 0.94 GB read, 1.02 GB written, 343 us).  Small blocks with few registers are what makes it fast: a row's chain of loads,
+// reductions and scalars takes microseconds, and enough other rows must be under way meanwhile.  Rows held in registers, by blocks
+// of 256 or 512 threads and clusters of them, took 580 us for the same, since too few blocks per SM hid too little of that chain
+// (copying the next row to shared memory ahead made it worse: 8192 x 8192 110 -> 138 us, where this form takes 92).
+// Rows of some 30 to 60 thousand columns lie between one block a row and small parts, and their second pass misses L2 most often:
+// 2000 x 50256 154 us (floor 123); 161 without the second pass's loads marked as the last, and 173 against 158 for 50257.
 template <bool Policy, bool Entropy, bool Aligned, int Threads, int kQuads>
 __global__ void __launch_bounds__(Threads) rows_walk_kernel(const RowParams p, int part)
 {
@@ -591,12 +607,13 @@ __global__ void __launch_bounds__(Threads) rows_walk_kernel(const RowParams p, i
         if (r.owns(at, tid)) dx[at] = g.at_target;
         if (r.step == 0) break;
         r.step -= kStep;
-        r.load(x, tid);
+        r.template load<true>(x, tid);
     }
 }
 
 // dlogits of the log-probabilities from the forward's statistics.  A group of threads takes 4 * Group * V columns of a row;
-// every load of the logits, and of the gradient that is added to, is under way before the first result is made.
+// every load of the logits, and of the gradient that is added to, is under way before the first result is made.  8192 x 8192: 76 us,
+// 6.7 TB/s.
 template <bool Accumulate, bool Aligned, int Group, int V>
 __global__ void __launch_bounds__(Group < 256 ? 128 : Group)
 logprob_bwd_kernel(const float* logits, long long ld, const int32_t* __restrict__ targets, float it,
