@@ -100,7 +100,7 @@ int znn_model_get_velocities(znn_model* m, float* host_slab);
  * "optimizer" (0 = SGD with "lr" / "momentum" as the example programs use, 1 = Adam, src/optim.zig:69-152, with "lr",
  * "beta1", "beta2", "eps" and the step count "adam_t"; no CUDA-graph replay with Adam: the step size changes per step),
  * "max_grad_norm" (above 0: every step's gradients, after the data-parallel sum, are clipped to this global norm, and a step whose
- * norm is not finite leaves parameters and optimizer state as they are; 0, the default, is off),
+ * norm is not finite leaves parameters and optimizer state as they are, though "adam_t" counts it; 0, the default, is off),
  * "targets_u8" (1/0: the targets pointer of znn_model_train_step holds byte labels, the reference's label type,
  * e.g. the y_dest of znn_loader_next_into; default 0 = int32) */
 int znn_model_set_option(znn_model* m, const char* key, double value);
@@ -117,7 +117,8 @@ int znn_model_train_step(znn_model* m, const float* x, const int32_t* targets, i
  *   policy step calls old_logp or ref_logp, what a preference step calls ref_logp.
  * znn_model_policy_step, znn_model_preference_step: one training step each, as znn_model_train_step (forward, loss, zeroGrad,
  *   backward, gradient all-reduce, clipping where max_grad_norm is set, optimizer).  Preference: 2 * pairs sequences of seq ids,
- *   the preferred and the other one of each pair in turn; rewards_host receives 2 * pairs values.
+ *   the preferred and the other one of each pair in turn; rewards_host receives 2 * pairs values.  Data parallel: every rank takes
+ *   the mean over its own rows or pairs, and the ranks' gradients are averaged.
  * znn_model_grad_norm: norm and clip factor (may be NULL) of the latest step, while the option max_grad_norm is set. */
 int znn_model_token_logprobs(znn_model* m, const float* ids, const int32_t* targets, int batch, int seq, int on_device, float inv_temp,
                              float* logp, float* entropy);
