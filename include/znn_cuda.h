@@ -290,7 +290,7 @@ int znn_token_logprob_bwd(const float* logits, long long ld, const int32_t* targ
  *   loss[0] = sum_i w_i l_i,  w_i = weights[i], or 1 / (number of rows not left out) where weights is NULL (0 when there is
  *   none); a row of weight 0 is left out.  loss[1] = the number of rows not left out.
  * token_loss[M] = l; logp[M] and entropy[M] (either may be NULL) as above; dlogits = d loss[0] / d logits, stored, NULL = the
- * loss alone; it may be the logits' own buffer (ld_d == ld).  ref_logp may be NULL where kl_coef is 0. */
+ * loss alone; it may be the logits' own buffer (ld_d == ld).  ref_logp may be NULL where kl_coef is 0.  M must be positive. */
 int znn_policy_loss(const float* logits, long long ld, const int32_t* targets, float inv_temp, const float* old_logp,
                     const float* ref_logp, const float* advantages, const float* weights, float clip_low, float clip_high,
                     float kl_coef, float entropy_coef, float* loss, float* token_loss, float* logp, float* entropy,
@@ -378,7 +378,8 @@ int znn_adam_step(float* w, const float* g, float* m, float* v, float lr, float 
  *   order: no overflow or underflow for any finite fp32 gradients, and the same bits every time.  max_norm = INFINITY: the
  *   norm alone.  `result` is ZNN_GRAD_NORM_FLOATS floats of device memory, 16-byte aligned; what follows the two values is the
  *   call's workspace.  Give calls that may run at the same time (two streams, two captured graphs) a result each.
- * znn_clip_grads: grads *= result[1], in place; a factor of 1 or 0 leaves them untouched.
+ *   A tensor that is listed twice counts twice.
+ * znn_clip_grads: grads *= result[1], in place; a factor of 1 or 0 leaves them untouched.  Tensors that overlap are refused.
  * znn_sgd_step_clipped, znn_adam_step_clipped: znn_sgd_step / znn_adam_step with the gradient multiplied by
  *   grad_scale * result[1], read on the device: no pass over the gradients for the clipping and nothing for the host to wait
  *   for.  A factor of 0 (the norm was not finite) skips the step: w, v and m stay as they are.  With a factor of 1 the result is

@@ -87,6 +87,8 @@ def test_gradient_set(L):
     assert "NULL" in refused(L, "znn_grad_norm", None, c, n, 1.0, 1.0, P)
     assert "NULL" in refused(L, "znn_clip_grads", g, None, n, P)
     assert "result" in refused(L, "znn_clip_grads", g, c, n, None)
+    for spans in (((P, 4), (P, 4)), ((P, 9), (P + 64, 2), (P + 32, 5)), ((P, 5), (P + 16, 1))):
+        assert "overlap" in refused(L, "znn_clip_grads", *table(*spans), P)
     for bad, word in (((None, 3), "NULL"), ((P + 2, 3), "aligned"), ((P, 1 << 41), "implausible")):
         g, c, n = table((P, 4), bad)
         for name, tail in (("znn_grad_norm", (1.0, 1.0, P)), ("znn_clip_grads", (P,))):

@@ -716,3 +716,88 @@ def test_policy_loss_captured_and_on_two_streams(ops, L, M, N):
     for c in calls:
         for k in range(3):
             c.check(k)
+
+
+@pytest.mark.parametrize("M,N", [(30, 700), (600, 1300), (520, 9001)])
+def test_calls_behind_copies_and_a_join_captured(ops, L, M, N):
+    """A graph whose logits come from a copy on one stream and whose targets come from another stream, joined right before the
+    policy loss, with a norm of the gradient on the second stream behind it: three replays with other inputs."""
+    torch = pytest.importorskip("torch")
+    r = np.random.default_rng(M)
+    up = ops.DevBuf.from_host
+    sets = []
+    for _ in range(3):
+        x, t = logits(r, M, N)
+        sets.append((np.nan_to_num(x, nan=0.0, neginf=-np.inf), t))
+    old, adv = np.full(M, -4, np.float32), r.standard_normal(M).astype(np.float32)
+    want = [ops.policy_loss(x, t, old, adv) for x, t in sets]
+    o, a = up(old), up(adv)
+    x0, t0, x, t = ops.DevBuf(4 * M * N), ops.DevBuf(4 * M), ops.DevBuf(4 * M * N), ops.DevBuf(4 * M)
+    loss, tl, dx, res = ops.DevBuf(8), ops.DevBuf(4 * M), ops.DevBuf(4 * M * N), ops.DevBuf(ops.GRAD_NORM_FLOATS * 4)
+    ptrs, counts = (C.c_void_p * 1)(dx.ptr), (C.c_size_t * 1)(M * N)
+    main, side = torch.cuda.Stream(), torch.cuda.Stream()
+    L.call("znn_sync")
+    g = torch.cuda.CUDAGraph()
+    try:
+        with torch.cuda.graph(g, stream=main, capture_error_mode="thread_local"):
+            side.wait_stream(main)
+            L.call("znn_set_stream", side.cuda_stream)
+            L.call("znn_memcpy_d2d", t.ptr, t0.ptr, 4 * M)
+            L.call("znn_set_stream", main.cuda_stream)
+            L.call("znn_memcpy_d2d", x.ptr, x0.ptr, 4 * M * N)
+            main.wait_stream(side)
+            L.call("znn_policy_loss", x.ptr, N, t.ptr, 1.0, o.ptr, None, a.ptr, None, 0.2, 0.2, 0.0, 0.0, loss.ptr, tl.ptr, None, None, dx.ptr, N, M, N)
+            side.wait_stream(main)
+            L.call("znn_set_stream", side.cuda_stream)
+            L.call("znn_grad_norm", ptrs, counts, 1, 1.0, 0.5, res.ptr)
+            main.wait_stream(side)
+            L.call("znn_set_stream", main.cuda_stream)
+            L.call("znn_clip_grads", ptrs, counts, 1, res.ptr)
+        for (hx, ht), w in zip(sets, want):
+            bx, bt = up(hx), up(ht)
+            L.call("znn_memcpy_d2d", x0.ptr, bx.ptr, 4 * M * N)
+            L.call("znn_memcpy_d2d", t0.ptr, bt.ptr, 4 * M)
+            with torch.cuda.stream(main):
+                g.replay()
+            L.call("znn_sync")
+            got = loss.to_host((2,))
+            assert got[0] == w["loss"] and got[1] == w["rows"]
+            factor = res.to_host((2,))[1]
+            assert 0 < factor <= 1
+            np.testing.assert_array_equal(dx.to_host((M, N)), w["dlogits"] * factor)
+    finally:
+        L.call("znn_set_stream", None)
+
+
+@pytest.mark.parametrize("M,N", [(40, 40001), (24, 131072)])
+def test_policy_gradient_over_the_logits_of_rows_in_parts(ops, L, M, N):
+    """In place where the blocks of a cluster share a row: whichever of them writes first, the others have the target's logit."""
+    r = np.random.default_rng(N)
+    up = ops.DevBuf.from_host
+    x, t = logits(r, M, N)
+    x = np.nan_to_num(x, nan=0.0, neginf=-np.inf)
+    old, adv = np.full(M, -4, np.float32), r.standard_normal(M).astype(np.float32)
+    want = ops.policy_loss(x, t, old, adv)
+    bt, o, a, loss, tl = up(t), up(old), up(adv), ops.DevBuf(8), ops.DevBuf(4 * M)
+    for _ in range(20):
+        b = up(x)
+        L.call("znn_policy_loss", b.ptr, N, bt.ptr, 1.0, o.ptr, None, a.ptr, None, 0.2, 0.2, 0.0, 0.0, loss.ptr, tl.ptr, None, None, b.ptr, N, M, N)
+        assert loss.to_host((2,))[0] == want["loss"]
+        np.testing.assert_array_equal(b.to_host((M, N)), want["dlogits"])
+
+
+def test_tensors_that_overlap_are_not_clipped(ops, L):
+    host = np.arange(64, dtype=np.float32)
+    b, res = ops.DevBuf.from_host(host), ops.DevBuf(ops.GRAD_NORM_FLOATS * 4)
+    twice = (C.c_void_p * 2)(b.ptr, b.ptr + 4 * 31)
+    counts = (C.c_size_t * 2)(32, 33)
+    L.call("znn_grad_norm", twice, counts, 2, 1.0, 1.0, res.ptr)   # a float of both counts twice
+    want = np.sqrt(np.square(host.astype(np.float64)).sum() + 31.0 ** 2)
+    assert abs(float(res.to_host((2,))[0]) - want) <= want * np.finfo(np.float32).eps
+    with pytest.raises(Exception, match="overlap"):
+        L.call("znn_clip_grads", twice, counts, 2, res.ptr)
+    np.testing.assert_array_equal(b.to_host((64,)), host)
+    counts = (C.c_size_t * 2)(31, 33)
+    L.call("znn_clip_grads", twice, counts, 2, res.ptr)
+    factor = res.to_host((2,))[1]
+    np.testing.assert_array_equal(b.to_host((64,)), host * factor)

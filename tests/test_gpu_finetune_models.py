@@ -291,6 +291,7 @@ def test_model_refusals(Model):
     refused(lambda: m.grad_norm(), "max_grad_norm")
     refused(lambda: m.set_option("max_grad_norm", -1.0), "max_grad_norm")
     refused(lambda: m.set_option("max_grad_norm", float("nan")), "max_grad_norm")
+    refused(lambda: m.set_option("max_grad_norm", 1e-60), "max_grad_norm")   # 0 in fp32
 
 
 # ------------------------------------------------------------------ clipping in the training steps

@@ -8,6 +8,9 @@
 #include <math.h>
 
 #include <algorithm>
+#include <new>
+#include <utility>
+#include <vector>
 
 #include "common.cuh"
 
@@ -374,6 +377,19 @@ static int clip_grads(float* const* grads, const size_t* counts, int n, const fl
     return ZNN_OK;
 }
 
+// Whether no float belongs to two of the tensors: clipping would multiply it twice, or lose one of the two.
+static bool apart(const float* const* grads, const size_t* counts, int n)
+{
+    std::vector<std::pair<uintptr_t, uintptr_t>> spans;
+    spans.reserve((size_t)n);
+    for (int i = 0; i < n; i++)
+        if (counts[i]) spans.emplace_back((uintptr_t)grads[i], (uintptr_t)grads[i] + 4 * counts[i]);
+    std::sort(spans.begin(), spans.end());
+    for (size_t i = 1; i < spans.size(); i++)
+        if (spans[i].first < spans[i - 1].second) return false;
+    return true;
+}
+
 static bool quads(const void* a, const void* b, const void* c, const void* d)
 {
     return (((uintptr_t)a | (uintptr_t)b | (uintptr_t)c | (uintptr_t)d) & 15) == 0;
@@ -407,6 +423,11 @@ int znn_clip_grads(float** grads, const size_t* counts, int n, const float* resu
     const int rc = check_set(grads, counts, n, grads);
     if (rc != ZNN_OK) return rc;
     ZNN_REQUIRE(result, "result is NULL");
+    try {
+        ZNN_REQUIRE(apart(grads, counts, n), "two of the tensors overlap");
+    } catch (const std::bad_alloc&) {
+        return fail(ZNN_ERR_NOMEM, "no host memory");
+    }
     ZNN_NEED_DEVICE();
     if (n <= kSmallTable) return clip_grads<kSmallTable>(grads, counts, n, result);
     if (n <= kMiddleTable) return clip_grads<kMiddleTable>(grads, counts, n, result);

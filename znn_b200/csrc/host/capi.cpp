@@ -505,7 +505,7 @@ int znn_model_set_option(znn_model* m, const char* key, double value)
     else if (k == "adam_t") m->adam.t = (float)value;
     else if (k == "momentum") m->opt.momentum = (float)value;
     else if (k == "max_grad_norm") {
-        if (!(value >= 0.0)) throw Error(ZNN_ERR_INVALID, "max_grad_norm: a norm, or 0 to leave gradients as they are");
+        if (!(value >= 0.0) || (value > 0.0 && (float)value == 0.0f)) throw Error(ZNN_ERR_INVALID, "max_grad_norm: a norm, or 0 to leave gradients as they are");
         if (value > 0.0) m->ps.norm_result();   // allocated here, not inside a step that may be under capture
         m->opt.max_norm = m->adam.max_norm = (float)value;
         drop_graph(m);

@@ -117,11 +117,10 @@ __device__ __forceinline__ double log_of_sum(float ties, float s)
     return (double)((bits >> 23) - 127) * 0.693147180559945309417 + (double)logf(__int_as_float((bits & 0x007fffff) | 0x3f800000)) + (total - total);
 }
 
-// Every kernel here may begin while the one before it on the stream still runs, and waits here for that one's end and for what it
-// wrote: the launch itself then costs no time between them.  Only the rows of a policy loss begin without, beside the kernel that
-// counts them, which has waited before it let them begin.
+// Every kernel here may begin while the one before it on the stream ends, and waits here, before it reads or writes anything, for
+// that one's end and for what it wrote: the launch itself then costs no time between them.  (Rows of a policy loss that began
+// beside the kernel that counts them would save 2 us of 90, but nothing would promise that they see what ran before that one.)
 __device__ __forceinline__ void wait_for_previous_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void let_next_kernel_begin() { asm volatile("griddepcontrol.launch_dependents;"); }
 
 struct RowParams {
     const float* logits;
@@ -139,13 +138,6 @@ struct RowParams {
     long long ld_d;
     int* status;
 };
-
-// The kernel that counts the rows runs while this one reads the logits.  One thread of every row waits for it, of rows that are left
-// out too: when this kernel has ended, that one has, for whatever comes next on the stream.
-__device__ __forceinline__ void wait_for_count(const RowParams& p)
-{
-    if (p.count) wait_for_previous_kernel();
-}
 
 // What a row's gradient is made of: dx_j = 2^t * (a + b * t) for j != target, and dx at the target as it is.  t is measured
 // from `mx`.
@@ -201,7 +193,6 @@ __device__ __forceinline__ RowGrad row_scalars(const RowParams& p, int row, cons
     }
     RowGrad g{0.0f, 0.0f, 0.0f, from};
     if (Policy) {
-        wait_for_count(p);
         const float A = in.advantage;
         float loss = 0.0f, slope = 0.0f;
         if (A != 0.0f) {
@@ -255,7 +246,6 @@ template <bool Policy>
 __device__ __forceinline__ void row_unused(const RowParams& p, int row, bool bad)
 {
     const float v = bad ? CUDART_NAN_F : 0.0f;
-    if (Policy) wait_for_count(p);
     if (p.logp) p.logp[row] = v;
     if (p.entropy) p.entropy[row] = 0.0f;
     if (p.stats) {
@@ -428,7 +418,7 @@ __global__ void __launch_bounds__(128) rows_held_kernel(const RowParams p, int)
     const unsigned mask = Group < 32 ? ((1u << (Group & 31)) - 1) << (threadIdx.x & 31 & ~(Group - 1)) : kAllLanes;
     const unsigned row = blockIdx.x * (128 / Group) + threadIdx.x / Group;
     if (row >= (unsigned)p.M) return;
-    if (!Policy || !p.count) wait_for_previous_kernel();
+    wait_for_previous_kernel();
     const float* x = p.logits + (size_t)row * p.ld;
     float* dx = Policy && p.dlogits ? p.dlogits + (size_t)row * p.ld_d : nullptr;
     RowPart<Group, V, Aligned> r;
@@ -518,7 +508,7 @@ __global__ void __launch_bounds__(Threads) rows_walk_kernel(const RowParams p, i
         __syncwarp();
         cluster_arrive();   // waited for when the first walk is done: by then every block runs and has its barrier
     }
-    if (!Policy || !p.count) wait_for_previous_kernel();
+    wait_for_previous_kernel();
     const int row = blockIdx.x / ranks, first = rank * part, n = max(0, min(part, p.N - first));
     const float* x = p.logits + (size_t)row * p.ld + first;
     float* dx = Policy && p.dlogits ? p.dlogits + (size_t)row * p.ld_d + first : nullptr;
@@ -530,7 +520,7 @@ __global__ void __launch_bounds__(Threads) rows_walk_kernel(const RowParams p, i
         return;
     }
     // before any gradient is written: dlogits may be the logits' own buffer
-    const float x_t = tid == 0 ? p.logits[(size_t)row * p.ld + in.t] : 0.0f;
+    float x_t = tid == 0 ? p.logits[(size_t)row * p.ld + in.t] : 0.0f;
 
     RowSums sums{-CUDART_INF_F, 0.0f, 0.0f, 0.0f};
     Part r;
@@ -577,6 +567,7 @@ __global__ void __launch_bounds__(Threads) rows_walk_kernel(const RowParams p, i
         const RowSums none{-CUDART_INF_F, 0.0f, 0.0f, 0.0f};
         sums = join_lanes(tid < kWarps ? sh_warps[tid] : none, p.c);
         if (ranks > 1) {
+            x_t = __shfl_sync(kAllLanes, x_t, 0);   // it has arrived before another block learns that it may write over it
             exchange(&sh_word, sums, ranks, rank, p.status);
             sums = join_lanes(tid < ranks ? sh_word.sums[tid] : none, p.c);
         }
@@ -665,7 +656,6 @@ policy_total_kernel(const int32_t* __restrict__ targets, const float* __restrict
     const int ranks = cluster_size(), rank = cluster_rank();
     if (ranks > 1) cluster_sync_all();   // a block must run before another writes to its memory
     wait_for_previous_kernel();
-    if (!with_sum) let_next_kernel_begin();
     int rows = 0;
     double sum = 0.0;
 #pragma unroll 8
