@@ -5,8 +5,8 @@
 // where there is not.  Measured on a B200 whose copies run at 6548 GB/s, the whole call, inputs in turn from three sets:
 //   log-probabilities and entropies 2045 x 50257, a fifth left out  58 us  5.7 TB/s     (floor 50 us)
 //   their gradient with entropy term 8192 x 8192, a tenth left out  79 us  6.4 TB/s     (78 us)
-//   policy loss 8192 x 8192, KL term                                92 us  5.8 TB/s     (82 us)
-//   policy loss 2048 x 131000, KL and entropy, 0.15 left out       342 us  5.8 TB/s     (303 us)
+//   policy loss 8192 x 8192, KL term                                94 us  5.7 TB/s     (82 us)
+//   policy loss 2048 x 131000, KL and entropy, 0.15 left out       345 us  5.8 TB/s     (303 us)
 //   preference loss 700 pairs, 1.4 million rows                     12 us               (3.4 us: latency)
 #include <math.h>
 #include <math_constants.h>
@@ -487,9 +487,9 @@ __global__ void __launch_bounds__(128) rows_held_kernel(const RowParams p, int)
 // 0.94 GB read, 1.02 GB written, 343 us).  Small blocks with few registers are what makes it fast: a row's chain of loads,
 // reductions and scalars takes microseconds, and enough other rows must be under way meanwhile.  Rows held in registers, by blocks
 // of 256 or 512 threads and clusters of them, took 580 us for the same, since too few blocks per SM hid too little of that chain
-// (copying the next row to shared memory ahead made it worse: 8192 x 8192 110 -> 138 us, where this form takes 92).
+// (copying the next row to shared memory ahead made it worse: 8192 x 8192 110 -> 138 us, where this form takes 94).
 // Rows of some 30 to 60 thousand columns lie between one block a row and small parts, and their second pass misses L2 most often:
-// 2000 x 50256 154 us (floor 123); 161 without the second pass's loads marked as the last, and 173 against 158 for 50257.
+// 2000 x 50256 156 us (floor 123); 5 % more without the second pass's loads marked as the last, 9 % for 50257 columns.
 template <bool Policy, bool Entropy, bool Aligned, int Threads, int kQuads>
 __global__ void __launch_bounds__(Threads) rows_walk_kernel(const RowParams p, int part)
 {
@@ -701,7 +701,8 @@ __device__ __forceinline__ PairTerms pair_terms(double m, double eps, int P)
 
 // A block (or a cluster of blocks, for long sequences) per pair: the two sums, the pair's loss, the gradient of its rows.
 // Small: one block has every pair, a warp each, and the mean as well.  The gradient is the same for all rows of a sequence, so the
-// second walk reads nothing but which rows are left out.  Bound by HBM where there is enough: 12 to 16 bytes per row.
+// second walk reads nothing but which rows are left out.  Bound by HBM where there is enough: 12 to 16 bytes per row; 700 pairs of
+// 2000 rows are a chain of loads, two sums, an exponential and a logarithm in fp64, and the mean's launch: 11.6 us (floor 3.4).
 template <bool Small, int Threads>
 __global__ void __launch_bounds__(Threads)
 preference_pair_kernel(const float* __restrict__ logp, const float* __restrict__ ref_logp, const int32_t* __restrict__ targets,
@@ -750,23 +751,25 @@ preference_pair_kernel(const float* __restrict__ logp, const float* __restrict__
             }
         }
     }
-    sums[2] = rows[0];
-    sums[3] = rows[1];
+    sums[2] = __reduce_add_sync(kAllLanes, rows[0]);
+    sums[3] = __reduce_add_sync(kAllLanes, rows[1]);
 #pragma unroll
-    for (int k = 0; k < 4; k++)
+    for (int l = 16; l > 0; l >>= 1)
 #pragma unroll
-        for (int l = 16; l > 0; l >>= 1) sums[k] += __shfl_xor_sync(kAllLanes, sums[k], l);
+        for (int k = 0; k < 2; k++) sums[k] += __shfl_xor_sync(kAllLanes, sums[k], l);
     if (!Small) {
         if ((tid & 31) == 0)
             for (int k = 0; k < 4; k++) sh[tid >> 5][k] = sums[k];
         __syncthreads();
         if (tid < 32) {
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-                sums[k] = tid < Threads / 32 ? sh[tid][k] : 0.0;
+            for (int k = 0; k < 4; k++) sums[k] = tid < Threads / 32 ? sh[tid][k] : 0.0;
+            sums[2] = __reduce_add_sync(kAllLanes, (int)sums[2]);
+            sums[3] = __reduce_add_sync(kAllLanes, (int)sums[3]);
 #pragma unroll
-                for (int l = 16; l > 0; l >>= 1) sums[k] += __shfl_xor_sync(kAllLanes, sums[k], l);
-            }
+            for (int l = Threads / 64; l > 0; l >>= 1)
+#pragma unroll
+                for (int k = 0; k < 2; k++) sums[k] += __shfl_xor_sync(kAllLanes, sums[k], l);
         }
         if (ranks > 1) {
             if (tid < ranks)
