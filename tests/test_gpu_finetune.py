@@ -801,3 +801,46 @@ def test_tensors_that_overlap_are_not_clipped(ops, L):
     L.call("znn_clip_grads", twice, counts, 2, res.ptr)
     factor = res.to_host((2,))[1]
     np.testing.assert_array_equal(b.to_host((64,)), host * factor)
+
+
+@pytest.mark.parametrize("N", [1, 3, 31, 32, 33, 64, 65, 127, 128, 129, 256, 257, 511, 512, 513, 1023, 1024])
+@pytest.mark.parametrize("M,pad,shift,ce", [(1, 0, 0, 0.0), (3, 0, 0, 0.1), (131, 0, 0, 0.0), (130, 3, 1, 0.1), (67, 4, 0, 0.0)])
+def test_short_rows_together_and_alone(ops, L, N, M, pad, shift, ce):
+    """A short row gives the same bits among others as alone (where groups of lanes take several rows), beside rows that are left out and
+    hold NaN and rows with a bad target, in place, and floats between the rows and behind the last one stay."""
+    r = np.random.default_rng(N * 7 + M)
+    x, t = logits(r, M, N, left=0.3)
+    t[r.random(M) < 0.05] = N
+    x[t < 0] = np.nan
+    ld = N + pad
+    old, adv = np.full(M, -3, np.float32), r.standard_normal(M).astype(np.float32)
+    w = r.random(M).astype(np.float32) + 0.5
+    w[r.random(M) < 0.1] = 0
+    buf = np.full(shift + M * ld + 64, 77.0, np.float32)
+    for i in range(M):
+        buf[shift + i * ld:shift + i * ld + N] = x[i]
+    up = ops.DevBuf.from_host
+    tb, ob, ab, wb = up(t), up(old), up(adv), up(w)
+    loss, tl, lp, en = ops.DevBuf(8), up(np.full(M + 8, 5, np.float32)), up(np.full(M + 8, 5, np.float32)), up(np.full(M + 8, 5, np.float32))
+
+    def run(b, first, rows):
+        at = b.ptr + 4 * (shift + first * ld)
+        L.call("znn_policy_loss", at, ld, tb.ptr + 4 * first, 1.0, ob.ptr + 4 * first, None, ab.ptr + 4 * first, wb.ptr + 4 * first, 0.2, 0.2, 0.0, ce,
+               loss.ptr, tl.ptr + 4 * first, lp.ptr + 4 * first, en.ptr + 4 * first, at, ld, rows, N)
+    together, alone = up(buf), up(buf)
+    run(together, 0, M)
+    a = [together.to_host(buf.shape)] + [v.to_host((M + 8,)) for v in (tl, lp, en)]
+    for i in range(M):
+        run(alone, i, 1)
+    b = [alone.to_host(buf.shape)] + [v.to_host((M + 8,)) for v in (tl, lp, en)]
+    for p, q in zip(a, b):
+        np.testing.assert_array_equal(p, q)
+    rest = a[0].copy()
+    for i in range(M):
+        row = rest[shift + i * ld:shift + i * ld + N]
+        assert np.all(np.isfinite(row)) and (0 <= t[i] < N and w[i] != 0 or np.all(row == 0.0))
+        row[:] = 77.0
+    assert np.all(rest == 77.0) and all(np.all(v[M:] == 5.0) for v in a[1:])
+    want = ft.policy(np.where((t < 0)[:, None], 0.0, x), t, old, adv, weights=w, ce=ce)
+    within(a[2][:M], want["logp"], 4 * (row_k(np.where((t >= 0)[:, None], np.nan_to_num(x, nan=0.0, neginf=0.0), 0.0), 1.0) + np.abs(np.nan_to_num(want["logp"]))) * U, "logp")
+    status(L)

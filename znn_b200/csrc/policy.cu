@@ -407,79 +407,95 @@ __device__ __forceinline__ void exchange(RowWord* word, const RowSums& mine, int
     __syncwarp();
 }
 
-// Short rows: 8 lanes or a warp hold a whole row in registers from its load to the gradient's store.  The maximum comes first, so
-// that every exponential is taken once, relative to it.  Log-probabilities 65536 x 1000: 40 us, 6.5 TB/s; policy loss with KL term
-// 100 us, 5.3 TB/s: the row's scalars and reductions show, and are most of the work below a few hundred columns (1000000 x 100:
-// 369 us, 2.3 TB/s).
-template <bool Policy, bool Entropy, bool Aligned, int Group, int V>
+// Short rows: 8 lanes or a warp hold whole rows in registers from their load to the gradient's store, Rows of them at a time: lane k
+// makes the scalars of the k-th, since those few hundred operations cost the same for one lane as for all.  The maximum comes first,
+// so that every exponential is taken once, relative to it.  A row that is left out is one of nothing but -inf: its gradient is 0.
+// Log-probabilities 65536 x 1000: 40 us, 6.5 TB/s, 65536 x 100: 6.9 us, 3.9 TB/s; policy loss with KL term 65536 x 1000: 95 us,
+// 5.5 TB/s, 1000000 x 100: 283 us, 2.9 TB/s (369 with one row at a time): the rows' scalars and reductions show, the more the shorter
+// the rows are.
+template <bool Policy, bool Entropy, bool Aligned, int Group, int V, int Rows>
 __global__ void __launch_bounds__(128) rows_held_kernel(const RowParams p, int)
 {
+    static_assert(Rows <= Group, "a lane makes the scalars of one row");
     const int tid = threadIdx.x % Group;
     const unsigned mask = Group < 32 ? ((1u << (Group & 31)) - 1) << (threadIdx.x & 31 & ~(Group - 1)) : kAllLanes;
-    const unsigned row = blockIdx.x * (128 / Group) + threadIdx.x / Group;
-    if (row >= (unsigned)p.M) return;
+    const unsigned row0 = (blockIdx.x * (128 / Group) + threadIdx.x / Group) * Rows, mine = row0 + tid;
+    if (row0 >= (unsigned)p.M) return;
     wait_for_previous_kernel();
-    const float* x = p.logits + (size_t)row * p.ld;
-    float* dx = Policy && p.dlogits ? p.dlogits + (size_t)row * p.ld_d : nullptr;
-    RowPart<Group, V, Aligned> r;
-    r.place(x, p.N);
-    const RowHead in = row_head<Policy>(p, row, tid == 0);
-    if (!in.used(p.N)) {
-        if (tid == 0) row_unused<Policy>(p, row, in.t >= p.N && in.w != 0.0f);
-        if (dx) r.clear(dx, p.N, tid);
-        return;
+    const bool there = tid < Rows && mine < (unsigned)p.M;
+    const RowHead in = row_head<Policy>(p, there ? mine : 0xffffffffu, true);
+    const bool used = in.used(p.N);
+    const float* x = p.logits + (size_t)row0 * p.ld;
+    RowPart<Group, V, Aligned> r[Rows];
+    int t[Rows];
+#pragma unroll
+    for (int k = 0; k < Rows; k++) {
+        t[k] = __shfl_sync(mask, used ? in.t : -1, k, Group);
+        r[k].place(x + k * p.ld, t[k] >= 0 ? p.N : 0);
+        r[k].load(x + k * p.ld, tid);
     }
-    r.load(x, tid);
-    const float x_t = tid == 0 ? x[in.t] : 0.0f;   // before a gradient is written over it
+    const float x_t = used ? p.logits[(size_t)mine * p.ld + in.t] : 0.0f;   // before a gradient is written over it
     const int rows = Policy && !p.weights && !p.count ? __reduce_add_sync(mask, count_rows<Group>(p, tid)) : 0;
-    float top = r.extra;
+    RowSums own{};
 #pragma unroll
-    for (int k = 0; k < V; k++) top = fmaxf(fmaxf(top, fmaxf(r.v[k][0], r.v[k][1])), fmaxf(r.v[k][2], r.v[k][3]));
-    RowSums sums{warp_max<Group>(top, mask), 0.0f, 0.0f, 0.0f};
-    const float base = base_of(sums.mx);
-    // with an entropy term t is clamped (0 * -inf is to be 0), and kept for the gradient, which takes 2^t again
-    auto take = [&](float& x) {
-        const float t2 = (x - base) * p.c, te = Entropy ? max_nan(t2, kNothing) : t2, e = exp2_fast(te);
-        sums.s += e;
-        if (Entropy) sums.u += te * e;
-        x = Entropy ? te : e;
-    };
+    for (int k = 0; k < Rows; k++) {
+        float top = r[k].extra;
 #pragma unroll
-    for (int k = 0; k < V; k++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) take(r.v[k][i]);
-    if (!Aligned) take(r.extra);
-    if (top == base) {   // the few threads that hold the largest logit tell its ones from the rest
-        const float with_ones = sums.s;
-        sums.s = 0.0f;
-        auto add = [&](float x) {
-            const float e = Entropy ? exp2_again(x) : x;
-            if (!(e == 1.0f)) sums.s += e;
+        for (int q = 0; q < V; q++) top = fmaxf(fmaxf(top, fmaxf(r[k].v[q][0], r[k].v[q][1])), fmaxf(r[k].v[q][2], r[k].v[q][3]));
+        RowSums sums{warp_max<Group>(top, mask), 0.0f, 0.0f, 0.0f};
+        const float base = base_of(sums.mx);
+        // with an entropy term t is clamped (0 * -inf is to be 0), and kept for the gradient, which takes 2^t again
+        auto take = [&](float& x) {
+            const float t2 = (x - base) * p.c, te = Entropy ? max_nan(t2, kNothing) : t2, e = exp2_fast(te);
+            sums.s += e;
+            if (Entropy) sums.u += te * e;
+            x = Entropy ? te : e;
         };
 #pragma unroll
-        for (int k = 0; k < V; k++)
+        for (int q = 0; q < V; q++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) add(r.v[k][i]);
-        if (!Aligned) add(r.extra);
-        sums.ties = rintf(with_ones - sums.s);
+            for (int i = 0; i < 4; i++) take(r[k].v[q][i]);
+        if (!Aligned) take(r[k].extra);
+        if (top == base) {   // the few threads that hold the largest logit tell its ones from the rest
+            const float with_ones = sums.s;
+            sums.s = 0.0f;
+            auto add = [&](float x) {
+                const float e = Entropy ? exp2_again(x) : x;
+                if (!(e == 1.0f)) sums.s += e;
+            };
+#pragma unroll
+            for (int q = 0; q < V; q++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) add(r[k].v[q][i]);
+            if (!Aligned) add(r[k].extra);
+            sums.ties = rintf(with_ones - sums.s);
+        }
+        sums.ties = warp_sum<Group>(sums.ties, mask);
+        sums.s = warp_sum<Group>(sums.s, mask);
+        if (Entropy) sums.u = warp_sum<Group>(sums.u, mask);
+        if (tid == k) own = sums;
     }
-    sums.ties = warp_sum<Group>(sums.ties, mask);
-    sums.s = warp_sum<Group>(sums.s, mask);
-    if (Entropy) sums.u = warp_sum<Group>(sums.u, mask);
     RowGrad g{};
-    if (tid == 0) g = row_scalars<Policy, Entropy>(p, row, sums, in, x_t, rows, true, sums.mx);
-    if (!dx) return;
-    g.a = __shfl_sync(mask, g.a, 0, Group);
-    g.b = __shfl_sync(mask, g.b, 0, Group);
-    g.at_target = __shfl_sync(mask, g.at_target, 0, Group);
-    auto slope = [&](float& x) { x = Entropy ? exp2_again(x) * (g.a + g.b * x) : x * g.a; };
+    if (there) {
+        if (used) g = row_scalars<Policy, Entropy>(p, mine, own, in, x_t, rows, true, own.mx);
+        else row_unused<Policy>(p, mine, in.t >= p.N && in.w != 0.0f);
+    }
+    if (!Policy || !p.dlogits) return;
+    float* dx = p.dlogits + (size_t)row0 * p.ld_d;
 #pragma unroll
-    for (int k = 0; k < V; k++)
+    for (int k = 0; k < Rows; k++) {
+        const float a = __shfl_sync(mask, g.a, k, Group), b = Entropy ? __shfl_sync(mask, g.b, k, Group) : 0.0f;
+        const float at_target = __shfl_sync(mask, g.at_target, k, Group);
+        auto slope = [&](float& x) { x = Entropy ? exp2_again(x) * (a + b * x) : x * a; };
 #pragma unroll
-        for (int i = 0; i < 4; i++) slope(r.v[k][i]);
-    if (!Aligned) slope(r.extra);
-    r.store(dx, tid);
-    if (r.owns(in.t, tid)) dx[in.t] = g.at_target;
+        for (int q = 0; q < V; q++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) slope(r[k].v[q][i]);
+        if (!Aligned) slope(r[k].extra);
+        r[k].place(x + k * p.ld, row0 + k < (unsigned)p.M ? p.N : 0);
+        r[k].store(dx + k * p.ld_d, tid);
+        if (r[k].owns(t[k], tid)) dx[k * p.ld_d + t[k]] = at_target;
+    }
 }
 
 // Longer rows: a block (or the blocks of a cluster, which take `part` columns each) walks over the row with running sums per thread,
@@ -875,11 +891,11 @@ static int launch(void (*kernel)(Params...), const char* name, long long blocks,
     return ZNN_OK;
 }
 
-template <bool Policy, bool Entropy, bool Aligned, int Group, int V>
+template <bool Policy, bool Entropy, bool Aligned, int Group, int V, int Rows>
 static int launch_held(const RowParams& p)
 {
-    constexpr int rows = 128 / Group;
-    return launch(rows_held_kernel<Policy, Entropy, Aligned, Group, V>, "rows_held_kernel", (p.M + (long long)rows - 1) / rows, 128, 1,
+    constexpr int rows = 128 / Group * Rows;
+    return launch(rows_held_kernel<Policy, Entropy, Aligned, Group, V, Rows>, "rows_held_kernel", (p.M + (long long)rows - 1) / rows, 128, 1,
                   p, 0);
 }
 
@@ -891,9 +907,11 @@ static int launch_walk(const RowParams& p, int ranks)
                   p, part);
 }
 
-// Which kernel: 8 lanes per row up to 256 columns, a warp up to 1024, then blocks that walk.  A block costs the same few
-// reductions whatever its size, so the smallest one that a few steps suffice wins; the policy loss, which walks twice, wants its
-// rows in flight to stay in L2 between the walks and so spreads long rows over clusters.  Measured (us, 32 / 64 / 128 / 256 threads):
+// Which kernel: 8 lanes per row up to 256 columns, a warp up to 1024, then blocks that walk.  Rows held at a time (us, 1 / 2 / 4, policy
+// loss of 65536 rows): 30 columns 22.3 / - / 19.0 (8: 21.7), 50 24.4 / 22.2 / 23.8, 100 29.0 / 27.6 / 30.3, 200 36.2 / 41.4 / -,
+// 400 59.1 / 53.2 / 53.4, 1000 95 / 95 / -.  A walking block costs the same few reductions whatever its size, so the smallest one that
+// a few steps suffice wins; the policy loss, which walks twice, wants its rows in flight to stay in L2 between the walks and so
+// spreads long rows over clusters.  Measured (us, 32 / 64 / 128 / 256 threads):
 //   policy   40000 x 2000: 111 / 125 / 183 / 339,  20000 x 4096: 133 / 114 / 120 / 185,  10000 x 8192: - / 135 / 112 / 124,
 //            4000 x 20000: - / - / 140 / 120;  256 threads in clusters of 1 / 2 / 4 / 8: 2500 x 32000: 133 / 117 / 139 / -,
 //            1500 x 65536: 180 / 162 / 143 / 165,  700 x 131072: - / - / 152 / 136
@@ -903,9 +921,12 @@ static int launch_walk(const RowParams& p, int ranks)
 template <bool Policy, bool Entropy, bool Aligned>
 static int launch_rows_as(const RowParams& p)
 {
-    if (p.N <= 64) return launch_held<Policy, Entropy, Aligned, 8, 2>(p);
-    if (p.N <= 256) return launch_held<Policy, Entropy, Aligned, 8, 8>(p);
-    if (p.N <= 1024) return launch_held<Policy, Entropy, Aligned, 32, 8>(p);
+    if (p.N <= 32) return launch_held<Policy, Entropy, Aligned, 8, 1, 4>(p);
+    if (p.N <= 64) return launch_held<Policy, Entropy, Aligned, 8, 2, 2>(p);
+    if (p.N <= 128) return launch_held<Policy, Entropy, Aligned, 8, 4, 2>(p);
+    if (p.N <= 256) return launch_held<Policy, Entropy, Aligned, 8, 8, 1>(p);
+    if (p.N <= 512) return launch_held<Policy, Entropy, Aligned, 32, 4, 2>(p);
+    if (p.N <= 1024) return launch_held<Policy, Entropy, Aligned, 32, 8, 1>(p);
     if (p.M < 2 * sm_count() && p.N > 2048) {
         int ranks = Policy && p.N > 102400 ? 8 : 1;
         while (ranks < 8 && p.N > 8192 * ranks && (long long)p.M * ranks < 2 * sm_count()) ranks *= 2;
