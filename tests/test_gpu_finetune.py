@@ -844,3 +844,14 @@ def test_short_rows_together_and_alone(ops, L, N, M, pad, shift, ce):
     want = ft.policy(np.where((t < 0)[:, None], 0.0, x), t, old, adv, weights=w, ce=ce)
     within(a[2][:M], want["logp"], 4 * (row_k(np.where((t >= 0)[:, None], np.nan_to_num(x, nan=0.0, neginf=0.0), 0.0), 1.0) + np.abs(np.nan_to_num(want["logp"]))) * U, "logp")
     status(L)
+
+
+@pytest.mark.parametrize("M,N", [(300, 1100), (520, 1501), (300, 2000), (301, 2100), (300, 2816), (300, 2900), (520, 4100), (300, 4999), (300, 5121), (297, 6000),
+                                 (300, 8191), (300, 9001), (520, 12288), (300, 12500), (300, 26000), (296, 51300)])
+def test_many_rows_of_every_length(ops, M, N):
+    """As many rows as take the kernels for large calls: every block size and number of quads that a length asks for."""
+    test_token_logprob(ops, M, N, 0.7)
+    test_token_logprob_grad(ops, M, N, True, M % 2 == 0)
+    test_token_logprob_grad(ops, M, N, False, M % 2 == 1)
+    test_policy_loss(ops, M, N, 0.1, 0.02, True, 0.7)
+    test_policy_loss(ops, M, N, 0.05, 0.0, False, 1.25)

@@ -903,6 +903,13 @@ template <bool Policy, bool Entropy, bool Aligned, int Threads>
 static int launch_walk(const RowParams& p, int ranks)
 {
     const int part = (ceil_div(p.N, ranks) + 3) & ~3;   // parts start where the row's quads do
+    if constexpr (Threads < 256) {
+        // rows of a few steps: six quads a thread where those cover fewer columns that are not there (policy 60000 x 2100: 177 us with
+        // six, 184 with eight; 60000 x 2000: 172 and 161; log-probabilities 65536 x 1100: 66 and 74)
+        if (part <= 12288 && 6 * ceil_div(part, 24 * Threads) < 8 * ceil_div(part, 32 * Threads))
+            return launch(rows_walk_kernel<Policy, Entropy, Aligned, Threads, 6>, "rows_walk_kernel", (long long)p.M * ranks, Threads, ranks,
+                          p, part);
+    }
     return launch(rows_walk_kernel<Policy, Entropy, Aligned, Threads, 8>, "rows_walk_kernel", (long long)p.M * ranks, Threads, ranks,
                   p, part);
 }
@@ -912,10 +919,10 @@ static int launch_walk(const RowParams& p, int ranks)
 // 400 59.1 / 53.2 / 53.4, 1000 95 / 95 / -.  A walking block costs the same few reductions whatever its size, so the smallest one that
 // a few steps suffice wins; the policy loss, which walks twice, wants its rows in flight to stay in L2 between the walks and so
 // spreads long rows over clusters.  Measured (us, 32 / 64 / 128 / 256 threads):
-//   policy   40000 x 2000: 111 / 125 / 183 / 339,  20000 x 4096: 133 / 114 / 120 / 185,  10000 x 8192: - / 135 / 112 / 124,
+//   policy   40000 x 2000: 111 / 125 / 183 / 339,  40000 x 2600: 145 / 156 / - / -,  20000 x 4096: 133 / 114 / 120 / 185,  10000 x 8192: - / 135 / 112 / 124,
 //            4000 x 20000: - / - / 140 / 120;  256 threads in clusters of 1 / 2 / 4 / 8: 2500 x 32000: 133 / 117 / 139 / -,
 //            1500 x 65536: 180 / 162 / 143 / 165,  700 x 131072: - / - / 152 / 136
-//   logprob  40000 x 2000: 54 / 66 / 105 / 220,  20000 x 4099: 54 / 55 / 58 / 117,  4000 x 20000: - / 59 / 54 / 59,
+//   logprob  40000 x 2000: 54 / 66 / 105 / 220,  20000 x 4099: 54 / 55 / 58 / 117,  20000 x 5000: 62 / 67 / - / -,  4000 x 20000: - / 59 / 54 / 59,
 //            1000 x 100000: - / - / 66 / 67,  2045 x 50257 (1.7 times the blocks of 128 threads that are resident at once): - / 57 / 60 / 58
 // Few rows are spread over clusters whatever they cost: 32 x 131072 takes 7.4 us with eight blocks per row, 8.7 with four.
 template <bool Policy, bool Entropy, bool Aligned>
@@ -932,7 +939,7 @@ static int launch_rows_as(const RowParams& p)
         while (ranks < 8 && p.N > 8192 * ranks && (long long)p.M * ranks < 2 * sm_count()) ranks *= 2;
         return launch_walk<Policy, Entropy, Aligned, 256>(p, ranks);
     }
-    if (p.N <= (Policy ? 2048 : 4096)) return launch_walk<Policy, Entropy, Aligned, 32>(p, 1);
+    if (p.N <= (Policy ? 2816 : 5120)) return launch_walk<Policy, Entropy, Aligned, 32>(p, 1);
     if (p.N <= (Policy ? 5120 : 8192)) return launch_walk<Policy, Entropy, Aligned, 64>(p, 1);
     if constexpr (!Policy) {
         // long rows: where the blocks of a size smaller or larger are all resident at once, that size (an SM has 1024 threads of them)
@@ -978,14 +985,17 @@ static int launch_bwd(const BwdArgs& b)
                   b.logits, b.ld, b.targets, b.it, b.stats, b.entropy, b.dlogp, b.dentropy, b.dlogits, b.ld_d, b.M, b.N, parts, part);
 }
 
+// Pieces of a row for 8 lanes, a warp or a block: a piece must be nearly full and its loads all under way at once; those of a gradient
+// that is added to are as many again.  Measured (us, stored / added to, 65536 rows: 200 columns by 8 lanes 20.3 / 26.6, by a warp 27.0 / 34.3,
+// 400 37.0 / 47.8 and 35.9 / 46.4, 1100 by warps with 4 quads 95.9 / 124, with 8 93.1 / 140, by blocks 121 / 174; 30000 x 4101: 163 / 229,
+// 149 / 245, 191 / 289; 20000 x 6200 with 4 quads 149, with 8 145, by blocks 154; 4000 x 32003: 160 / 215, 149 / 216, 150 / 210).
 template <bool Accumulate, bool Aligned>
 static int launch_bwd_as(const BwdArgs& b)
 {
     if (b.N <= 64) return launch_bwd<Accumulate, Aligned, 8, 2>(b);
-    if (b.N <= 128) return launch_bwd<Accumulate, Aligned, 8, 4>(b);
+    if (b.N <= 384) return launch_bwd<Accumulate, Aligned, 8, 4>(b);
     if (b.N <= 512) return launch_bwd<Accumulate, Aligned, 32, 4>(b);
-    if (b.N <= 1024) return launch_bwd<Accumulate, Aligned, 32, 8>(b);
-    if (b.N <= 2048) return launch_bwd<Accumulate, Aligned, 256, 2>(b);
+    if (b.N < 8192) return launch_bwd<Accumulate, Aligned, 32, Accumulate ? 4 : 8>(b);
     return launch_bwd<Accumulate, Aligned, 256, 4>(b);
 }
 
