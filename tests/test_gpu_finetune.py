@@ -846,8 +846,8 @@ def test_short_rows_together_and_alone(ops, L, N, M, pad, shift, ce):
     status(L)
 
 
-@pytest.mark.parametrize("M,N", [(300, 1100), (520, 1501), (300, 2000), (301, 2100), (300, 2816), (300, 2900), (520, 4100), (300, 4999), (300, 5121), (297, 6000),
-                                 (300, 8191), (300, 9001), (520, 12288), (300, 12500), (300, 26000), (296, 51300)])
+@pytest.mark.parametrize("M,N", [(450, 1100), (520, 1501), (450, 2000), (451, 2100), (450, 2816), (300, 2900), (450, 2900), (520, 4100), (450, 4999), (450, 5121),
+                                 (447, 6000), (450, 8191), (300, 9001), (450, 9001), (520, 12288), (450, 12500), (446, 26000), (300, 51300), (450, 51300)])
 def test_many_rows_of_every_length(ops, M, N):
     """As many rows as take the kernels for large calls: every block size and number of quads that a length asks for."""
     test_token_logprob(ops, M, N, 0.7)

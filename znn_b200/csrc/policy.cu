@@ -924,7 +924,8 @@ static int launch_walk(const RowParams& p, int ranks)
 //            1500 x 65536: 180 / 162 / 143 / 165,  700 x 131072: - / - / 152 / 136
 //   logprob  40000 x 2000: 54 / 66 / 105 / 220,  20000 x 4099: 54 / 55 / 58 / 117,  20000 x 5000: 62 / 67 / - / -,  4000 x 20000: - / 59 / 54 / 59,
 //            1000 x 100000: - / - / 66 / 67,  2045 x 50257 (1.7 times the blocks of 128 threads that are resident at once): - / 57 / 60 / 58
-// Few rows are spread over clusters whatever they cost: 32 x 131072 takes 7.4 us with eight blocks per row, 8.7 with four.
+// Few rows are spread over clusters, as many as let all blocks run at once: 32 x 131072 takes 7.4 us with eight blocks per row, 8.7
+// with four; policy 100 x 130000 31.4 and 27.5, 320 x 130000 73 and 77, 320 x 32000 27.3 with two and 24.2 with one.
 template <bool Policy, bool Entropy, bool Aligned>
 static int launch_rows_as(const RowParams& p)
 {
@@ -934,8 +935,8 @@ static int launch_rows_as(const RowParams& p)
     if (p.N <= 256) return launch_held<Policy, Entropy, Aligned, 8, 8, 1>(p);
     if (p.N <= 512) return launch_held<Policy, Entropy, Aligned, 32, 4, 2>(p);
     if (p.N <= 1024) return launch_held<Policy, Entropy, Aligned, 32, 8, 1>(p);
-    if (p.M < 2 * sm_count() && p.N > 2048) {
-        int ranks = Policy && p.N > 102400 ? 8 : 1;
+    if (p.M < (Policy ? 3 : 2) * sm_count() && p.N > 2048) {
+        int ranks = Policy && p.N > 102400 && p.M >= sm_count() ? 8 : 1;
         while (ranks < 8 && p.N > 8192 * ranks && (long long)p.M * ranks < 2 * sm_count()) ranks *= 2;
         return launch_walk<Policy, Entropy, Aligned, 256>(p, ranks);
     }
