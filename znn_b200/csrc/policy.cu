@@ -172,7 +172,8 @@ __device__ __forceinline__ RowHead row_head(const RowParams& p, unsigned row, bo
 // The scalars of one row from its sums (one thread): writes logp, entropy, stats, token_loss (where `write`), returns the
 // gradient's coefficients for a walk over logits measured from `from`.  The log-probability, and the differences that ratio and
 // KL term are made of, are fp64: fp32 would leave a ratio of two probabilities of e^-10 an error of 1e-6.  What follows from
-// them are products, which fp32 keeps.  (In short rows these few hundred operations of one lane are most of the work.)
+// them is fp32: products, and the KL term, which is kept from cancelling.  (In short rows these few hundred operations of one lane are
+// most of the work.)
 template <bool Policy, bool Entropy>
 __device__ __forceinline__ RowGrad row_scalars(const RowParams& p, int row, const RowSums& r, const RowHead& in, float x_t, int rows,
                                                bool write, float from)
@@ -205,9 +206,10 @@ __device__ __forceinline__ RowGrad row_scalars(const RowParams& p, int row, cons
         }
         if (p.kl_coef != 0.0f) {
             const float q = (float)((double)in.ref_logp - logp), e = expm1f(q);
-            // e - q loses what e and q share: for a small q the first terms of its series, q^2/2 + q^3/6 + q^4/24 + q^5/120 (the next
-            // is below 1e-8 of the first for |q| < 1/32)
-            const float rest = fabsf(q) < 0.03125f ? q * q * (0.5f + q * (1.0f / 6.0f + q * (1.0f / 24.0f + q * (1.0f / 120.0f)))) : e - q;
+            // e - q loses what e and q share: 63 halves of a step just above 1/32, 7 at 1/4.  Below 1/2 the term comes from its series
+            // q^2 (1/2! + q/3! + ... + q^7/9!), whose next member is below 2e-9 of it: 3 halves, as many as e - q has from 1/2 on.
+            const float series = 0.5f + q * (1.0f / 6 + q * (1.0f / 24 + q * (1.0f / 120 + q * (1.0f / 720 + q * (1.0f / 5040 + q * (1.0f / 40320 + q * (1.0f / 362880)))))));
+            const float rest = fabsf(q) < 0.5f ? q * q * series : e - q;
             loss += p.kl_coef * rest;
             slope -= p.kl_coef * e;
         }
