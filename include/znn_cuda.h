@@ -267,8 +267,9 @@ int znn_softmax_xent_fwd_static(const float* logits, const int32_t* targets, flo
  *   - targets[i] < 0 leaves the row out (prompt, padding): its logits and its entries of the other inputs are not used
  *     (they may hold NaN), its outputs are 0 and it gets no gradient.  targets[i] >= N is never used as an index: the
  *     row's logp (and a loss it is part of) becomes NaN, it gets no gradient and ZNN_DEV_BAD_INDEX is set;
- *   - a logit of -inf switches its column off (p_j = 0, gradient 0).  A row of -inf alone has logp = -inf, entropy 0 and
- *     gradient 0; a row that holds NaN or +inf gives NaN;
+ *   - a logit of -inf switches its column off: p_j = 0, gradient 0, except that a target that is switched off (logp = -inf) still has
+ *     the gradient of a p_t of 0.  A row of -inf alone has logp = -inf, entropy 0 and gradient 0; a row that holds NaN or +inf
+ *     gives NaN;
  *   - sums of a row are kept in fp32 per thread and joined in a fixed order, per-row scalars and sums over rows in fp64:
  *     results do not depend on timing.  Nothing is kept in the library between calls.
  *
@@ -286,7 +287,9 @@ int znn_token_logprob_bwd(const float* logits, long long ld, const int32_t* targ
 /* Clipped policy loss with a KL term and an entropy bonus, and its gradient, in one pass over the logits.  Per row
  *   r = exp(logp - old_logp),  q = ref_logp - logp,
  *   l = -min(r * A, clip(r, 1 - clip_low, 1 + clip_high) * A) + kl_coef * (exp(q) - q - 1) - entropy_coef * entropy
- * with A = advantages[i] (A = 0: the first term and its gradient are 0 whatever r is).  On a border r counts as inside.
+ * with A = advantages[i] (A = 0: the first term and its gradient are 0 whatever r is).  On a border r counts as inside.  A row whose
+ * loss is beyond fp32 (logp = -inf with a KL term; r with A < 0, or exp(q), above 3e38) has l = +inf and gradients of +-inf where
+ * p_j > 0 (the target's of the opposite sign), 0 where p_j = 0.  Two infinite log-probabilities have no ratio: NaN.
  *   loss[0] = sum_i w_i l_i,  w_i = weights[i], or 1 / (number of rows not left out) where weights is NULL (0 when there is
  *   none); a row of weight 0 is left out.  loss[1] = the number of rows not left out.
  * token_loss[M] = l; logp[M] and entropy[M] (either may be NULL) as above; dlogits = d loss[0] / d logits, stored, NULL = the

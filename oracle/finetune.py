@@ -38,7 +38,7 @@ def rows_grad(x, targets, dlogp, dentropy, inv_temp=1.0):
         hot[targets[i]] = 1.0
         with np.errstate(invalid="ignore"):
             inner = np.where(p[i] > 0, p[i] * (lp[i] + ent[i]), 0.0)
-        out[i] = inv_temp * (dlogp[i] * (hot - p[i]) - dentropy[i] * inner)
+            out[i] = inv_temp * (np.where(hot == p[i], 0.0, dlogp[i] * (hot - p[i])) - dentropy[i] * inner)   # 0 times an infinite slope is 0
     return out
 
 
@@ -62,7 +62,7 @@ def policy(x, targets, old, adv, ref=None, weights=None, clip=(0.2, 0.2), kl=0.0
         if kl != 0.0:
             with np.errstate(invalid="ignore", over="ignore"):
                 q = float(ref[i]) - logp[i]
-                token[i] += kl * (np.exp(q) - q - 1.0)
+                token[i] += kl * (np.exp(q) - q - 1.0 if q < np.inf else q)   # the limit, not inf - inf
                 g[i] += kl * (1.0 - np.exp(q))
         token[i] -= ce * ent[i]
         h[i] = -ce

@@ -48,3 +48,61 @@ def test_kl_term_alone(ops, N):
     series = sum(q ** k / np.prod(np.arange(1.0, k + 1)) for k in range(2, 25))
     want = kl * np.where(small, series, e - q)
     within(got["token_loss"], want, U * (kl * (np.abs(q * e) + np.where(np.abs(q) < 0.5, 0.0, 2 * np.abs(e))) + 5 * want), "kl_coef * (e^q - q - 1)")
+
+
+# ------------------------------------------------------------------ infinite losses
+@pytest.mark.parametrize("N", [6, 40, 300, 900, 1500, 5001, 20000, 131072])
+@pytest.mark.parametrize("kl,ce", [(0.1, 0.0), (0.1, 0.05), (0.0, 0.0), (0.0, 0.05)])
+def test_infinite_policy_losses(ops, N, kl, ce):
+    """A target that is switched off, a row with no logit at all, and differences whose exponential is beyond fp32: the loss is +inf (KL
+    term, or a loss of an unbounded ratio), columns that are switched off have gradient 0, the others of the row +-inf; a row with no
+    logit has gradient 0; the rows beside them are as ever."""
+    r = np.random.default_rng(N)
+    M = 7
+    x = r.standard_normal((M, N)).astype(np.float32)
+    off = np.zeros((M, N), bool)
+    off[:, 2] = True
+    if N > 40:
+        off[:, N // 2:N // 2 + N // 8] = True
+    x[off] = -INF
+    t = np.array([0, 2, 1, N - 1, 1, 0, 2], np.int32)
+    x[2] = -INF
+    clean = np.zeros((M, N), np.float32)
+    clean[:] = x
+    clean[[1, 2, 6]] = 0.0
+    logp = ft.rows(clean, np.where(np.isin(np.arange(M), [1, 2, 6]), 0, t))[0]
+    old, ref = (logp - 0.1).astype(np.float32), (logp + 0.2).astype(np.float32)
+    adv = np.array([0.7, 1.0, -1.0, 0.5, -2.0, 0.3, 0.0], np.float32)
+    ref[3] = 95.0                      # q above 88.7
+    old[4] = -150.0                    # the ratio, with an advantage that does not bound it
+    out = ops.policy_loss(x, t, old, adv, ref if kl else None, None, (0.2, 0.2), float(np.float32(kl)), float(np.float32(ce)))
+    infinite = np.array([False, kl > 0, kl > 0, kl > 0, True, False, kl > 0])
+    assert np.all(out["token_loss"][infinite] == INF), out["token_loss"]
+    assert np.all(np.isfinite(out["token_loss"][~infinite])), out["token_loss"]
+    assert out["loss"] == INF and out["rows"] == M
+    dx = out["dlogits"]
+    hot = np.arange(N)[None] == t[:, None]
+    assert np.all(dx[2] == 0.0)
+    assert np.all(dx[off & ~hot] == 0.0)
+    for i in np.flatnonzero(infinite):
+        if i == 2:
+            continue
+        # KL: the gradient asks for a larger log-probability; an unbounded ratio with a negative advantage for a smaller one
+        sign = 1.0 if i == 4 else -1.0
+        assert np.all(dx[i][~off[i] & ~hot[i]] == -sign * INF), dx[i]
+        assert dx[i, t[i]] == sign * INF, dx[i, t[i]]
+    fine = np.flatnonzero(~infinite)
+    alone = ops.policy_loss(x[fine], t[fine], old[fine], adv[fine], ref[fine] if kl else None, np.full(len(fine), 1 / M, np.float32), (0.2, 0.2),
+                            float(np.float32(kl)), float(np.float32(ce)))
+    # (the weight 1 / M is made by the same fp32 division)
+    np.testing.assert_array_equal(dx[fine], alone["dlogits"])
+    np.testing.assert_array_equal(out["token_loss"][fine], alone["token_loss"])
+
+
+def test_a_certain_token_with_an_infinite_ratio_has_no_gradient(ops):
+    """p = 1 at the target and nothing beside it: 1 - p and every other p_j are 0, whatever the slope"""
+    for N in (5, 200, 700, 3000, 40000):
+        x = np.full((1, N), -INF, np.float32)
+        x[0, N - 2] = 3.0
+        out = ops.policy_loss(x, np.array([N - 2], np.int32), np.array([-120.0], np.float32), np.array([-1.0], np.float32))
+        assert out["token_loss"][0] == INF and out["logp"][0] == 0.0 and np.all(out["dlogits"] == 0.0)

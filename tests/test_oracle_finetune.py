@@ -52,3 +52,13 @@ def test_preference_loss(by_length):
     logp, ref = -r.random(15) * 3, -r.random(15) * 3
     f = lambda v: ft.preference(v, off, ref, t, 0.7, 0.1, 0.2, by_length)["loss"]   # noqa: E731
     np.testing.assert_allclose(ft.preference(logp, off, ref, t, 0.7, 0.1, 0.2, by_length)["dlogp"], differences(f, logp), atol=1e-8)
+
+
+def test_limits_of_infinite_losses():
+    """A target whose log-probability is -inf: the KL term's limit is +inf, its slope -inf; a switched-off column has gradient 0."""
+    x = np.array([[0.5, -np.inf, 1.0, -np.inf]])
+    out = ft.policy(x, np.array([1]), [-1.0], [1.0], ref=[-2.0], kl=0.1)
+    assert out["loss"] == np.inf and out["token_loss"][0] == np.inf
+    np.testing.assert_array_equal(out["dlogits"], [[np.inf, -np.inf, np.inf, 0.0]])
+    out = ft.policy(np.full((1, 4), -np.inf), np.array([1]), [-1.0], [1.0], ref=[-2.0], kl=0.1)
+    assert out["loss"] == np.inf and np.all(out["dlogits"] == 0.0)

@@ -205,11 +205,17 @@ __device__ __forceinline__ RowGrad row_scalars(const RowParams& p, int row, cons
             slope = outside ? 0.0f : loss;
         }
         if (p.kl_coef != 0.0f) {
-            const float q = (float)((double)in.ref_logp - logp), e = expm1f(q);
-            // e - q loses what e and q share: 63 halves of a step just above 1/32, 7 at 1/4.  Below 1/2 the term comes from its series
-            // q^2 (1/2! + q/3! + ... + q^7/9!), whose next member is below 2e-9 of it: 3 halves, as many as e - q has from 1/2 on.
-            const float series = 0.5f + q * (1.0f / 6 + q * (1.0f / 24 + q * (1.0f / 120 + q * (1.0f / 720 + q * (1.0f / 5040 + q * (1.0f / 40320 + q * (1.0f / 362880)))))));
-            const float rest = fabsf(q) < 0.5f ? q * q * series : e - q;
+            const float q = (float)((double)in.ref_logp - logp);
+            float e, rest;   // e^q - 1, e^q - 1 - q
+            if (fabsf(q) < 0.5f) {
+                // e - q would lose what e and q share: 63 halves of a step just above 1/32, 7 at 1/4.  The term comes from its series
+                // q^2 (1/2! + q/3! + ... + q^7/9!), whose next member is below 2e-9 of it: 3 halves, as many as e - q has from 1/2 on.
+                rest = q * q * (0.5f + q * (1.0f / 6 + q * (1.0f / 24 + q * (1.0f / 120 + q * (1.0f / 720 + q * (1.0f / 5040 + q * (1.0f / 40320 + q * (1.0f / 362880))))))));
+                e = q + rest;
+            } else {
+                e = expm1f(q);
+                rest = isinf(e) ? e : e - q;   // of q = +inf, e - q would leave NaN
+            }
             loss += p.kl_coef * rest;
             slope -= p.kl_coef * e;
         }
@@ -222,7 +228,7 @@ __device__ __forceinline__ RowGrad row_scalars(const RowParams& p, int row, cons
             // p_t, and 1 - p_t: where the target is the largest, what the others sum to; elsewhere p_t is at most 1/2
             const float top = base_of(r.mx), e_t = x_t == top ? 1.0f : exp2_fast(fmaxf((x_t - top) * p.c, kNothing));
             const float others = (x_t == top ? r.ties - 1.0f + r.s : total - e_t) * inv_total;
-            g.at_target = G * others - (Entropy && e_t > 0.0f ? E * e_t * inv_total * ((float)logp + H) : 0.0f);
+            g.at_target = (others == 0.0f ? 0.0f : G * others) - (Entropy && e_t > 0.0f ? E * e_t * inv_total * ((float)logp + H) : 0.0f);
             // p_j (-G - E (log p_j + H)),  p_j = 2^(t + delta) / s,  log p_j + H = log(2) (t + delta) - U
             const float delta = from == r.mx ? 0.0f : fmaxf((from - r.mx) * p.c, kNothing), inv = exp2_fast(delta) * inv_total;
             g.a = inv * (-G - (Entropy ? E * (kLn2 * delta - U) : 0.0f));
@@ -348,6 +354,22 @@ struct RowPart {
         }
         const int c = extra_column(tid);
         if (c >= 0) __stcs(y + c, extra);
+    }
+
+    // A row whose loss is +inf has an infinite coefficient: gradients of +-inf, and NaN (0 times it) where the column's probability is 0
+    // and its gradient is to be 0.  This goes over what the thread has written to such a row y.  (The rows are few: a test per column in
+    // the loops of all rows takes 1 to 6 % of their time.)
+    __device__ __forceinline__ void clear_nan(float* y, int tid)
+    {
+        for (step = 0; step == 0 || step < quads; step += Group * V) {
+#pragma unroll 1
+            for (int k = 0; k < V; k++)
+                if (has(tid, k))
+                    for (int i = 0; i < 4; i++)
+                        if (isnan(y[column(tid, k) + i])) y[column(tid, k) + i] = 0.0f;
+            const int c = extra_column(tid);
+            if (c >= 0 && isnan(y[c])) y[c] = 0.0f;
+        }
     }
 
     // zeros for the whole part
@@ -498,6 +520,10 @@ __global__ void __launch_bounds__(128) rows_held_kernel(const RowParams p, int)
         r[k].store(dx + k * p.ld_d, tid);
         if (r[k].owns(t[k], tid)) dx[k * p.ld_d + t[k]] = at_target;
     }
+    if (__any_sync(mask, isinf(g.a)))
+#pragma unroll
+        for (int k = 0; k < Rows; k++)
+            if (isinf(__shfl_sync(mask, g.a, k, Group))) r[k].clear_nan(dx + k * p.ld_d, tid);
 }
 
 // Longer rows: a block (or the blocks of a cluster, which take `part` columns each) walks over the row with running sums per thread,
@@ -618,6 +644,7 @@ __global__ void __launch_bounds__(Threads) rows_walk_kernel(const RowParams p, i
         r.step -= kStep;
         r.template load<true>(x, tid);
     }
+    if (isinf(g.a)) r.clear_nan(dx, tid);
 }
 
 // dlogits of the log-probabilities from the forward's statistics.  A group of threads takes 4 * Group * V columns of a row;
