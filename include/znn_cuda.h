@@ -304,6 +304,8 @@ int znn_policy_loss(const float* logits, long long ld, const int32_t* targets, f
  *   rewards[s] = beta * sum_i (logp_i - ref_logp_i) (ref_logp may be NULL = 0), divided by the number of its rows not left
  *   out where length_normalize = 1 (0 for none);  m = rewards[2p] - rewards[2p + 1] - margin;
  *   pair_loss[p] = -(1 - label_smoothing) * log sigmoid(m) - label_smoothing * log sigmoid(-m);  loss[0] = mean of pair_loss.
+ *   Rewards may be -inf (a token of log-probability -inf): m = +inf costs nothing without smoothing, every other infinite m costs +inf,
+ *   and the slopes are the limits; two of them in one pair have no difference: NaN.
  * dlogp (may be NULL) = d loss[0] / d logp for the rows of the sequences, 0 for those left out, which
  * znn_token_logprob_bwd takes; rows behind the last sequence stay as they were.  A pair whose offsets are not ascending within
  * 0 .. M has rewards and loss NaN, its rows are neither read nor written, and ZNN_DEV_BAD_INDEX is set. */

@@ -92,7 +92,7 @@ def preference(logp, offsets, ref=None, targets=None, beta=0.1, smoothing=0.0, m
             share.append(beta / n if by_length and n else 0.0 if by_length else beta)
             rewards[2 * p + k] = share[k] * d[sl][kept[sl]].sum()
         m = rewards[2 * p] - rewards[2 * p + 1] - margin
-        pair[p] = (1 - smoothing) * np.logaddexp(0, -m) + smoothing * np.logaddexp(0, m)
+        pair[p] = (1 - smoothing) * np.logaddexp(0, -m) + (smoothing * np.logaddexp(0, m) if smoothing else 0.0)   # 0 of an infinite margin
         slope = (smoothing * np.exp(-np.logaddexp(0, -m)) - (1 - smoothing) * np.exp(-np.logaddexp(0, m))) / P
         for k, sign in ((0, 1.0), (1, -1.0)):
             sl = slice(o[k], o[k + 1])

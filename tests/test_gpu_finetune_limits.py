@@ -106,3 +106,37 @@ def test_a_certain_token_with_an_infinite_ratio_has_no_gradient(ops):
         x[0, N - 2] = 3.0
         out = ops.policy_loss(x, np.array([N - 2], np.int32), np.array([-120.0], np.float32), np.array([-1.0], np.float32))
         assert out["token_loss"][0] == INF and out["logp"][0] == 0.0 and np.all(out["dlogits"] == 0.0)
+
+
+@pytest.mark.parametrize("P,length", [(4, 5), (40, 30), (4, 3000), (2, 20000)])
+@pytest.mark.parametrize("smooth", [0.0, 0.1])
+@pytest.mark.parametrize("by_length", [False, True])
+def test_infinite_rewards(ops, P, length, smooth, by_length):
+    """A log-probability of -inf in the other answer (margin +inf: loss 0, or +inf where labels are smoothed), in the preferred one
+    (margin -inf: loss +inf, slope 1 - label_smoothing), in both (no margin: NaN); an ordinary pair beside them."""
+    r = np.random.default_rng(P)
+    M = 2 * P * length
+    logp = (-2 * r.random(M)).astype(np.float32)
+    off = (np.arange(2 * P + 1) * length).astype(np.int32)
+    logp[1 * length + 2] = -INF                      # pair 0: the other answer
+    logp[2 * length + 1] = -INF                      # pair 1: the preferred one
+    beta, smooth = float(np.float32(0.3)), float(np.float32(smooth))
+    got = ops.preference_loss(logp, off, None, None, beta, smooth, 0.0, by_length)
+    want = ft.preference(logp, off, None, None, beta, smooth, 0.0, by_length)
+    share = beta / length if by_length else beta
+    assert want["pair_loss"][0] == (np.inf if smooth else 0.0) and want["pair_loss"][1] == np.inf
+    np.testing.assert_allclose(want["dlogp"][:length], smooth / P * share, rtol=1e-12)
+    np.testing.assert_allclose(want["dlogp"][2 * length:3 * length], (smooth - 1) / P * share, rtol=1e-12)
+    # as test_preference_loss: fp64 inside, one rounding of each output
+    for k in ("pair_loss", "rewards", "dlogp"):
+        within(got[k], want[k], U * np.abs(np.where(np.isfinite(want[k]), want[k], 0.0)) * 1.001 + 1e-12, k)
+    assert got["loss"] == INF
+    if P > 2:
+        logp[2 * length + 1] = -1.0
+        got = ops.preference_loss(logp, off, None, None, beta, 0.0, 0.0, by_length)
+        want = ft.preference(logp, off, None, None, beta, 0.0, 0.0, by_length)
+        assert np.isfinite(want["loss"])
+        within(got["loss"], want["loss"], 2 * U * want["loss"] * 1.001 + 1e-12, "loss")
+        logp[4 * length] = logp[5 * length] = -INF
+        got = ops.preference_loss(logp, off, None, None, beta, 0.0, 0.0, by_length)
+        assert np.isnan(got["loss"]) and np.isnan(got["pair_loss"][2]) and np.all(np.isfinite(np.delete(got["pair_loss"], 2)))

@@ -62,3 +62,11 @@ def test_limits_of_infinite_losses():
     np.testing.assert_array_equal(out["dlogits"], [[np.inf, -np.inf, np.inf, 0.0]])
     out = ft.policy(np.full((1, 4), -np.inf), np.array([1]), [-1.0], [1.0], ref=[-2.0], kl=0.1)
     assert out["loss"] == np.inf and np.all(out["dlogits"] == 0.0)
+
+
+def test_limits_of_infinite_margins():
+    inf = np.inf
+    for smooth, losses in ((0.0, [0.0, inf]), (0.1, [inf, inf])):
+        out = ft.preference([-1.0, -inf, -inf, -1.0], [0, 1, 2, 3, 4], beta=0.5, smoothing=smooth)
+        np.testing.assert_array_equal(out["pair_loss"], losses)
+        np.testing.assert_allclose(out["dlogp"], np.array([smooth, -smooth, smooth - 1, 1 - smooth]) * 0.25, atol=1e-15)

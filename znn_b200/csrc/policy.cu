@@ -739,7 +739,8 @@ __device__ __forceinline__ PairTerms pair_terms(double m, double eps, int P)
 {
     const double e = exp(-fabs(m)), soft = log1p(e), inv = 1.0 / (1.0 + e);   // log(1 + e^-|m|), sigmoid(|m|): no overflow either way
     PairTerms t;
-    t.loss = (1.0 - eps) * (soft + fmax(-m, 0.0)) + eps * (soft + fmax(m, 0.0));
+    t.loss = (1.0 - eps) * (soft + fmax(-m, 0.0));
+    if (eps != 0.0) t.loss += eps * (soft + fmax(m, 0.0));   // (without smoothing an infinite margin costs nothing, where 0 * inf would be NaN)
     t.slope = (eps - (m >= 0.0 ? e * inv : inv)) / (double)P;   // -(1 - eps) sigmoid(-m) + eps sigmoid(m)
     return t;
 }
