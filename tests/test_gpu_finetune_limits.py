@@ -140,3 +140,93 @@ def test_infinite_rewards(ops, P, length, smooth, by_length):
         logp[4 * length] = logp[5 * length] = -INF
         got = ops.preference_loss(logp, off, None, None, beta, 0.0, 0.0, by_length)
         assert np.isnan(got["loss"]) and np.isnan(got["pair_loss"][2]) and np.all(np.isfinite(np.delete(got["pair_loss"], 2)))
+
+
+# ------------------------------------------------------------------ rows that are nearly certain
+def nearly_certain(r, sigma, N, top, shift):
+    """A row whose largest logit stands at `top` and whose others' exponentials sum to about sigma, relative to the largest"""
+    d = np.minimum(np.log(sigma / max(N - 1, 1)) + 0.5 * r.standard_normal(N), -0.2)
+    x = (shift + d).astype(np.float32)
+    x[top] = shift
+    return x
+
+
+def certain_case(N, seed, inv_temp):
+    """sums of the others from 0.7 down to 1e-9, the target at the largest logit or (every fourth row) elsewhere; float64 scalars that
+    keep the small part"""
+    r = np.random.default_rng(seed)
+    sigma = np.repeat([0.7, 0.3, 0.2, 0.05, 1e-2, 1e-3, 1e-4, 1e-6, 1e-9], 4)
+    M = len(sigma)
+    top = r.integers(0, N, M)
+    x = np.stack([nearly_certain(r, s ** (1 / inv_temp), N, k, np.float32(r.uniform(-8, 8))) for s, k in zip(sigma, top)])
+    t = np.where(np.arange(M) % 4 == 3, (top + 1 + r.integers(0, N - 1, M)) % N, top).astype(np.int32)
+    d = (x.astype(np.float64) - x[np.arange(M), top].astype(np.float64)[:, None]) * inv_temp
+    e = np.exp(d)
+    e[np.arange(M), top] = 0.0                       # the others alone
+    small = e.sum(1)
+    log_s = np.log1p(small)
+    p = e / (1 + small)[:, None]
+    u = (p * d).sum(1)
+    return r, x, t, top, d, small, log_s, p, u, log_s - u
+
+
+SIZES = [2, 5, 33, 64, 65, 300, 400, 512, 700, 1000, 1025, 5000, 8191, 8192, 9001, 40000]
+
+
+@pytest.mark.parametrize("N", SIZES)
+@pytest.mark.parametrize("inv_temp", [1.0, 0.8])
+def test_log_probabilities_of_nearly_certain_rows(ops, N, inv_temp):
+    """logp and entropy to a few K halves of a step of their own value, however small: every exponential carries 2 D + 4, the sums
+    N / 32 + 16 (K), log1p and the division 2 more each; -u (positive) is made of products d e with 3 more; nothing cancels at the
+    largest logit.  Elsewhere logp is d - log s, of size |logp|."""
+    inv_temp = float(np.float32(inv_temp))
+    r, x, t, top, d, small, log_s, p, u, H = certain_case(N, N, inv_temp)
+    K = row_k(x, inv_temp) + 8
+    logp, ent, _ = ops.token_logprob_fwd(x, t, inv_temp)
+    want = np.where(t == top, -log_s, d[np.arange(len(t)), t] - log_s)
+    tol = np.where(t == top, K, 4) * U * np.abs(want) + np.where(t == top, 0.0, K * U * log_s)
+    within(logp, want, tol, "logp")
+    within(ent, H, K * U * H, "entropy")
+    out = ops.policy_loss(x, t, want.astype(np.float32), np.ones(len(t), np.float32), inv_temp=inv_temp)
+    within(out["logp"], want, tol, "logp of the policy loss")
+
+
+@pytest.mark.parametrize("N", SIZES)
+@pytest.mark.parametrize("entropy", [False, True])
+@pytest.mark.parametrize("accumulate,in_place", [(False, False), (True, False), (False, True)])
+def test_gradient_of_nearly_certain_rows(ops, L, N, entropy, accumulate, in_place):
+    """inv_temp (g ([j = t] - p_j) - h p_j (log p_j + H)), each part to K + 24 halves of a step of its own size.  At the largest logit
+    1 - p is the others' sum over the whole, and log p + H = -u; where the others sum to 1/32 or more, 1 - p is a difference of
+    fp32 numbers, which leaves 3 halves of a step of p (the sum's, the quotient's, the exponential's)."""
+    inv_temp = float(np.float32(0.8))
+    r, x, t, top, d, small, log_s, p, u, H = certain_case(N, N + 1, inv_temp)
+    M, rows = len(t), np.arange(len(t))
+    _, ent, stats = ops.token_logprob_fwd(x, t, inv_temp)
+    g, h = r.standard_normal(M).astype(np.float32), (r.standard_normal(M) * entropy).astype(np.float32)
+    part = p.copy()
+    part[rows, top] = 1 / (1 + small)
+    hot = np.zeros((M, N))
+    hot[rows, t] = 1.0
+    one_less = hot - part
+    one_less[rows, top] = np.where(t == top, small / (1 + small), -1 / (1 + small))
+    inner = part * (d - log_s[:, None] + H[:, None])
+    size = part * (np.abs(d) + log_s[:, None] + H[:, None])
+    inner[rows, top] = part[rows, top] * -u
+    size[rows, top] = part[rows, top] * (H + log_s)
+    G, E = g.astype(np.float64)[:, None], h.astype(np.float64)[:, None]
+    want = inv_temp * (G * one_less - E * inner)
+    tol = inv_temp * (np.abs(G) * np.abs(one_less) + np.abs(E) * size) * (row_k(x, inv_temp)[:, None] + 24) * U
+    tol += inv_temp * 3 * U * np.abs(G) * (part * hot) * (small >= 1 / 32.01)[:, None]
+    before = (r.standard_normal((M, N)) * small[:, None]).astype(np.float32)
+    if in_place:
+        up = ops.DevBuf.from_host
+        xb, tb, sb, gb, eb, hb = up(x), up(t), up(stats), up(g), up(ent), up(h)
+        L.call("znn_token_logprob_bwd", xb.ptr, N, tb.ptr, inv_temp, sb.ptr, eb.ptr if entropy else None, gb.ptr, hb.ptr if entropy else None, xb.ptr, N, 0, M, N)
+        got = xb.to_host((M, N))
+        apart = ops.token_logprob_bwd(x, t, stats, g, None, ent if entropy else None, h if entropy else None, inv_temp)
+        np.testing.assert_array_equal(got, apart)
+    else:
+        got = ops.token_logprob_bwd(x, t, stats, g, before.copy() if accumulate else None, ent if entropy else None, h if entropy else None, inv_temp)
+    if accumulate:
+        want = want + before
+    within(got, want, tol + U * np.abs(want), "dlogits")

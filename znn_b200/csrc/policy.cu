@@ -647,26 +647,210 @@ __global__ void __launch_bounds__(Threads) rows_walk_kernel(const RowParams p, i
     if (isinf(g.a)) r.clear_nan(dx, tid);
 }
 
-// dlogits of the log-probabilities from the forward's statistics.  A group of threads takes 4 * Group * V columns of a row;
-// every load of the logits, and of the gradient that is added to, is under way before the first result is made.  8192 x 8192: 76 us,
-// 6.7 TB/s.
+// Rows whose sum s is below this are nearly certain.  1 - p of the largest logit, and log s beside an entropy of the same size, are then
+// what the others sum to: s in fp32 has the error of its 1 in them (3 halves of a step of 1: 99 of 1 - p at this limit, and nothing is
+// left of 1 - p = 1e-8).  The others are summed up once more for that one column, which takes another walk over a row that is in more
+// than one part: 8192 x 8192 79 us without such rows, 88 where half are, 4000 x 32003 153 and 200 where all are.
+constexpr float kNearlyCertain = 1.03125f;
+
+// the lanes of this thread's group (of up to a warp)
+template <int Group>
+__device__ __forceinline__ unsigned group_mask()
+{
+    return Group < 32 ? ((1u << (Group & 31)) - 1) << (threadIdx.x & 31 & ~(Group - 1)) : kAllLanes;
+}
+
+// the sum of v over a group's lanes, in each of them (once per block); all reads that v is made of are done then
+template <int Group>
+__device__ __forceinline__ float group_sum(float v, unsigned mask, float* sh)
+{
+    v = warp_sum<(Group < 32 ? Group : 32)>(v, mask);
+    if (Group < 256) return v;
+    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = 0.0f;
+#pragma unroll
+    for (int i = 0; i < Group / 32; i++) v += sh[i];
+    return v;
+}
+
+// what the logits of a row but the largest sum to, this thread's share
+template <int Group>
+__device__ __forceinline__ float others_of_row(const float* x, int N, float top, float c, int tid)
+{
+    constexpr int V = Group < 32 ? 2 : 4;
+    RowPart<Group, V, false> r;
+    float sum = 0.0f;
+    r.place(x, N);
+#pragma unroll 1
+    for (;; r.step += V * Group) {
+        r.load(x, tid);
+        auto add = [&](float v) { sum += v == top ? 0.0f : exp2_fast((v - top) * c); };
+#pragma unroll
+        for (int k = 0; k < V; k++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) add(r.v[k][i]);
+        add(r.extra);
+        if (r.step + V * Group >= r.quads) return sum;
+    }
+}
+
+// The gradient of a row's logit x_j without the target's own part, p_j (-G - E (log p_j + H)), with p_j = 2^t / s, log p_j = log(2) t - log s:
+// 2^t (a + b t).  (Roundings are spelled out where two kernels' results are to be the same bits.)
+struct BwdSlope {
+    float base, c, a, b;
+    __device__ __forceinline__ BwdSlope(float top, float it, float s, float G, float E, float H)
+    {
+        const float inv = 1.0f / s;
+        base = base_of(top);
+        c = it * kLog2e;
+        a = __fmul_rn(inv, E != 0.0f ? __fmaf_rn(-E, H - logf(s), -G) : -G);
+        b = -inv * E * kLn2;
+    }
+    __device__ __forceinline__ float operator()(float x) const
+    {
+        const float te = max_nan((x - base) * c, kNothing);
+        return __fmul_rn(exp2_fast(te), __fmaf_rn(b, te, a));
+    }
+};
+
+// The gradient of a nearly certain row's largest logit where it is the target and where it is not: 1 - p = others / (1 + others),
+// log p = -log(1 + others).
+struct LargestGrad {
+    float target, other;
+};
+__device__ __forceinline__ LargestGrad largest_grad(float others, float G, float E, float H)
+{
+    const float p = __fdividef(1.0f, 1.0f + others), Gp = __fmul_rn(G, p), Ep = E != 0.0f ? __fmul_rn(E * p, H - log1pf(others)) : 0.0f;
+    return {__fsub_rn(__fmul_rn(Gp, others), Ep), __fsub_rn(-Gp, Ep)};
+}
+
+// A nearly certain row over the logits' own buffer, in more than one part: one group has them all, since each is needed before any is
+// written over.
+template <int Group>
+__device__ __noinline__ void bwd_certain_row_in_place(float* x, int N, int t, const BwdSlope slope, float G, float E, float H, float* sh)
+{
+    const int tid = Group < 256 ? threadIdx.x % Group : threadIdx.x;
+    const LargestGrad largest = largest_grad(group_sum<Group>(others_of_row<Group>(x, N, slope.base, slope.c, tid), group_mask<Group>(), sh), G, E, H);
+    RowPart<Group, 2, false> r;
+    r.place(x, N);
+#pragma unroll 1
+    for (;; r.step += 2 * Group) {
+        r.load(x, tid);
+        auto make = [&](float& v, int column) {
+            const bool target = column == t;
+            v = v == slope.base ? (target ? largest.target : largest.other) : target ? __fadd_rn(slope(v), G) : slope(v);
+        };
+#pragma unroll
+        for (int k = 0; k < 2; k++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) make(r.v[k][i], r.column(tid, k) + i);
+        make(r.extra, r.extra_column(tid));
+        r.store(x, tid);
+        if (r.step + 2 * Group >= r.quads) return;
+    }
+}
+
+// A part, from column `first` on, its logits loaded, of a row that may be nearly certain.  `mask`: the lanes of the warp that come here.
 template <bool Accumulate, bool Aligned, int Group, int V>
-__global__ void __launch_bounds__(Group < 256 ? 128 : Group)
+__device__ __forceinline__ void bwd_certain_part(RowPart<Group, V, Aligned>& r, const float (&old)[V][4], float old_extra, const float* x, float* dx, int first,
+                                                 int N, int parts, int t, const BwdSlope& slope, float G, float E, float H, bool certain, int tid, unsigned mask,
+                                                 float* sh)
+{
+    const auto each = [&](auto&& f) {
+#pragma unroll
+        for (int k = 0; k < V; k++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) f(r.v[k][i], Accumulate ? old[k][i] : 0.0f, r.column(tid, k) + i);
+        if (!Aligned) f(r.extra, old_extra, r.extra_column(tid));
+    };
+    const float top = certain ? slope.base : CUDART_NAN_F;   // equal to no logit where the row needs nothing
+    const bool any = Group > 8 || __any_sync(mask, certain);
+    float top_before = 0.0f;
+    int top_at = -1;   // where the largest logit is, in the thread that has it
+    LargestGrad largest{0.0f, 0.0f};
+    if (any && parts == 1) {
+        float others = 0.0f;
+        each([&](float v, float, int) { others += v == top ? 0.0f : exp2_fast((v - slope.base) * slope.c); });
+        largest = largest_grad(group_sum<Group>(others, mask, sh), G, E, H);
+    }
+    each([&](float& v, float before, int column) {
+        float o = slope(v);
+        if (column == t - first) o = __fadd_rn(o, G);
+        if (v == top) {
+            o = column == t - first ? largest.target : largest.other;
+            top_at = column;
+            top_before = before;
+        }
+        v = Accumulate ? before + o : o;
+    });
+    r.store(dx, tid);
+    if (!any || parts == 1) return;
+    // in more than one part: the part that has the largest logit makes it when all else is
+    if (Group == 256) {
+        if (!__syncthreads_or(top_at >= 0)) return;
+    } else {
+        const unsigned have = __ballot_sync(mask, top_at >= 0) & group_mask<Group>();
+        mask = Group < 32 ? __ballot_sync(mask, have != 0) : kAllLanes;
+        if (have == 0) return;
+    }
+    largest = largest_grad(group_sum<Group>(others_of_row<Group>(x - first, N, slope.base, slope.c, tid), mask, sh), G, E, H);
+    if (top_at >= 0) dx[top_at] = top_before + (top_at == t - first ? largest.target : largest.other);
+}
+
+// a part of a nearly certain row from its load on; a call, so that what it needs is not in the way of the rows that are not
+template <bool Accumulate, bool Aligned, int Group, int V>
+__device__ __noinline__ void bwd_certain_row(const float* x, float* dx, int first, int n, int N, int parts, int t, const BwdSlope slope, float G, float E, float H,
+                                             int tid, float* sh)
+{
+    RowPart<Group, V, Aligned> r;
+    float old[V][4], old_extra = 0.0f;
+    r.place(x, n);
+    r.load(x, tid);
+    if (Accumulate) r.load_beside(dx, tid, old, old_extra);
+    bwd_certain_part<Accumulate, Aligned, Group, V>(r, old, old_extra, x, dx, first, N, parts, t, slope, G, E, H, true, tid, kAllLanes, sh);
+}
+
+// Blocks per SM that the rows that are not nearly certain have room for.  Without the bound the others' way takes registers from them:
+// 4 to 14 % of their time.
+constexpr int bwd_blocks(bool accumulate, bool aligned, int group, int quads)
+{
+    const int registers = accumulate ? (aligned ? (group == 256 ? 48 : quads == 4 ? 56 : 40) : (group == 256 ? 64 : quads == 4 ? 72 : quads == 2 ? 48 : 40))
+                                     : (group == 256 || quads <= 2 ? 40 : quads == 4 ? (aligned ? 48 : 56) : (aligned ? 64 : 72));
+    return 65536 / (registers * (group < 256 ? 128 : group));
+}
+
+// dlogits of the log-probabilities from the forward's statistics.  A group of threads takes 4 * Group * V columns of a row, one of its
+// `parts`; every load of the logits, and of the gradient that is added to, is under way before the first result is made.  8192 x 8192:
+// 78 us, 6.5 TB/s.
+template <bool Accumulate, bool Aligned, int Group, int V>
+__global__ void __launch_bounds__(Group < 256 ? 128 : Group, bwd_blocks(Accumulate, Aligned, Group, V))
 logprob_bwd_kernel(const float* logits, long long ld, const int32_t* __restrict__ targets, float it,
                    const float* __restrict__ stats, const float* __restrict__ entropy, const float* __restrict__ dlogp,
                    const float* __restrict__ dentropy, float* dlogits, long long ld_d, int M, int N, int parts, int part)
 {
+    __shared__ float sh[Group < 256 ? 1 : Group / 32];
     const int tid = Group < 256 ? threadIdx.x % Group : threadIdx.x;
     const unsigned unit = Group < 256 ? blockIdx.x * (128 / Group) + threadIdx.x / Group : blockIdx.x;
     const int row = (int)(unit / (unsigned)parts), first = (int)(unit % (unsigned)parts) * part, n = min(part, N - first);
-    if (row >= M) return;
+    if (Group > 8 && row >= M) return;
     wait_for_previous_kernel();
+    const bool there = row < M;
     const float* x = logits + (size_t)row * ld + first;
     float* dx = dlogits + (size_t)row * ld_d + first;
-    const int t = targets[row];
-    const float s = stats[2 * (size_t)row + 1];
-    if (t < 0 || t >= N || s == 0.0f) {
-        if (!Accumulate) RowPart<Group, V, Aligned>::clear(dx, n, tid);
+    const int t = there ? targets[row] : -1;
+    const float s = there ? stats[2 * (size_t)row + 1] : 0.0f;
+    const bool used = t >= 0 && t < N && s != 0.0f, certain = s < kNearlyCertain, whole = certain && parts > 1 && !Accumulate && x == dx;
+    const unsigned lanes = Group == 8 ? __ballot_sync(kAllLanes, used && !whole) : kAllLanes;
+    if (!used) {
+        if (!Accumulate && there) RowPart<Group, V, Aligned>::clear(dx, n, tid);
+        return;
+    }
+    if (certain && (whole || Group > 8)) {
+        const float G = it * (dlogp ? dlogp[row] : 0.0f), E = it * (dentropy ? dentropy[row] : 0.0f), H = E != 0.0f ? entropy[row] : 0.0f;
+        const BwdSlope slope(stats[2 * (size_t)row], it, s, G, E, H);
+        if (!whole) bwd_certain_row<Accumulate, Aligned, Group, V>(x, dx, first, n, N, parts, t, slope, G, E, H, tid, sh);
+        else if (first == 0) bwd_certain_row_in_place<Group>(dx, N, t, slope, G, E, H, sh);
         return;
     }
     RowPart<Group, V, Aligned> r;
@@ -674,19 +858,27 @@ logprob_bwd_kernel(const float* logits, long long ld, const int32_t* __restrict_
     r.place(x, n);
     r.load(x, tid);
     if (Accumulate) r.load_beside(dx, tid, old, old_extra);
-    // p_j (-G - E (log p_j + H)) with p_j = 2^t / s, log p_j = log(2) t - log s
     const float G = it * (dlogp ? dlogp[row] : 0.0f), E = it * (dentropy ? dentropy[row] : 0.0f);
+    if (Group == 8) {
+        // several rows share a warp: one way for all of them, and the target's part with the rest (adding it to what is stored takes a
+        // trip to memory at each warp's end: 65536 x 30 8.9 us)
+        const float H = E != 0.0f ? entropy[row] : 0.0f;
+        const BwdSlope slope(stats[2 * (size_t)row], it, s, G, E, H);
+        bwd_certain_part<Accumulate, Aligned, Group, V>(r, old, old_extra, x, dx, first, N, parts, t, slope, G, E, H, certain, tid, lanes, sh);
+        return;
+    }
+    // as BwdSlope (which reads the entropy whether or not it is needed yet: 3 % of 8192 x 8192)
     const float base = base_of(stats[2 * (size_t)row]), c = it * kLog2e, inv = 1.0f / s;
     const float a = inv * (-G - (E != 0.0f ? E * (entropy[row] - logf(s)) : 0.0f)), b = -inv * E * kLn2;
-    auto slope = [&](float& x, float before) {
+    auto make = [&](float& x, float before) {
         const float te = max_nan((x - base) * c, kNothing), o = exp2_fast(te) * (a + b * te);
         x = Accumulate ? before + o : o;
     };
 #pragma unroll
     for (int k = 0; k < V; k++)
 #pragma unroll
-        for (int i = 0; i < 4; i++) slope(r.v[k][i], Accumulate ? old[k][i] : 0.0f);
-    if (!Aligned) slope(r.extra, old_extra);
+        for (int i = 0; i < 4; i++) make(r.v[k][i], Accumulate ? old[k][i] : 0.0f);
+    if (!Aligned) make(r.extra, old_extra);
     r.store(dx, tid);
     if (r.owns(t - first, tid)) dx[t - first] += G;
 }
@@ -1023,6 +1215,7 @@ static int launch_bwd(const BwdArgs& b)
 template <bool Accumulate, bool Aligned>
 static int launch_bwd_as(const BwdArgs& b)
 {
+    if (b.N <= 32) return launch_bwd<Accumulate, Aligned, 8, 1>(b);
     if (b.N <= 64) return launch_bwd<Accumulate, Aligned, 8, 2>(b);
     if (b.N <= 384) return launch_bwd<Accumulate, Aligned, 8, 4>(b);
     if (b.N <= 512) return launch_bwd<Accumulate, Aligned, 32, 4>(b);
