@@ -278,7 +278,8 @@ int znn_softmax_xent_fwd_static(const float* logits, const int32_t* targets, flo
  * znn_token_logprob_bwd, from dlogp and dentropy (NULL = no such gradient; then entropy may be NULL too):
  *   dlogits_j (+)= inv_temp * (dlogp * ([j = t] - p_j) - dentropy * p_j * (log p_j + entropy)).
  * accumulate = 1 adds (rows left out stay as they are), 0 stores (rows left out become 0).  With accumulate = 0 dlogits
- * may be the logits' own buffer (ld_d == ld). */
+ * may be the logits' own buffer (ld_d == ld).  dlogp and dentropy of the rows in use are finite numbers (a row with one that is not has
+ * no finite gradient, in its switched-off columns either). */
 int znn_token_logprob_fwd(const float* logits, long long ld, const int32_t* targets, float inv_temp, float* logp, float* entropy,
                           float* stats, int M, int N);
 int znn_token_logprob_bwd(const float* logits, long long ld, const int32_t* targets, float inv_temp, const float* stats,
