@@ -1,0 +1,45 @@
+"""Graph ops of the fine-tuning losses over many passes of one tape, and what a refused op leaves behind."""
+import numpy as np
+import pytest
+
+from test_gpu_finetune_models import U, case
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from znn_b200 import ops as _ops
+    _ops.init(0)
+    return _ops
+
+
+@pytest.fixture(scope="module")
+def G(ops):
+    from znn_b200.graph import Graph
+    return Graph
+
+
+@pytest.mark.parametrize("two", [False, True])
+def test_a_tape_that_runs_many_times_needs_no_more_memory(ops, G, two):
+    """zeroGrad, forward, backward of one tape, hundreds of times, in an arena that has room for each loss's spare gradient once
+    (logits and their gradient, two spare gradients: 4 x 19240 bytes; what is left of 160 KB holds less than another five)."""
+    x, t, old, adv, ref = case(11)
+    want = ops.policy_loss(x, t, old, adv)["dlogits"]
+    g = G(160 << 10)
+    X = g.array(x, True)
+    loss = g.policyLoss(X, t, g.array(old), g.array(adv))
+    if two:
+        want = want + ops.policy_loss(x, t, old, adv, ref, None, (0.2, 0.2), 0.5)["dlogits"]
+        loss = g.add(loss, g.policyLoss(X, t, g.array(old), g.array(adv), g.array(ref), None, (0.2, 0.2), 0.5))
+    for k in range(300):
+        g.zeroGrad()
+        g.forward()
+        g.backward(loss)
+        if k % 100 == 99:
+            np.testing.assert_allclose(X.grad, want, rtol=0, atol=2 * U * np.abs(want).max())
+    # and added to what earlier passes left, as every gradient is
+    g.zeroGrad()
+    for k in range(3):
+        g.backward(loss)
+    np.testing.assert_allclose(X.grad, 3 * want, rtol=0, atol=8 * U * np.abs(want).max())

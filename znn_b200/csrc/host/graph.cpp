@@ -1059,10 +1059,10 @@ void Op::backward()
             if (grad_is_fresh(A) && grad_root(A)->grad_stored_by == this) {
                 mark_grad_written(A);
             } else {   // another op or arm was here: make the gradient once more and add it
-                float* dlogits = (float*)arena->alloc(A->numel() * sizeof(float));
-                policy_loss(dlogits);
+                if (!spare_grad) spare_grad = (float*)arena->alloc(A->numel() * sizeof(float));
+                policy_loss(spare_grad);
                 ensure_grad(A);
-                check(znn_accumulate(dlogits, A->grad, A->numel()), "PolicyLoss backward");
+                check(znn_accumulate(spare_grad, A->grad, A->numel()), "PolicyLoss backward");
             }
         }
         break;

@@ -137,6 +137,7 @@ struct Op {
     const int32_t* offsets = nullptr;
     int pairs = 0;
     Arena* arena = nullptr;
+    float* spare_grad = nullptr;   // PolicyLoss: where a gradient that is added to another is made, one for all backward passes of the tape
     void forward();             // src/autodiff.zig:107-575
     void backward();            // src/autodiff.zig:579-1231
 
