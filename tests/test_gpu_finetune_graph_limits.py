@@ -43,3 +43,34 @@ def test_a_tape_that_runs_many_times_needs_no_more_memory(ops, G, two):
     for k in range(3):
         g.backward(loss)
     np.testing.assert_allclose(X.grad, 3 * want, rtol=0, atol=8 * U * np.abs(want).max())
+
+
+def test_a_refused_op_leaves_the_tape(ops, G):
+    """Settings that the entry point refuses, and an arena that is full: the tape is what it was, runs again and gives the same gradients."""
+    from znn_b200._lib import ZnnError
+    x, t, old, adv, ref = case(12)
+    want = ops.policy_loss(x, t, old, adv)["dlogits"]
+    g = G(320 << 10)
+    X, o, a = g.array(x, True), g.array(old), g.array(adv)
+    loss = g.policyLoss(X, t, o, a)
+    L = g.tokenLogProb(X, t)
+    n = g.num_ops()
+    for refused in (lambda: g.policyLoss(X, t, o, a, kl_coef=0.1), lambda: g.policyLoss(X, t, o, a, clip=(2.0, 0.2)), lambda: g.policyLoss(X, t, o, a, inv_temp=0.0),
+                    lambda: g.tokenLogProb(X, t, -1.0), lambda: g.preferenceLoss(L, [0, 3, 9], beta=np.nan), lambda: g.preferenceLoss(L, [0, 3, 9], label_smoothing=1.0)):
+        with pytest.raises(ZnnError):
+            refused()
+        assert g.num_ops() == n
+    g.forward()
+    g.backward(loss)
+    np.testing.assert_array_equal(X.grad, want)
+    with pytest.raises(ZnnError, match="arena"):
+        for _ in range(10000):
+            g.policyLoss(X, t, o, a)
+            n += 1
+    assert g.num_ops() == n
+    with pytest.raises(ZnnError, match="arena"):
+        for _ in range(10000):
+            g.tokenLogProb(X, t)
+            n += 1
+    assert g.num_ops() == n
+    g.forward()

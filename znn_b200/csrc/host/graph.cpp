@@ -167,6 +167,25 @@ Op* Graph::new_op(OpType type, std::initializer_list<Tensor*> inputs, Tensor* ou
     return o;
 }
 
+void Graph::first_run(Op* o)
+{
+    try {
+        o->forward();
+    } catch (...) {
+        ops_.pop_back();
+        for (Tensor* in : o->inputs) {
+            in->consumers--;
+            in->last_consumer = nullptr;
+            for (size_t i = ops_.size(); i > 0 && !in->last_consumer; i--)
+                for (Tensor* t : ops_[i - 1]->inputs)
+                    if (t == in) in->last_consumer = ops_[i - 1];
+        }
+        o->outputs[0]->creator = nullptr;
+        delete o;
+        throw;
+    }
+}
+
 Tensor* Graph::tensorND(const Shape& shape, bool requires_grad) { return new_tensor(shape, requires_grad, true); }
 
 Tensor* Graph::array(const Shape& shape, const float* host_data, bool requires_grad)
@@ -411,11 +430,12 @@ Tensor* Graph::tokenLogProb(Tensor* logits, const int32_t* dev_targets, float in
 {
     const int M = rows_of(logits, "tokenLogProb");
     Tensor* C = new_tensor(Shape{(size_t)M, 1}, logits->requires_grad, false);
+    float* scratch = (float*)arena_->alloc((size_t)M * 2 * sizeof(float));
     Op* o = new_op(OpType::TokenLogProb, {logits}, C);
     o->targets = const_cast<int32_t*>(dev_targets);
     o->policy.inv_temp = inv_temp;
-    o->scratch = (float*)arena_->alloc((size_t)M * 2 * sizeof(float));
-    o->forward();
+    o->scratch = scratch;
+    first_run(o);
     return C;
 }
 
@@ -427,14 +447,15 @@ Tensor* Graph::policyLoss(Tensor* logits, const int32_t* dev_targets, Tensor* ol
         if (t && t->numel() != M) throw Error(ZNN_ERR_INVALID, "policyLoss: old, advantages, ref and weights need one value per row");
     if (!old || !advantages) throw Error(ZNN_ERR_INVALID, "policyLoss: old and advantages are needed");
     Tensor* loss = new_tensor(Shape{1, 2}, logits->requires_grad, false);
+    float* scratch = (float*)arena_->alloc(M * 3 * sizeof(float));
     Op* o = new_op(OpType::PolicyLoss, {logits, old, advantages}, loss);
     o->targets = const_cast<int32_t*>(dev_targets);
     o->ref = ref ? ref->data : nullptr;
     o->weights = weights ? weights->data : nullptr;
     o->policy = args;
     o->arena = arena_;
-    o->scratch = (float*)arena_->alloc(M * 3 * sizeof(float));
-    o->forward();
+    o->scratch = scratch;
+    first_run(o);
     return loss;
 }
 
@@ -446,17 +467,18 @@ Tensor* Graph::preferenceLoss(Tensor* logp, Tensor* ref, const int32_t* dev_targ
     if (M == 0 || M > 0x7fffffff) throw Error(ZNN_ERR_INVALID, "preferenceLoss: between 1 and 2^31 - 1 rows are needed");
     if (ref && ref->numel() != M) throw Error(ZNN_ERR_INVALID, "preferenceLoss: ref needs one value per row");
     Tensor* loss = new_tensor(Shape{1, 1}, logp->requires_grad, false);
+    const size_t n = 3 * (size_t)pairs + M;
+    float* scratch = (float*)arena_->alloc(n * sizeof(float));
+    check(znn_memset(scratch, 0, n * sizeof(float)), "znn_memset");   // rows of no sequence keep a gradient of 0
     Op* o = new_op(OpType::PreferenceLoss, {logp}, loss);
     o->targets = const_cast<int32_t*>(dev_targets);
     o->offsets = dev_offsets;
     o->ref = ref ? ref->data : nullptr;
     o->pairs = pairs;
     o->preference = args;
-    const size_t n = 3 * (size_t)pairs + M;
-    o->scratch = (float*)arena_->alloc(n * sizeof(float));
-    check(znn_memset(o->scratch, 0, n * sizeof(float)), "znn_memset");   // rows of no sequence keep a gradient of 0
+    o->scratch = scratch;
     if (rewards) *rewards = o->scratch + pairs;
-    o->forward();
+    first_run(o);
     return loss;
 }
 
@@ -707,8 +729,8 @@ void Op::forward()
     case OpType::PolicyLoss: {
         // One pass makes the loss and the gradient: it goes where it belongs at once, unless something is there already.
         const bool store = A->grad && grad_is_fresh(A);
-        if (store) grad_root(A)->grad_stored_by = this;
         policy_loss(store ? A->grad : nullptr);
+        if (store) grad_root(A)->grad_stored_by = this;
         break;
     }
     case OpType::PreferenceLoss: {

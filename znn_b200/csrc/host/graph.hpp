@@ -251,6 +251,7 @@ public:
 private:
     Tensor* new_tensor(const Shape& shape, bool requires_grad, bool zero_data);
     Op* new_op(OpType type, std::initializer_list<Tensor*> inputs, Tensor* out);
+    void first_run(Op* o);   // forward of the op just made, which leaves the tape again where that is refused
     void sweep(Tensor* root, const std::function<void(Op*)>* after_op);
     Arena* arena_;
     std::vector<Tensor*> tensors_;
