@@ -123,3 +123,18 @@ def test_arrays_of_the_wrong_size():
     for f in bad:
         with pytest.raises(ValueError):
             f()
+
+
+def test_values_that_are_no_32_bit_integers():
+    """The numpy front end: targets and offsets are refused, not wrapped around to other tokens and rows."""
+    import numpy as np
+    from znn_b200 import ops
+    x, v = np.zeros((4, 7), np.float32), np.zeros(4, np.float32)
+    for bad in ([0, 1, 2, 2 ** 32 + 1], [0, 1, 2, -2 ** 31 - 1], [0, 1, 2, 2.5], [0, 1, 2, np.nan], [0, 1, 2, np.inf]):
+        for f in (lambda: ops.token_logprob_fwd(x, np.array(bad)), lambda: ops.token_logprob_bwd(x, np.array(bad), np.zeros((4, 2)), v),
+                  lambda: ops.policy_loss(x, np.array(bad), v, v), lambda: ops.preference_loss(v, [0, 2, 4], None, np.array(bad)),
+                  lambda: ops.preference_loss(v, np.array([0, 2, 2 ** 32 + 4]))):
+            with pytest.raises(ValueError, match="32-bit"):
+                f()
+    np.testing.assert_array_equal(ops.int32_array("t", np.array([[1, -2 ** 31], [2 ** 31 - 1, -7]])), np.array([[1, -2 ** 31], [2 ** 31 - 1, -7]], np.int32))
+    np.testing.assert_array_equal(ops.int32_array("t", [1.0, -3.0]), np.array([1, -3], np.int32))

@@ -74,3 +74,25 @@ def test_a_refused_op_leaves_the_tape(ops, G):
             n += 1
     assert g.num_ops() == n
     g.forward()
+
+
+def test_integers_of_graph_ops_and_models(ops, G):
+    """Targets and row numbers travel as doubles: what is no 32-bit integer is refused, not cast to a row that is left out."""
+    from znn_b200._lib import ZnnError
+    from znn_b200.models import Model
+    x, t, old, adv, _ = case(13, M=6)
+    g = G()
+    X, o, a = g.array(x, True), g.array(old), g.array(adv)
+    L = g.tokenLogProb(X, t)
+    for bad in (3e9, -3e9, 1.5, np.nan, np.inf):
+        b = list(t[:-1]) + [bad]
+        for f in (lambda: g.tokenLogProb(X, b), lambda: g.policyLoss(X, b, o, a), lambda: g.preferenceLoss(L, [0, 3, 6], None, b), lambda: g.preferenceLoss(L, [0, 3, bad])):
+            with pytest.raises(ZnnError, match="32-bit integer"):
+                f()
+    m = Model("gpt", (67, 24, 32, 2, 1), arena_bytes=64 << 20)
+    ids = np.zeros((2, 5), np.float32)
+    wide = np.full((2, 5), 2 ** 32 + 3)
+    for f in (lambda: m.token_logprobs(ids, wide), lambda: m.policy_step(ids, wide, ids, ids), lambda: m.preference_step(ids, wide)):
+        with pytest.raises(ValueError, match="32-bit"):
+            f()
+    assert np.all(m.token_logprobs(ids, np.full((2, 5), 3)) < 0)

@@ -48,13 +48,17 @@ static Shape shape_from(const long long* dims, int rank)
     return Shape(d, (size_t)rank);
 }
 
-// args[from .. n_args) as int32 in the graph's arena; there must be `want` of them
+// args[from .. n_args) as int32 in the graph's arena; there must be `want` of them, and each must be one
 static const int32_t* upload_ints(znn_graph* zg, const std::string& op, const double* args, int from, int n_args, size_t want)
 {
     if (n_args < from || (size_t)(n_args - from) != want)
         throw Error(ZNN_ERR_INVALID, op + ": " + std::to_string(want) + " integers expected, " + std::to_string(n_args - from) + " given");
     std::vector<int32_t> v(want);
-    for (size_t i = 0; i < want; i++) v[i] = (int32_t)args[from + i];
+    for (size_t i = 0; i < want; i++) {
+        const double a = args[from + i];
+        if (!(a >= -2147483648.0 && a <= 2147483647.0) || a != floor(a)) throw Error(ZNN_ERR_INVALID, op + ": " + std::to_string(a) + " is not a 32-bit integer");
+        v[i] = (int32_t)a;
+    }
     int32_t* dev = (int32_t*)zg->arena->alloc(want * sizeof(int32_t));
     check(znn_memcpy_h2d(dev, v.data(), want * sizeof(int32_t)), "upload integers");
     check(znn_sync(), "znn_sync");
@@ -164,7 +168,7 @@ int znn_graph_op(znn_graph* zg, const char* name, const int* inputs, int n_input
         a.margin = (float)arg(2);
         a.length_normalize = arg(3) != 0.0;
         const double pairs = arg(4);
-        if (!(pairs >= 1.0 && pairs < 1e9)) throw Error(ZNN_ERR_INVALID, "preferenceLoss: at least one pair is needed");
+        if (!(pairs >= 1.0 && pairs < 1e9) || pairs != floor(pairs)) throw Error(ZNN_ERR_INVALID, "preferenceLoss: at least one pair is needed");
         const int n_off = 2 * (int)pairs + 1, rest = n_args - 5 - n_off;
         const int32_t* offsets = upload_ints(zg, op, args, 5, n_args - (rest > 0 ? rest : 0), (size_t)n_off);
         const int32_t* targets = rest > 0 ? upload_ints(zg, op, args, 5 + n_off, n_args, in(0)->numel()) : nullptr;

@@ -6,6 +6,7 @@ import ctypes as C
 import numpy as np
 
 from ._lib import lib
+from .ops import int32_array
 
 KINDS = {"mlp": 1, "cnn_ref": 2, "cnn_padded": 3, "block": 4, "gpt": 5}
 
@@ -101,7 +102,7 @@ class Model:
     def token_logprobs(self, ids, targets, inv_temp=1.0, want_entropy=False):
         """Log-probabilities [batch, seq] of the targets (negative = left out), and their entropies where asked for."""
         ids = np.ascontiguousarray(ids, np.float32)
-        t = np.ascontiguousarray(targets, np.int32)
+        t = int32_array("targets", targets)
         assert ids.shape == t.shape and ids.ndim == 2, (ids.shape, t.shape)
         lp = np.empty(ids.shape, np.float32)
         en = np.empty(ids.shape, np.float32) if want_entropy else None
@@ -113,7 +114,7 @@ class Model:
                     entropy_coef=0.0, inv_temp=1.0):
         """One training step on the clipped policy loss; every array is [batch, seq].  Returns the loss."""
         ids = np.ascontiguousarray(ids, np.float32)
-        t = np.ascontiguousarray(targets, np.int32)
+        t = int32_array("targets", targets)
         cols = [None if a is None else np.ascontiguousarray(a, np.float32) for a in (old_logp, ref_logp, advantages, weights)]
         assert ids.ndim == 2 and all(a is None or a.shape == ids.shape for a in [t] + cols)
         loss = C.c_float()
@@ -125,7 +126,7 @@ class Model:
         """One training step on the preference loss; ids, targets and ref_logp are [2 * pairs, seq], preferred sequences in the even rows.
         Returns (loss, rewards [pairs, 2])."""
         ids = np.ascontiguousarray(ids, np.float32)
-        t = np.ascontiguousarray(targets, np.int32)
+        t = int32_array("targets", targets)
         ref = None if ref_logp is None else np.ascontiguousarray(ref_logp, np.float32)
         assert ids.ndim == 2 and ids.shape[0] % 2 == 0 and t.shape == ids.shape and (ref is None or ref.shape == ids.shape)
         loss, rewards = C.c_float(), np.empty((ids.shape[0] // 2, 2), np.float32)

@@ -628,6 +628,18 @@ def _sizes(n, **arrays):
             raise ValueError(f"{name} has {np.size(a)} values, {n} are needed")
 
 
+def int32_array(name, a):
+    """The integers of `a` as int32; values that are none are refused, not wrapped around to another token or row."""
+    if a is None:
+        return None
+    a = np.asarray(a)
+    with np.errstate(invalid="ignore"):
+        out = a.astype(np.int32)
+    if a.size and not np.array_equal(out, a):
+        raise ValueError(f"{name} holds values that are not 32-bit integers")
+    return np.ascontiguousarray(out)
+
+
 def _matrix(logits):
     logits = _f(logits)
     if logits.ndim != 2:
@@ -640,6 +652,7 @@ def token_logprob_fwd(logits, targets, inv_temp=1.0, want_entropy=True):
     logits = _matrix(logits)
     M, N = logits.shape
     _sizes(M, targets=targets)
+    targets = int32_array("targets", targets)
     _ensure()
     x, t = _up(logits), _up(targets, np.int32)
     lp, st = DevBuf(M * 4), DevBuf(M * 8)
@@ -655,6 +668,7 @@ def token_logprob_bwd(logits, targets, stats, dlogp, dlogits=None, entropy=None,
     _sizes(M, targets=targets, dlogp=dlogp, entropy=entropy, dentropy=dentropy)
     _sizes(2 * M, stats=stats)
     _sizes(M * N, dlogits=dlogits)
+    targets = int32_array("targets", targets)
     _ensure()
     x, t, st, g = _up(logits), _up(targets, np.int32), _up(stats), _up(dlogp)
     en, h = _up(entropy), _up(dentropy)
@@ -673,6 +687,7 @@ def policy_loss(logits, targets, old_logp, advantages, ref_logp=None, weights=No
     logits = _matrix(logits)
     M, N = logits.shape
     _sizes(M, targets=targets, old_logp=old_logp, advantages=advantages, ref_logp=ref_logp, weights=weights)
+    targets = int32_array("targets", targets)
     _ensure()
     x, t, old, adv = _up(logits), _up(targets, np.int32), _up(old_logp), _up(advantages)
     ref, w = _up(ref_logp), _up(weights)
@@ -693,6 +708,7 @@ def preference_loss(logp, seq_offsets, ref_logp=None, targets=None, beta=0.1, la
     M, P = logp.size, (len(seq_offsets) - 1) // 2
     _sizes(2 * P + 1, seq_offsets=seq_offsets)
     _sizes(M, ref_logp=ref_logp, targets=targets, dlogp=dlogp)
+    targets, seq_offsets = int32_array("targets", targets), int32_array("seq_offsets", seq_offsets)
     _ensure()
     lp, ref, t, off = _up(logp), _up(ref_logp), _up(targets, np.int32), _up(seq_offsets, np.int32)
     loss, pl, rw = DevBuf(4), DevBuf(P * 4), DevBuf(2 * P * 4)
