@@ -138,3 +138,21 @@ def test_values_that_are_no_32_bit_integers():
                 f()
     np.testing.assert_array_equal(ops.int32_array("t", np.array([[1, -2 ** 31], [2 ** 31 - 1, -7]])), np.array([[1, -2 ** 31], [2 ** 31 - 1, -7]], np.int32))
     np.testing.assert_array_equal(ops.int32_array("t", [1.0, -3.0]), np.array([1, -3], np.int32))
+
+
+def test_arrays_that_cannot_be_written_in_place():
+    """The numpy front end copies a result's bytes over such an array: another type, a view with gaps or a read-only one is refused."""
+    import numpy as np
+    from znn_b200 import ops
+    v, x, t, st = np.zeros(4, np.float32), np.zeros((4, 6), np.float32), np.zeros(4, np.int32), np.zeros((4, 2), np.float32)
+    fixed = v.copy()
+    fixed.flags.writeable = False
+    for bad in (np.zeros(4), np.zeros(8, np.float32)[::2], np.zeros(4, np.float16), fixed, [0.0] * 4):
+        for f in (lambda: ops.clip_grads([v, bad], 1.0), lambda: ops.sgd_step_clipped(bad, v, None, 0.1, 0.0, 1.0),
+                  lambda: ops.sgd_step_clipped(v, v, bad, 0.1, 0.9, 1.0), lambda: ops.adam_step_clipped(bad, v, v, v, 0.1, 0.9, 0.9, 1e-8, 1.0, 1.0),
+                  lambda: ops.adam_step_clipped(v, v, bad, v, 0.1, 0.9, 0.9, 1e-8, 1.0, 1.0), lambda: ops.adam_step_clipped(v, v, v, bad, 0.1, 0.9, 0.9, 1e-8, 1.0, 1.0)):
+            with pytest.raises(ValueError, match="in place"):
+                f()
+    for bad in (np.zeros((4, 6)), np.zeros((6, 4), np.float32).T, np.zeros((4, 12), np.float32)[:, ::2]):
+        with pytest.raises(ValueError, match="in place"):
+            ops.token_logprob_bwd(x, t, st, v, dlogits=bad)

@@ -628,6 +628,13 @@ def _sizes(n, **arrays):
             raise ValueError(f"{name} has {np.size(a)} values, {n} are needed")
 
 
+def _in_place(**arrays):
+    """Refuses arrays that a result cannot be written into as they are: float32, one piece of memory, writable."""
+    for name, a in arrays.items():
+        if a is not None and not (isinstance(a, np.ndarray) and a.dtype == np.float32 and a.flags.c_contiguous and a.flags.writeable):
+            raise ValueError(f"{name} is changed in place and has to be a writable, contiguous float32 array")
+
+
 def int32_array(name, a):
     """The integers of `a` as int32; values that are none are refused, not wrapped around to another token or row."""
     if a is None:
@@ -668,6 +675,7 @@ def token_logprob_bwd(logits, targets, stats, dlogp, dlogits=None, entropy=None,
     _sizes(M, targets=targets, dlogp=dlogp, entropy=entropy, dentropy=dentropy)
     _sizes(2 * M, stats=stats)
     _sizes(M * N, dlogits=dlogits)
+    _in_place(dlogits=dlogits)
     targets = int32_array("targets", targets)
     _ensure()
     x, t, st, g = _up(logits), _up(targets, np.int32), _up(stats), _up(dlogp)
@@ -724,7 +732,7 @@ GRAD_NORM_FLOATS = 4096
 def _grad_set(arrays):
     bufs = [_up(a) for a in arrays]
     ptrs = (C.c_void_p * max(1, len(bufs)))(*[b.ptr for b in bufs])
-    counts = (C.c_size_t * max(1, len(bufs)))(*[a.size for a in arrays])
+    counts = (C.c_size_t * max(1, len(bufs)))(*[np.size(a) for a in arrays])
     return bufs, ptrs, counts
 
 
@@ -740,6 +748,8 @@ def grad_norm(grads, max_norm=float("inf"), grad_scale=1.0):
 
 def clip_grads(grads, max_norm, grad_scale=1.0):
     """Clips the gradient arrays in place by their global norm; returns (norm before, factor)."""
+    for i, a in enumerate(grads):
+        _in_place(**{f"gradient {i}": a})
     _ensure()
     bufs, ptrs, counts = _grad_set(grads)
     res = DevBuf(GRAD_NORM_FLOATS * 4)
@@ -753,6 +763,7 @@ def clip_grads(grads, max_norm, grad_scale=1.0):
 
 def sgd_step_clipped(w, g, v, lr, momentum, max_norm, grad_scale=1.0):
     """One SGD step on w (and v), in place, with the gradient clipped to max_norm; returns (norm, factor)."""
+    _in_place(w=w, v=v)
     _sizes(w.size, g=g, v=v)
     _ensure()
     dw, dv = _up(w), _up(v)
@@ -769,6 +780,7 @@ def sgd_step_clipped(w, g, v, lr, momentum, max_norm, grad_scale=1.0):
 
 def adam_step_clipped(w, g, m, v, lr, beta1, beta2, eps, t, max_norm, grad_scale=1.0):
     """One Adam step on w, m, v, in place, with the gradient clipped to max_norm; returns (norm, factor)."""
+    _in_place(w=w, m=m, v=v)
     _sizes(w.size, g=g, m=m, v=v)
     _ensure()
     dw, dm, dv = _up(w), _up(m), _up(v)
