@@ -380,8 +380,9 @@ int znn_adam_step(float* w, const float* g, float* m, float* v, float lr, float 
  * be unaligned to 16 bytes) and counts (host array, floats per tensor; 0 is allowed) describe the set; both are read during
  * the call.
  * znn_grad_norm: result[0] = |grad_scale| * sqrt(sum of all squares), result[1] = the factor that brings it to max_norm:
- *   max_norm / norm where norm > max_norm, 1 otherwise, 0 where the norm is not finite.  Squares are summed in fp64 in a fixed
- *   order: no overflow or underflow for any finite fp32 gradients, and the same bits every time.  max_norm = INFINITY: the
+ *   max_norm / norm where norm > max_norm (at least fp32's smallest number), 1 otherwise, 0 where the norm is not finite.  Squares
+ *   are summed in fp64 in a fixed order: no overflow or underflow for any finite fp32 gradients (a norm above fp32's largest number
+ *   reads as inf in result[0], the factor is right all the same), and the same bits every time.  max_norm = INFINITY: the
  *   norm alone.  `result` is ZNN_GRAD_NORM_FLOATS floats of device memory, 16-byte aligned; what follows the two values is the
  *   call's workspace.  Give calls that may run at the same time (two streams, two captured graphs) a result each.
  *   A tensor that is listed twice counts twice.

@@ -230,3 +230,22 @@ def test_gradient_of_nearly_certain_rows(ops, L, N, entropy, accumulate, in_plac
     if accumulate:
         want = want + before
     within(got, want, tol + U * np.abs(want), "dlogits")
+
+
+# ------------------------------------------------------------------ norms beyond any bound
+@pytest.mark.parametrize("n", [5, 5000, 2000003])
+def test_a_factor_below_fp32_is_not_a_skipped_step(ops, n):
+    """A finite norm so far above the bound that their quotient is below fp32: the gradients are clipped (by the smallest factor there
+    is), not left as they are as if the norm were not finite."""
+    value = np.float32(3e38)
+    for big in (1, n):                                   # a norm within fp32, and one beyond it
+        g = np.zeros(n, np.float32)
+        g[:big] = value
+        norm = float(value) * np.sqrt(big)
+        got = ops.clip_grads([g], 1e-20)
+        assert got[0] == np.float32(norm) if norm < 3.4e38 else got[0] == INF
+        assert 0 < got[1] <= 2.0 ** -149
+        np.testing.assert_array_equal(g[:big], value * got[1])
+        w = np.full(n, 0.5, np.float32)
+        ops.sgd_step_clipped(w, np.where(np.arange(n) < big, value, 0).astype(np.float32), None, 1.0, 0.0, 1e-20)
+        assert np.all(w[:big] < 0.5) and np.all(np.isfinite(w))

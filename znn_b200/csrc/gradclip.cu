@@ -126,7 +126,8 @@ __device__ __forceinline__ void write_result(double sum, float grad_scale, float
 {
     const double norm = fabs((double)grad_scale) * sqrt(sum);
     result[0] = (float)norm;
-    result[1] = !isfinite(norm) ? 0.0f : norm > (double)max_norm ? (float)((double)max_norm / norm) : 1.0f;
+    // (a factor that fp32 would round to 0 is its smallest number: 0 says that there is no finite norm)
+    result[1] = !isfinite(norm) ? 0.0f : norm > (double)max_norm ? fmaxf((float)((double)max_norm / norm), 1.4e-45f) : 1.0f;
 }
 
 // partial[block] (+)= squares of the block's tiles
