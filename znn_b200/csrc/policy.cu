@@ -170,13 +170,13 @@ __device__ __forceinline__ RowHead row_head(const RowParams& p, unsigned row, bo
 }
 
 // The scalars of one row from its sums (one thread): writes logp, entropy, stats, token_loss (where `write`), returns the
-// gradient's coefficients for a walk over logits measured from `from`.  The log-probability, and the differences that ratio and
+// gradient's coefficients.  The log-probability, and the differences that ratio and
 // KL term are made of, are fp64: fp32 would leave a ratio of two probabilities of e^-10 an error of 1e-6.  What follows from
 // them is fp32: products, and the KL term, which is kept from cancelling.  (In short rows these few hundred operations of one lane are
 // most of the work.)
 template <bool Policy, bool Entropy>
 __device__ __forceinline__ RowGrad row_scalars(const RowParams& p, int row, const RowSums& r, const RowHead& in, float x_t, int rows,
-                                               bool write, float from)
+                                               bool write)
 {
     const float total = r.ties + r.s, inv_total = 1.0f / total;
     const bool empty = total == 0.0f;
@@ -192,7 +192,7 @@ __device__ __forceinline__ RowGrad row_scalars(const RowParams& p, int row, cons
             p.stats[2 * (size_t)row + 1] = total;
         }
     }
-    RowGrad g{0.0f, 0.0f, 0.0f, from};
+    RowGrad g{0.0f, 0.0f, 0.0f, r.mx};
     if (Policy) {
         const float A = in.advantage;
         float loss = 0.0f, slope = 0.0f;
@@ -229,10 +229,9 @@ __device__ __forceinline__ RowGrad row_scalars(const RowParams& p, int row, cons
             const float top = base_of(r.mx), e_t = x_t == top ? 1.0f : exp2_fast(fmaxf((x_t - top) * p.c, kNothing));
             const float others = (x_t == top ? r.ties - 1.0f + r.s : total - e_t) * inv_total;
             g.at_target = (others == 0.0f ? 0.0f : G * others) - (Entropy && e_t > 0.0f ? E * e_t * inv_total * ((float)logp + H) : 0.0f);
-            // p_j (-G - E (log p_j + H)),  p_j = 2^(t + delta) / s,  log p_j + H = log(2) (t + delta) - U
-            const float delta = from == r.mx ? 0.0f : fmaxf((from - r.mx) * p.c, kNothing), inv = exp2_fast(delta) * inv_total;
-            g.a = inv * (-G - (Entropy ? E * (kLn2 * delta - U) : 0.0f));
-            g.b = Entropy ? -inv * E * kLn2 : 0.0f;
+            // p_j (-G - E (log p_j + H)),  p_j = 2^t / s,  log p_j + H = log(2) t - U
+            g.a = inv_total * (-G + (Entropy ? E * U : 0.0f));
+            g.b = Entropy ? -inv_total * E * kLn2 : 0.0f;
         }
     }
     return g;
@@ -438,7 +437,7 @@ __device__ __forceinline__ void exchange(RowWord* word, const RowSums& mine, int
 // 5.5 TB/s, 1000000 x 100: 283 us, 2.9 TB/s (369 with one row at a time): the rows' scalars and reductions show, the more the shorter
 // the rows are.
 template <bool Policy, bool Entropy, bool Aligned, int Group, int V, int Rows>
-__global__ void __launch_bounds__(128) rows_held_kernel(const RowParams p, int)
+__global__ void __launch_bounds__(128) rows_held_kernel(const RowParams p)
 {
     static_assert(Rows <= Group, "a lane makes the scalars of one row");
     const int tid = threadIdx.x % Group;
@@ -501,7 +500,7 @@ __global__ void __launch_bounds__(128) rows_held_kernel(const RowParams p, int)
     }
     RowGrad g{};
     if (there) {
-        if (used) g = row_scalars<Policy, Entropy>(p, mine, own, in, x_t, rows, true, own.mx);
+        if (used) g = row_scalars<Policy, Entropy>(p, mine, own, in, x_t, rows, true);
         else row_unused<Policy>(p, mine, in.t >= p.N && in.w != 0.0f);
     }
     if (!Policy || !p.dlogits) return;
@@ -619,7 +618,7 @@ __global__ void __launch_bounds__(Threads) rows_walk_kernel(const RowParams p, i
             int rows = 0;
             if (Policy && !p.weights && !p.count)
                 for (int i = 0; i < kWarps; i++) rows += sh_rows[i];
-            sh_grad = row_scalars<Policy, Entropy>(p, row, sums, in, x_t, rows, rank == 0, sums.mx);
+            sh_grad = row_scalars<Policy, Entropy>(p, row, sums, in, x_t, rows, rank == 0);
         }
     }
     if (!dx) return;
@@ -1117,8 +1116,7 @@ template <bool Policy, bool Entropy, bool Aligned, int Group, int V, int Rows>
 static int launch_held(const RowParams& p)
 {
     constexpr int rows = 128 / Group * Rows;
-    return launch(rows_held_kernel<Policy, Entropy, Aligned, Group, V, Rows>, "rows_held_kernel", (p.M + (long long)rows - 1) / rows, 128, 1,
-                  p, 0);
+    return launch(rows_held_kernel<Policy, Entropy, Aligned, Group, V, Rows>, "rows_held_kernel", (p.M + (long long)rows - 1) / rows, 128, 1, p);
 }
 
 template <bool Policy, bool Entropy, bool Aligned, int Threads>
