@@ -249,3 +249,28 @@ def test_a_factor_below_fp32_is_not_a_skipped_step(ops, n):
         w = np.full(n, 0.5, np.float32)
         ops.sgd_step_clipped(w, np.where(np.arange(n) < big, value, 0).astype(np.float32), None, 1.0, 0.0, 1e-20)
         assert np.all(w[:big] < 0.5) and np.all(np.isfinite(w))
+
+
+# ------------------------------------------------------------------ the policy loss that makes no entropies
+class WithoutEntropies:
+    """ops, with policy losses as a step without an entropy term calls them: no buffer for entropies.  Those that the caller compares
+    come from a call of their own."""
+
+    def __init__(self, ops):
+        self.ops = ops
+
+    def policy_loss(self, *args, **kw):
+        out = self.ops.policy_loss(*args, want_entropy=False, **kw)
+        assert out["entropy"] is None
+        kw["want_grad"] = False
+        out["entropy"] = self.ops.policy_loss(*args, **kw)["entropy"]
+        return out
+
+
+MANY = [(450, 1100), (520, 1501), (450, 2000), (451, 2100), (450, 2900), (450, 5121), (447, 6000), (450, 9001), (450, 12500), (300, 51300), (160, 110000)]
+
+
+@pytest.mark.parametrize("M,N", base.SHAPES + MANY)
+@pytest.mark.parametrize("kl,weighted,inv_temp", [(0.0, False, 1.0), (0.05, False, 1.25), (0.1, True, 0.7)])
+def test_policy_loss_without_entropies(ops, M, N, kl, weighted, inv_temp):
+    base.test_policy_loss(WithoutEntropies(ops), M, N, kl, 0.0, weighted, inv_temp)

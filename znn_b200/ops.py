@@ -690,8 +690,9 @@ def token_logprob_bwd(logits, targets, stats, dlogp, dlogits=None, entropy=None,
 
 
 def policy_loss(logits, targets, old_logp, advantages, ref_logp=None, weights=None, clip=(0.2, 0.2), kl_coef=0.0,
-                entropy_coef=0.0, inv_temp=1.0, want_grad=True):
-    """Clipped policy loss: dict with loss, rows, token_loss[M], logp[M], entropy[M] and dlogits[M, N] (None without want_grad)."""
+                entropy_coef=0.0, inv_temp=1.0, want_grad=True, want_entropy=True):
+    """Clipped policy loss: dict with loss, rows, token_loss[M], logp[M], entropy[M] (None without want_entropy) and dlogits[M, N] (None
+    without want_grad)."""
     logits = _matrix(logits)
     M, N = logits.shape
     _sizes(M, targets=targets, old_logp=old_logp, advantages=advantages, ref_logp=ref_logp, weights=weights)
@@ -699,13 +700,13 @@ def policy_loss(logits, targets, old_logp, advantages, ref_logp=None, weights=No
     _ensure()
     x, t, old, adv = _up(logits), _up(targets, np.int32), _up(old_logp), _up(advantages)
     ref, w = _up(ref_logp), _up(weights)
-    loss, tl, lp, en = DevBuf(8), DevBuf(M * 4), DevBuf(M * 4), DevBuf(M * 4)
+    loss, tl, lp, en = DevBuf(8), DevBuf(M * 4), DevBuf(M * 4), DevBuf(M * 4) if want_entropy else None
     dx = DevBuf(logits.nbytes) if want_grad else None
     lib().call("znn_policy_loss", x.ptr, N, t.ptr, inv_temp, old.ptr, _ptr(ref), adv.ptr, _ptr(w), clip[0], clip[1], kl_coef,
-               entropy_coef, loss.ptr, tl.ptr, lp.ptr, en.ptr, _ptr(dx), N, M, N)
+               entropy_coef, loss.ptr, tl.ptr, lp.ptr, _ptr(en), _ptr(dx), N, M, N)
     both = loss.to_host((2,))
     return {"loss": both[0], "rows": int(both[1]), "token_loss": tl.to_host((M,)), "logp": lp.to_host((M,)),
-            "entropy": en.to_host((M,)), "dlogits": dx.to_host((M, N)) if want_grad else None}
+            "entropy": en.to_host((M,)) if want_entropy else None, "dlogits": dx.to_host((M, N)) if want_grad else None}
 
 
 def preference_loss(logp, seq_offsets, ref_logp=None, targets=None, beta=0.1, label_smoothing=0.0, margin=0.0,
