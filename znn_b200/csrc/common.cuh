@@ -67,6 +67,11 @@ void count_launch();
         if (!(cond)) return ::znn::fail(ZNN_ERR_INVALID, __VA_ARGS__);                 \
     } while (0)
 
+#define ZNN_NEED_DEVICE()                                                                                              \
+    do {                                                                                                               \
+        if (!::znn::stream()) return ::znn::fail(ZNN_ERR_CUDA, "no CUDA device state; call znn_init (no CPU fallback)"); \
+    } while (0)
+
 static inline int ceil_div(long a, long b) { return (int)((a + b - 1) / b); }
 
 }  // namespace znn

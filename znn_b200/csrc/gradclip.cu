@@ -12,7 +12,7 @@
 #include <utility>
 #include <vector>
 
-#include "common.cuh"
+#include "overlap.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -34,22 +34,6 @@ struct TensorTable {
     int n;
 };
 constexpr int kSmallTable = 16, kMiddleTable = 200, kLargeTable = 1000;
-
-// returns when the kernel before this one on the stream has ended and what it wrote can be read
-__device__ __forceinline__ void wait_for_previous_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-
-__device__ __forceinline__ double block_sum(double v, double* sh)
-{
-    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, nw = blockDim.x >> 5;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    __syncthreads();
-    if (lane == 0) sh[w] = v;
-    __syncthreads();
-    double t = 0.0;
-    for (int i = 0; i < nw; i++) t += sh[i];
-    return t;
-}
 
 // The floats of one tile: whole 16-byte quads, kNormQuads per thread, and up to three floats before and after them, one each for
 // a few threads, since a tensor may start at any float.
@@ -286,30 +270,6 @@ adam_clipped_kernel(float* __restrict__ w, const float* __restrict__ g, float* _
 
 using namespace znn;
 
-#define ZNN_NEED_DEVICE()                                                                                  \
-    do {                                                                                                   \
-        if (!stream()) return fail(ZNN_ERR_CUDA, "no CUDA device state; call znn_init (no CPU fallback)"); \
-    } while (0)
-
-// Every kernel here may begin while the one before it on the stream ends, and waits before it does anything: the launch itself then
-// costs no time between them (norm and Adam step of 2 million floats: 15.0 us a call, 18.7 without).
-template <class... Params, class... Args>
-static int launch(void (*kernel)(Params...), const char* name, size_t blocks, int threads, const Args&... args)
-{
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)blocks);
-    cfg.blockDim = dim3(threads);
-    cfg.stream = stream();
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    ZNN_CUDA_OK(cudaLaunchKernelEx(&cfg, kernel, args...));
-    ZNN_LAUNCH_OK(name);
-    return ZNN_OK;
-}
-
 static int check_set(const void* grads, const size_t* counts, int n, const float* const* ptrs)
 {
     ZNN_REQUIRE(n >= 0, "n is negative");
@@ -356,14 +316,14 @@ static int grad_norm(const float* const* grads, const size_t* counts, int n, flo
         const int tiles = t.first_tile[t.n];
         // one cluster where it has a few rounds at most: 645 thousand floats in six tensors take 10.1 us a call with it and 13.1 with two
         // launches, 1.5 million 16.7 and 13.4
-        if (used == 0 && at == n && tiles <= 96) return launch(norm_small_kernel<Cap>, "norm_small_kernel", 8, kNormThreads, t, grad_scale, max_norm, result);
+        if (used == 0 && at == n && tiles <= 96) return launch_overlapped(norm_small_kernel<Cap>, "norm_small_kernel", 8, kNormThreads, 1, t, grad_scale, max_norm, result);
         // the first launch writes every partial sum that a later one adds to
         const int grid = (at < n || used) ? blocks : std::min(blocks, tiles);
-        const int rc = launch(norm_partial_kernel<Cap>, "norm_partial_kernel", grid, kNormThreads, t, partial, used ? 1 : 0);
+        const int rc = launch_overlapped(norm_partial_kernel<Cap>, "norm_partial_kernel", grid, kNormThreads, 1, t, partial, used ? 1 : 0);
         if (rc != ZNN_OK) return rc;
         used = std::max(used, grid);
     }
-    return launch(norm_finish_kernel, "norm_finish_kernel", 1, kNormThreads, (const double*)partial, used, grad_scale, max_norm, result);
+    return launch_overlapped(norm_finish_kernel, "norm_finish_kernel", 1, kNormThreads, 1, (const double*)partial, used, grad_scale, max_norm, result);
 }
 
 template <int Cap>
@@ -372,7 +332,7 @@ static int clip_grads(float* const* grads, const size_t* counts, int n, const fl
     TensorTable<Cap> t;
     int at = 0;
     while (next_table(grads, counts, n, &at, &t)) {
-        const int rc = launch(clip_kernel<Cap>, "clip_kernel", std::min(t.first_tile[t.n], sm_count() * 4), kNormThreads, t, result);
+        const int rc = launch_overlapped(clip_kernel<Cap>, "clip_kernel", std::min(t.first_tile[t.n], sm_count() * 4), kNormThreads, 1, t, result);
         if (rc != ZNN_OK) return rc;
     }
     return ZNN_OK;
@@ -446,7 +406,7 @@ int znn_sgd_step_clipped(float* w, const float* g, float* v, float lr, float mom
     ZNN_REQUIRE(blocks, "n = %zu is too large", n);
     auto kernel = with_v ? (q ? sgd_clipped_kernel<true, true> : sgd_clipped_kernel<true, false>)
                          : (q ? sgd_clipped_kernel<false, true> : sgd_clipped_kernel<false, false>);
-    return launch(kernel, "sgd_clipped_kernel", blocks, kStepThreads, w, g, v, SgdStep{lr, momentum}, grad_scale, result, n);
+    return launch_overlapped(kernel, "sgd_clipped_kernel", blocks, kStepThreads, 1, w, g, v, SgdStep{lr, momentum}, grad_scale, result, n);
 }
 
 int znn_adam_step_clipped(float* w, const float* g, float* m, float* v, float lr, float beta1, float beta2, float eps, float t,
@@ -462,7 +422,7 @@ int znn_adam_step_clipped(float* w, const float* g, float* m, float* v, float lr
     const bool q = quads(w, g, m, v);
     const size_t blocks = step_blocks(n, q);
     ZNN_REQUIRE(blocks, "n = %zu is too large", n);
-    return launch(q ? adam_clipped_kernel<true> : adam_clipped_kernel<false>, "adam_clipped_kernel", blocks, kStepThreads, w, g, m, v,
+    return launch_overlapped(q ? adam_clipped_kernel<true> : adam_clipped_kernel<false>, "adam_clipped_kernel", blocks, kStepThreads, 1, w, g, m, v,
                   AdamStep{lr_t, beta1, beta2, eps}, grad_scale, result, n);
 }
 

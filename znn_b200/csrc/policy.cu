@@ -13,7 +13,7 @@
 
 #include <algorithm>
 
-#include "common.cuh"
+#include "overlap.cuh"
 #include "tc_ptx.cuh"
 
 namespace znn {
@@ -92,20 +92,6 @@ __device__ __forceinline__ RowSums join_lanes(const RowSums& v, float c, unsigne
     return r;
 }
 
-// sum over a block of up to 1024 threads in a fixed order, valid in every thread
-__device__ __forceinline__ double block_sum(double v, double* sh)
-{
-    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, nw = blockDim.x >> 5;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kAllLanes, v, o);
-    __syncthreads();
-    if (lane == 0) sh[w] = v;
-    __syncthreads();
-    double t = 0.0;
-    for (int i = 0; i < nw; i++) t += sh[i];
-    return t;
-}
-
 // log(ties + s) to about 4e-8, absolutely and (for sums near 1) relatively, with fp32's own logarithms: log1p() of s beside a
 // single one, and elsewhere the logarithm of the mantissa beside an exact power of two.
 __device__ __forceinline__ double log_of_sum(float ties, float s)
@@ -117,11 +103,8 @@ __device__ __forceinline__ double log_of_sum(float ties, float s)
     return (double)((bits >> 23) - 127) * 0.693147180559945309417 + (double)logf(__int_as_float((bits & 0x007fffff) | 0x3f800000)) + (total - total);
 }
 
-// Every kernel here may begin while the one before it on the stream ends, and waits here, before it reads or writes anything, for
-// that one's end and for what it wrote: the launch itself then costs no time between them.  (Rows of a policy loss that began
-// beside the kernel that counts them would save 2 us of 90, but nothing would promise that they see what ran before that one.)
-__device__ __forceinline__ void wait_for_previous_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-
+// Every kernel here may begin while the one before it on the stream ends (overlap.cuh).  (Rows of a policy loss that began beside the
+// kernel that counts them would save 2 us of 90, but nothing would promise that they see what ran before that one.)
 struct RowParams {
     const float* logits;
     long long ld;
@@ -1085,38 +1068,12 @@ __global__ void __launch_bounds__(1024) mean_kernel(const float* __restrict__ v,
 
 using namespace znn;
 
-#define ZNN_NEED_DEVICE()                                                                                  \
-    do {                                                                                                   \
-        if (!stream()) return fail(ZNN_ERR_CUDA, "no CUDA device state; call znn_init (no CPU fallback)"); \
-    } while (0)
-
 // ---- launches
-// A launch in clusters of `ranks` blocks that may begin while the kernel before it still runs.
-template <class... Params, class... Args>
-static int launch(void (*kernel)(Params...), const char* name, long long blocks, int threads, int ranks, Args... args)
-{
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)blocks);
-    cfg.blockDim = dim3(threads);
-    cfg.stream = stream();
-    cudaLaunchAttribute attrs[2] = {};
-    if (ranks > 1) {
-        attrs[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
-        attrs[cfg.numAttrs++].val.clusterDim = {(unsigned)ranks, 1, 1};
-    }
-    attrs[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attrs[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attrs;
-    ZNN_CUDA_OK(cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...));
-    ZNN_LAUNCH_OK(name);
-    return ZNN_OK;
-}
-
 template <bool Policy, bool Entropy, bool Aligned, int Group, int V, int Rows>
 static int launch_held(const RowParams& p)
 {
     constexpr int rows = 128 / Group * Rows;
-    return launch(rows_held_kernel<Policy, Entropy, Aligned, Group, V, Rows>, "rows_held_kernel", (p.M + (long long)rows - 1) / rows, 128, 1, p);
+    return launch_overlapped(rows_held_kernel<Policy, Entropy, Aligned, Group, V, Rows>, "rows_held_kernel", (p.M + (long long)rows - 1) / rows, 128, 1, p);
 }
 
 template <bool Policy, bool Entropy, bool Aligned, int Threads>
@@ -1127,10 +1084,10 @@ static int launch_walk(const RowParams& p, int ranks)
         // rows of a few steps: six quads a thread where those cover fewer columns that are not there (policy 60000 x 2100: 177 us with
         // six, 184 with eight; 60000 x 2000: 172 and 161; log-probabilities 65536 x 1100: 66 and 74)
         if (part <= 12288 && 6 * ceil_div(part, 24 * Threads) < 8 * ceil_div(part, 32 * Threads))
-            return launch(rows_walk_kernel<Policy, Entropy, Aligned, Threads, 6>, "rows_walk_kernel", (long long)p.M * ranks, Threads, ranks,
+            return launch_overlapped(rows_walk_kernel<Policy, Entropy, Aligned, Threads, 6>, "rows_walk_kernel", (long long)p.M * ranks, Threads, ranks,
                           p, part);
     }
-    return launch(rows_walk_kernel<Policy, Entropy, Aligned, Threads, 8>, "rows_walk_kernel", (long long)p.M * ranks, Threads, ranks,
+    return launch_overlapped(rows_walk_kernel<Policy, Entropy, Aligned, Threads, 8>, "rows_walk_kernel", (long long)p.M * ranks, Threads, ranks,
                   p, part);
 }
 
@@ -1202,7 +1159,7 @@ static int launch_bwd(const BwdArgs& b)
     constexpr int fit = 4 * Group * V;
     const int part = (ceil_div(b.N, ceil_div(b.N, fit)) + 3) & ~3, parts = ceil_div(b.N, part);
     const long long units = (long long)b.M * parts;
-    return launch(logprob_bwd_kernel<Accumulate, Aligned, Group, V>, "logprob_bwd_kernel", (units + rows - 1) / rows, Group < 256 ? 128 : Group, 1,
+    return launch_overlapped(logprob_bwd_kernel<Accumulate, Aligned, Group, V>, "logprob_bwd_kernel", (units + rows - 1) / rows, Group < 256 ? 128 : Group, 1,
                   b.logits, b.ld, b.targets, b.it, b.stats, b.entropy, b.dlogp, b.dentropy, b.dlogits, b.ld_d, b.M, b.N, parts, part);
 }
 
@@ -1291,12 +1248,12 @@ int znn_policy_loss(const float* logits, long long ld, const int32_t* targets, f
     const int total_ranks = M > 4096 ? 8 : 1;
     if (!weights && M > 512) {   // the rows' weight 1 / count is needed before their gradients are written
         p.count = loss + 1;
-        const int counted = launch(policy_total_kernel, "policy_total_kernel", total_ranks, 1024, total_ranks, targets, weights, token_loss, loss, M, 0);
+        const int counted = launch_overlapped(policy_total_kernel, "policy_total_kernel", total_ranks, 1024, total_ranks, targets, weights, token_loss, loss, M, 0);
         if (counted != ZNN_OK) return counted;
     }
     const int done = launch_rows<true>(p, entropy || entropy_coef != 0.0f);
     if (done != ZNN_OK) return done;
-    return launch(policy_total_kernel, "policy_total_kernel", total_ranks, 1024, total_ranks, targets, weights, token_loss, loss, M, 1);
+    return launch_overlapped(policy_total_kernel, "policy_total_kernel", total_ranks, 1024, total_ranks, targets, weights, token_loss, loss, M, 1);
 }
 
 int znn_preference_loss(const float* logp, const float* ref_logp, const int32_t* targets, const int32_t* seq_offsets, float beta,
@@ -1310,7 +1267,7 @@ int znn_preference_loss(const float* logp, const float* ref_logp, const int32_t*
     ZNN_REQUIRE(label_smoothing >= 0.0f && label_smoothing < 1.0f, "label_smoothing must lie in [0, 1)");
     ZNN_NEED_DEVICE();
 #define ZNN_PAIRS(small, threads, blocks, used, ranks)                                                                                    \
-    launch(preference_pair_kernel<small, threads>, "preference_pair_kernel", blocks, used, ranks, logp, ref_logp, targets, seq_offsets, \
+    launch_overlapped(preference_pair_kernel<small, threads>, "preference_pair_kernel", blocks, used, ranks, logp, ref_logp, targets, seq_offsets, \
            beta, label_smoothing, margin, length_normalize, loss, pair_loss, rewards, dlogp, P, M, device_status_word())
     // A warp per pair in one launch for small calls.  Few pairs of long sequences: eight blocks each, where one block's own bandwidth
     // (about 100 GB/s) would be the limit.  Many short ones: small blocks.
@@ -1322,7 +1279,7 @@ int znn_preference_loss(const float* logp, const float* ref_logp, const int32_t*
                                                        : ZNN_PAIRS(false, 64, P, 64, 1);
 #undef ZNN_PAIRS
     if (rc != ZNN_OK || P == 1) return rc;   // (a single pair's loss is the mean)
-    return launch(mean_kernel, "mean_kernel", 1, 1024, 1, (const float*)pair_loss, loss, P);
+    return launch_overlapped(mean_kernel, "mean_kernel", 1, 1024, 1, (const float*)pair_loss, loss, P);
 }
 
 }  // extern "C"

@@ -1299,11 +1299,6 @@ __global__ void accuracy_u8_kernel(const float* __restrict__ preds, const uint8_
 
 using namespace znn;
 
-#define ZNN_NEED_DEVICE()                                                                                  \
-    do {                                                                                                   \
-        if (!stream()) return fail(ZNN_ERR_CUDA, "no CUDA device state; call znn_init (no CPU fallback)"); \
-    } while (0)
-
 extern "C" {
 
 int znn_pixels_to_unit(const uint8_t* pixels, float* out, size_t n)
