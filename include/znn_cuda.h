@@ -270,8 +270,10 @@ int znn_softmax_xent_fwd_static(const float* logits, const int32_t* targets, flo
  *   - a logit of -inf switches its column off: p_j = 0, gradient 0, except that a target that is switched off (logp = -inf) still has
  *     the gradient of a p_t of 0.  A row of -inf alone has logp = -inf, entropy 0 and gradient 0; a row that holds NaN or +inf
  *     gives NaN;
- *   - sums of a row are kept in fp32 per thread and joined in a fixed order, per-row scalars and sums over rows in fp64:
- *     results do not depend on timing.  Nothing is kept in the library between calls.
+ *   - sums of a row are kept in fp32 per thread and joined in a fixed order; log-probabilities, the differences that ratio and KL
+ *     term are made of, everything of a preference pair and sums over rows are fp64, the other scalars of a row (ratio, KL term, slope,
+ *     loss, entropy, gradient coefficients) fp32: results do not depend on timing.  Nothing is kept in the library between calls;
+ *   - beside dlogits over the logits (below), no output may overlap another array of the call.
  *
  * znn_token_logprob_fwd: logp[M], entropy[M] (may be NULL) and stats[M][2] = (xm, s) (may be NULL), which the backward
  * needs; log sum exp = inv_temp * xm + log s.  Rows left out: stats = (0, 0).
@@ -309,7 +311,8 @@ int znn_policy_loss(const float* logits, long long ld, const int32_t* targets, f
  *   and the slopes are the limits; two of them in one pair have no difference: NaN.
  * dlogp (may be NULL) = d loss[0] / d logp for the rows of the sequences, 0 for those left out, which
  * znn_token_logprob_bwd takes; rows behind the last sequence stay as they were.  A pair whose offsets are not ascending within
- * 0 .. M has rewards and loss NaN, its rows are neither read nor written, and ZNN_DEV_BAD_INDEX is set. */
+ * 0 .. M has rewards and loss NaN, its rows are neither read nor written, and ZNN_DEV_BAD_INDEX is set; rows that two other pairs share
+ * because the offsets between them descend get the gradient of either. */
 int znn_preference_loss(const float* logp, const float* ref_logp, const int32_t* targets, const int32_t* seq_offsets, float beta,
                         float label_smoothing, float margin, int length_normalize, float* loss, float* pair_loss, float* rewards,
                         float* dlogp, int P, int M);

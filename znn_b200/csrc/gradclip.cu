@@ -3,7 +3,8 @@
 //
 // Bound by HBM: 4 bytes per gradient for the norm, 20 (SGD with momentum) or 28 (Adam) for a step.  Measured on a B200 whose copies
 // run at 6548 GB/s: norm of 98 million floats 61 us, 6.5 TB/s; Adam step on them 395 us, 6.8 TB/s of the 2.69 GB that cross HBM (the
-// gradients that the norm read last come from L2); both as called 470 us.
+// gradients that the norm read last come from L2); both as called 470 us.  Norm and SGD step of them 234 us, with momentum 355 (floors 180
+// and 300); clipping them in place 125 us, 6.3 TB/s, with the norm 196 (180); norm and clipping of six tensors, 109 thousand floats, 6.4 us.
 #include <cooperative_groups.h>
 #include <math.h>
 

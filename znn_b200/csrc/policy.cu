@@ -2,12 +2,12 @@
 // with its gradient, the preference loss on pairs of sequences.  Formulas: include/znn_cuda.h.
 //
 // Bound by HBM where there is enough to do (10 to 20 operations per logit against 4 to 12 bytes), by launch and reduction latency
-// where there is not.  Measured on a B200 whose copies run at 6548 GB/s, the whole call, inputs in turn from three sets:
-//   log-probabilities and entropies 2045 x 50257, a fifth left out  58 us  5.7 TB/s     (floor 50 us)
-//   their gradient with entropy term 8192 x 8192, a tenth left out  79 us  6.4 TB/s     (78 us)
-//   policy loss 8192 x 8192, KL term                                94 us  5.7 TB/s     (82 us)
-//   policy loss 2048 x 131000, KL and entropy, 0.15 left out       345 us  5.8 TB/s     (303 us)
-//   preference loss 700 pairs, 1.4 million rows                     12 us               (3.4 us: latency)
+// where there is not.  Measured on B200s whose copies run at 6548 GB/s, the whole call, inputs in turn from three sets, several boxes:
+//   log-probabilities and entropies 2045 x 50257, a fifth left out  57 - 62 us   5.3 - 5.7 TB/s   (floor 50 us)
+//   their gradient with entropy term 8192 x 8192, a tenth left out  78 - 79 us   6.4 TB/s         (78 us)
+//   policy loss 8192 x 8192, KL term                                94 - 96 us   5.7 TB/s         (82 us)
+//   policy loss 2048 x 131000, KL and entropy, 0.15 left out       340 - 370 us  5.4 - 5.8 TB/s   (303 us)
+//   preference loss 700 pairs, 1.4 million rows                     12 us                         (3.4 us: latency)
 #include <math.h>
 #include <math_constants.h>
 
@@ -510,7 +510,7 @@ __global__ void __launch_bounds__(128) rows_held_kernel(const RowParams p)
 
 // Longer rows: a block (or the blocks of a cluster, which take `part` columns each) walks over the row with running sums per thread,
 // and for the gradient a second time, back from the end, through the L2 cache: 8 bytes per logit cross HBM, not 12 (2048 x 131000:
-// 0.94 GB read, 1.02 GB written, 343 us).  Small blocks with few registers are what makes it fast: a row's chain of loads,
+// 0.94 GB read, 1.02 GB written, 343 us under the profiler).  Small blocks with few registers are what makes it fast: a row's chain of loads,
 // reductions and scalars takes microseconds, and enough other rows must be under way meanwhile.  Rows held in registers, by blocks
 // of 256 or 512 threads and clusters of them, took 580 us for the same, since too few blocks per SM hid too little of that chain
 // (copying the next row to shared memory ahead made it worse: 8192 x 8192 110 -> 138 us, where this form takes 94).
@@ -1101,6 +1101,8 @@ static int launch_walk(const RowParams& p, int ranks)
 //            1500 x 65536: 180 / 162 / 143 / 165,  700 x 131072: - / - / 152 / 136
 //   logprob  40000 x 2000: 54 / 66 / 105 / 220,  20000 x 4099: 54 / 55 / 58 / 117,  20000 x 5000: 62 / 67 / - / -,  4000 x 20000: - / 59 / 54 / 59,
 //            1000 x 100000: - / - / 66 / 67,  2045 x 50257 (1.7 times the blocks of 128 threads that are resident at once): - / 57 / 60 / 58
+// The loss alone (no dlogits) goes by the same rule, although it walks once: 8192 x 8192 56 us, 2048 x 131000 215, 40000 x 2600 87, where
+// the log-probabilities' sizes take 43, 164 and 73.
 // Few rows are spread over clusters, as many as let all blocks run at once: 32 x 131072 takes 7.4 us with eight blocks per row, 8.7
 // with four; policy 100 x 130000 31.4 and 27.5, 320 x 130000 73 and 77, 320 x 32000 27.3 with two and 24.2 with one.
 template <bool Policy, bool Entropy, bool Aligned>
@@ -1164,7 +1166,8 @@ static int launch_bwd(const BwdArgs& b)
 }
 
 // Pieces of a row for 8 lanes, a warp or a block: a piece must be nearly full and its loads all under way at once; those of a gradient
-// that is added to are as many again.  Measured (us, stored / added to, 65536 rows: 200 columns by 8 lanes 20.3 / 26.6, by a warp 27.0 / 34.3,
+// that is added to are as many again.  Measured (us, stored / added to, 65536 rows: 30 columns by 8 lanes with one quad 6.4, with two 7.8,
+// 200 columns by 8 lanes 20.3 / 26.6, by a warp 27.0 / 34.3,
 // 400 37.0 / 47.8 and 35.9 / 46.4, 1100 by warps with 4 quads 95.9 / 124, with 8 93.1 / 140, by blocks 121 / 174; 30000 x 4101: 163 / 229,
 // 149 / 245, 191 / 289; 20000 x 6200 with 4 quads 149, with 8 145, by blocks 154; 4000 x 32003: 160 / 215, 149 / 216, 150 / 210).
 template <bool Accumulate, bool Aligned>
@@ -1269,8 +1272,10 @@ int znn_preference_loss(const float* logp, const float* ref_logp, const int32_t*
 #define ZNN_PAIRS(small, threads, blocks, used, ranks)                                                                                    \
     launch_overlapped(preference_pair_kernel<small, threads>, "preference_pair_kernel", blocks, used, ranks, logp, ref_logp, targets, seq_offsets, \
            beta, label_smoothing, margin, length_normalize, loss, pair_loss, rewards, dlogp, P, M, device_status_word())
-    // A warp per pair in one launch for small calls.  Few pairs of long sequences: eight blocks each, where one block's own bandwidth
-    // (about 100 GB/s) would be the limit.  Many short ones: small blocks.
+    // A warp per pair in one launch for small calls: 32 pairs of 256 rows 5.2 us, 8 of 1024 5.5, where the next forms' two launches take 6.1
+    // (32 x 260, 16 x 520).  (The limit counts the call's rows.  One to four pairs that fill it are slower this way: 4 x 2048 7.6 us, 2 x
+    // 4096 13.3, 1 x 8192 24.7, against 6.1 for 4 x 4096 and 7.4 for 2 x 8192.)  Few pairs of long sequences: eight blocks each, where one
+    // block's own bandwidth (about 100 GB/s) would be the limit.  Many short ones: small blocks.
     if (P <= 32 && M <= 8192) return ZNN_PAIRS(true, 1024, 1, 32 * P, 1);
     const int rows = M / P;
     const int rc = rows > 8192 && P <= 32              ? ZNN_PAIRS(false, 1024, 8LL * P, 1024, 8)
