@@ -275,3 +275,57 @@ MANY = [(450, 1100), (520, 1501), (450, 2000), (451, 2100), (450, 2900), (450, 5
 @pytest.mark.parametrize("kl,weighted,inv_temp", [(0.0, False, 1.0), (0.05, False, 1.25), (0.1, True, 0.7)])
 def test_policy_loss_without_entropies(ops, M, N, kl, weighted, inv_temp):
     base.test_policy_loss(WithoutEntropies(ops), M, N, kl, 0.0, weighted, inv_temp)
+
+
+# ------------------------------------------------------------------ rows of every kind in one call
+@pytest.mark.parametrize("N", [1, 7, 31, 33, 64, 65, 100, 128, 129, 200, 257, 384, 385, 513, 700, 1025, 5000, 9001])
+@pytest.mark.parametrize("accumulate,in_place", [(False, False), (True, False), (False, True)])
+@pytest.mark.parametrize("shift", [0, 1])
+def test_gradients_of_rows_among_others_and_alone(ops, L, N, accumulate, in_place, shift):
+    """Nearly certain rows, others, rows that are left out, empty ones and bad targets share warps: each gives the bits that it gives
+    alone, and the floats between the rows and behind the last one stay."""
+    r = np.random.default_rng(N * 2 + shift)
+    M, ld = 75, N + (3 if shift else 4)
+    x = (r.standard_normal((M, N)) * 2).astype(np.float32)
+    t = r.integers(0, N, M).astype(np.int32)
+    certain = r.random(M) < 0.4
+    x[certain, r.integers(0, N, M)[certain]] += 30.0
+    target_at_top = r.random(M) < 0.7
+    t[target_at_top] = x.argmax(1)[target_at_top]
+    x[r.random(M) < 0.05] = -INF
+    t[r.random(M) < 0.15] = -1
+    t[r.random(M) < 0.05] = N + 3
+    g, h = r.standard_normal(M).astype(np.float32), r.standard_normal(M).astype(np.float32)
+    logp, ent, stats = ops.token_logprob_fwd(x, t)
+    base.status(L)
+    up = ops.DevBuf.from_host
+
+    def spread(a):
+        buf = np.full(shift + M * ld + 16, 77.0, np.float32)
+        for i in range(M):
+            buf[shift + i * ld:shift + i * ld + N] = a[i]
+        return buf
+    hx, before = spread(x), spread(r.standard_normal((M, N)).astype(np.float32))
+    tb, sb, gb, hb, eb = up(t), up(stats), up(g), up(h), up(ent)
+
+    def run(xb, db, first, rows, entropy):
+        L.call("znn_token_logprob_bwd", xb.ptr + 4 * (shift + first * ld), ld, tb.ptr + 4 * first, 1.0, sb.ptr + 8 * first, eb.ptr + 4 * first if entropy else None,
+               gb.ptr + 4 * first, hb.ptr + 4 * first if entropy else None, db.ptr + 4 * (shift + first * ld), ld, int(accumulate), rows, N)
+    for entropy in (False, True):
+        x1, x2, d1, d2 = up(hx), up(hx), up(before), up(before)
+        a, b = (x1, x2) if in_place else (d1, d2)
+        run(x1, a, 0, M, entropy)
+        for i in range(M):
+            run(x2, b, i, 1, entropy)
+        together, alone = a.to_host(hx.shape), b.to_host(hx.shape)
+        np.testing.assert_array_equal(together, alone)
+        rest = together.copy()
+        for i in range(M):
+            row = rest[shift + i * ld:shift + i * ld + N]
+            assert np.all(np.isfinite(row))
+            if not 0 <= t[i] < N or stats[i, 1] == 0:
+                np.testing.assert_array_equal(row, before[shift + i * ld:shift + i * ld + N] if accumulate else 0.0)
+            row[:] = 77.0
+        assert np.all(rest == 77.0)
+        if not in_place:
+            np.testing.assert_array_equal(x1.to_host(hx.shape), hx)

@@ -2,7 +2,7 @@
 // with its gradient, the preference loss on pairs of sequences.  Formulas: include/znn_cuda.h.
 //
 // Bound by HBM where there is enough to do (10 to 20 operations per logit against 4 to 12 bytes), by launch and reduction latency
-// where there is not.  Measured on B200s whose copies run at 6548 GB/s, the whole call, inputs in turn from three sets, several boxes:
+// where there is not.  Measured on B200s whose copies run at 6548 GB/s, the whole call, inputs in turn from three sets, on several devices:
 //   log-probabilities and entropies 2045 x 50257, a fifth left out  57 - 62 us   5.3 - 5.7 TB/s   (floor 50 us)
 //   their gradient with entropy term 8192 x 8192, a tenth left out  78 - 79 us   6.4 TB/s         (78 us)
 //   policy loss 8192 x 8192, KL term                                94 - 96 us   5.7 TB/s         (82 us)
